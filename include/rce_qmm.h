@@ -353,6 +353,130 @@ rce_qmm_status rce_qmm_llama_forward_token_dev(rce_qmm_llama *m, const int32_t *
  * only the steps that ran). */
 rce_qmm_status rce_qmm_llama_check(rce_qmm_llama *m);
 
+/* ---- paged 8-bit KV cache, attention over it, sampling -------------------- */
+
+/* No counterpart in the reference, whose runtimes hold one sequence's keys
+ * and values in f32 (TinyLlamaState, rce-tinyllama/src/lib.rs L144-155): a
+ * cache for many sequences that a program steps with rce_qmm_mm_batched_dev.
+ * The caller owns the pool (device memory) and describes it here.
+ *
+ * A page holds page_tokens (16 .. 4096, a power of two) positions of every kv
+ * head.  Values are 8-bit codes, -127 .. 127, times one f32 scale per block
+ * of 16 positions and kv head, keys and values apart.  With B = page_tokens /
+ * 16, block b = position % page_tokens / 16 and slot i = position % 16 of
+ * page p, head h:
+ *   k code of dimension d  k[(((p * n_kv_heads + h) * B + b) * 16 + i) * d_head + d]
+ *   v code of dimension d  v[(((p * n_kv_heads + h) * B + b) * d_head + d) * 16 + i]
+ *   scales                 k_scale, v_scale[(p * n_kv_heads + h) * B + b]
+ * d_head: 64, 128, 192 or 256.  k and v 16-byte aligned, the scales 4. */
+typedef struct rce_qmm_kv_cache {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    size_t n_pages, page_tokens, n_kv_heads, d_head;
+} rce_qmm_kv_cache;
+
+/* Bytes of k (and of v) and the count of k_scale (and of v_scale). */
+rce_qmm_status rce_qmm_kv_sizes(const rce_qmm_kv_cache *cache, size_t *code_bytes, size_t *n_scales);
+
+/* The rows of a call and the sequences they belong to (device arrays).  Rows
+ * row_offsets[s] .. row_offsets[s + 1] - 1 (n_seqs + 1 ascending offsets; rows
+ * behind the last are no sequence's) are the newest positions of sequence s:
+ * row r stands at position seq_lens[s] - (row_offsets[s + 1] - r), so
+ * seq_lens counts the rows themselves.  Position p lies in page
+ * pages[s * max_pages + p / page_tokens].  A row whose position is negative or
+ * not below max_pages * page_tokens, and a position whose page id is outside
+ * the pool, are left out: not written, not read, not attended to. */
+typedef struct rce_qmm_kv_batch {
+    const int32_t *row_offsets, *seq_lens, *pages;
+    size_t n_seqs, n_rows, max_pages;
+} rce_qmm_kv_batch;
+
+/* The rotation of positions 0 .. n_pos - 1 (device): cs[n_pos][dim / 2][2] =
+ * (cos, sin); the pairs (i, i + dim / 2) of a head's first dim values turn to
+ * (a cos - b sin, a sin + b cos) (rope_inplace, rce-op-attn/src/lib.rs
+ * L107-151), one binary32 rounding per operation.  n_pos must be at least
+ * max_pages * page_tokens of the batch. */
+typedef struct rce_qmm_rope {
+    const float *cs;
+    size_t dim, n_pos;
+} rce_qmm_rope;
+
+/* The decoder's rotation table on the host: cs[n_pos * dim / 2 * 2] by the C
+ * library's logf / expf / cosf / sinf in the reference's order. */
+rce_qmm_status rce_qmm_rope_table(float freq_base, size_t dim, size_t n_pos, float *cs);
+
+/* Append n_rows rows of keys and values to their sequences' pages; the keys
+ * are rotated on the way (rope NULL: as they are).  k_dev [n_rows][n_kv_heads *
+ * d_head] with k_stride values from row to row (v likewise; slices of one
+ * fused projection are fine), dtype F32, F16 or BF16.
+ * Per block: d = max|x| / 127 over its new rows (0 where that is below
+ * 2^-126), scale = d where the call writes the block's first slot, else
+ * max(the block's scale, d); codes rint(x * (1 / scale)); where a block's scale
+ * grew, the codes of its earlier slots become rint(q * (old scale / scale)).
+ * Slots behind the new rows keep their bytes.  A block that gets an infinite
+ * or NaN value has that scale and codes 0 and reads as NaN until its first
+ * slot is written again.  No block may be written for two sequences in one
+ * call.  n_rows at most 2^27. */
+rce_qmm_status rce_qmm_kv_append_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                     const rce_qmm_kv_batch *batch, const void *k_dev, size_t k_stride,
+                                     const void *v_dev, size_t v_stride, uint32_t dtype, const rce_qmm_rope *rope,
+                                     void *stream);
+
+/* The cached values (code * scale, rounded to dtype F32, F16 or BF16) of the
+ * batch's rows into k_out, v_out [n_rows][n_kv_heads][d_head] (either may be
+ * NULL); what rce_qmm_dequant_row is to a weight.  Rows left out keep their
+ * bytes. */
+rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache, const rce_qmm_kv_batch *batch,
+                                   void *k_out, void *v_out, uint32_t dtype, void *stream);
+
+/* Causal attention of n_rows query rows over the cache, their own positions
+ * (appended before) included: for query head h of row r at position p, kv head
+ * g = h / (n_q_heads / n_kv_heads) (fused_attend_head_window, rce-op-attn
+ * L196-251, by softmax over all keys at once),
+ *   out = sum_j softmax_j(scale * q' . k_j) v_j,  j = max(0, p - window + 1) .. p
+ * (window 0: from 0), q' the rotated q (rope NULL: q).  A row that sees no
+ * key, or is left out, gives zeros; rows behind row_offsets[n_seqs] keep their
+ * bytes.  q_dev [n_rows][n_q_heads * d_head] with q_stride values from row to
+ * row, q_dtype F32, F16 or BF16; out_dev likewise with out_stride, out_dtype.
+ * scale >= 0 and finite.
+ * Numerics: q' as whole numbers of 15 bits (out_dtype F32: 22 bits) of its
+ * head's largest value against the 8-bit key codes in exact int32 products
+ * on the matrix cores; softmax in f32; its weights rounded to binary16 (out_dtype
+ * F32: two binary16 terms) against the value codes, f32 sums.  Fixed order for
+ * a batch: run-to-run bit-identical; a row's last bits depend on the batch.
+ * Calls that split long sequences use a buffer allocated with the context. */
+rce_qmm_status rce_qmm_kv_attention_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                        const rce_qmm_kv_batch *batch, const void *q_dev, uint32_t q_dtype,
+                                        size_t q_stride, size_t n_q_heads, const rce_qmm_rope *rope, float scale,
+                                        size_t window, void *out_dev, uint32_t out_dtype, size_t out_stride,
+                                        void *stream);
+
+/* How the rows of rce_qmm_sample_dev are sampled: device arrays of one value
+ * per row; NULL turns a filter off (temperature: 1). */
+typedef struct rce_qmm_sampling {
+    const float *u;            /* uniform numbers in [0, 1), not NULL */
+    const float *temperature;  /* not above 0 (or NaN): the most likely token */
+    const int32_t *top_k;      /* <= 0: off */
+    const float *top_p;        /* >= 1 (or NaN): off; <= 0: the most likely token */
+    const float *min_p;        /* <= 0 (or NaN): off */
+} rce_qmm_sampling;
+
+/* One token per row from logits_dev [n_rows][vocab] (row_stride values from
+ * row to row; F32, F16 or BF16), without a host round trip (the reference
+ * samples on the host).  w_i = exp((l_i - max l) / temperature) (1 at the
+ * maximum); NaN and -inf have no weight.  In the order of falling l, the lower id
+ * first among equals: keep the first top_k; of these the shortest run whose
+ * weights sum to at least top_p of theirs; of these the ones with w >= min_p;
+ * the first always.  ids_dev[r] = the lowest id i for which the kept weights
+ * of ids 0 .. i sum to more than u times their total; probs_dev[r] (may be
+ * NULL) = its share of that total.  A row without any weight gives id -1,
+ * probability 0.  vocab at most 2^24.
+ * Weights are double-precision exponentials as whole numbers (the largest weight
+ * is 2^(62 - ceil(log2 vocab))), so every sum is exact in any order: run-to-run identical. */
+rce_qmm_status rce_qmm_sample_dev(rce_qmm_context *ctx, const void *logits_dev, uint32_t dtype, size_t n_rows,
+                                  size_t vocab, size_t row_stride, const rce_qmm_sampling *sampling, int32_t *ids_dev,
+                                  float *probs_dev, void *stream);
+
 /* ---- the "hip:op-qmm" priced backend (rce-placement-adapter) ------------- */
 
 /* The adapter's qmm dtype ids (QMM_DTYPE_*, rce-placement-adapter/src/lib.rs

@@ -55,6 +55,12 @@ SIGNATURES = {
     "rce_qmm_gguf_find_tensor": (STATUS, [P, ctypes.c_char_p, P]),
     "rce_qmm_weight_from_gguf": (STATUS, [P, P, ctypes.c_char_p, S, S, P]),
     "rce_qmm_gguf_read_f32": (STATUS, [P, ctypes.c_char_p, P, S]),
+    "rce_qmm_kv_sizes": (STATUS, [P, P, P]),
+    "rce_qmm_rope_table": (STATUS, [F, S, S, P]),
+    "rce_qmm_kv_append_dev": (STATUS, [P, P, P, P, S, P, S, U32, P, P]),
+    "rce_qmm_kv_read_dev": (STATUS, [P, P, P, P, P, U32, P]),
+    "rce_qmm_kv_attention_dev": (STATUS, [P, P, P, P, U32, S, S, P, F, S, P, U32, S, P]),
+    "rce_qmm_sample_dev": (STATUS, [P, P, U32, S, S, S, P, P, P, P]),
     "rce_qmm_dtype_for_qmm_id": (U32, [S]),
     "rce_qmm_hip_cost_prior": (None, [P, P, P]),
     "rce_qmm_hip_cost": (STATUS, [P, S, P, S, ctypes.c_double, ctypes.c_double, ctypes.c_double, P]),

@@ -71,6 +71,9 @@ struct rce_qmm_context {
     // needs, allocated with the context and never moved, so a call recorded
     // into a graph stays valid whatever calls follow it.
     rce_qmm_abi::Scratch parts;
+    // Partial results of attention's split key ranges: kv_attention_parts_bytes(),
+    // as parts.
+    rce_qmm_abi::Scratch kv_parts;
     rce_qmm_abi::Scratch act_q;  // several tokens' Q8 activations, quantized once per launch
     // grouped experts: grouping metadata, expert tables, stage buffers
     rce_qmm_abi::Scratch moe_meta, moe_wtab, moe_x, moe_h, moe_h16, moe_y, moe_u;
@@ -131,6 +134,12 @@ size_t batched_scratch_bytes(const DevWeight &dw, uint32_t a_dtype, size_t t_row
 // Resolve the device address of the no-allocation entry point's fixed
 // scratch on `device` (the current device), once per device (noalloc.hip).
 rce_qmm_status noalloc_setup(int device);
+
+// cs[n_pos][dim / 2][2] = (cos, sin) of the position times the pair's
+// frequency, by the C library in the order of rope_inplace_scaled
+// (rce-op-attn/src/lib.rs L115-151): inv_freq = 1 / exp(ln(base) * (2i) /
+// dim), theta = pos * inv_freq (kv_abi.cpp).
+void fill_rope_table(float freq_base, size_t dim, size_t n_pos, float *cs);
 
 inline rce_qmm_status check_weight_ctx(rce_qmm_context *ctx, const rce_qmm_weight *w) {
     if (!ctx || !w) return fail(RCE_QMM_NULL_ARGUMENT, "null context or weight");

@@ -381,23 +381,8 @@ rce_qmm_status rce_qmm_llama_create(rce_qmm_context *ctx, const rce_qmm_llama_co
         std::memcpy(&norms[(2 * il + 1) * dm], blocks[il].ffn_norm, dm * sizeof(float));
     }
     std::memcpy(&norms[2 * c.n_layers * dm], output_norm, dm * sizeof(float));
-    // rope_inplace_scaled (rce-op-attn/src/lib.rs L115-151), per position
-    // and pair i: inv_freq = 1 / exp(ln(base) * (2i) / rope_dim), theta =
-    // pos * inv_freq, with the C library's logf / expf / sinf / cosf.
     std::vector<float> cs(c.context_length * std::max<size_t>(half, 1) * 2, 0.0f);
-    const float log_base = logf(c.rope_freq_base);
-    std::vector<float> inv_freq(half);
-    for (size_t i = 0; i < half; i++) {
-        float ex = log_base * (2.0f * (float)i);
-        ex = ex / (float)c.rope_dim;
-        inv_freq[i] = 1.0f / expf(ex);
-    }
-    for (size_t p = 0; p < c.context_length; p++)
-        for (size_t i = 0; i < half; i++) {
-            const float theta = (float)p * inv_freq[i];
-            cs[(p * half + i) * 2] = cosf(theta);
-            cs[(p * half + i) * 2 + 1] = sinf(theta);
-        }
+    fill_rope_table(c.rope_freq_base, c.rope_dim, c.context_length, cs.data());
     hipStream_t s = ctx->stream;
     if ((e = hipMemcpyAsync(m->norms, norms.data(), norms.size() * sizeof(float), hipMemcpyHostToDevice, s)) ||
         (e = hipMemcpyAsync(m->rope_cs, cs.data(), cs.size() * sizeof(float), hipMemcpyHostToDevice, s)) ||

@@ -6,6 +6,7 @@
 // exception crosses the ABI; failures set a thread-local message
 // (rce_qmm_last_error), the convention of compute/crates/rce-c/include/rce.h.
 #include "abi_internal.h"
+#include "kv_cache.h"
 #include "lds_limit.h"
 
 #include <algorithm>
@@ -342,7 +343,8 @@ rce_qmm_status rce_qmm_context_create(int device, rce_qmm_context **out) {
     }
     c->device = device;
     c->stream = s;
-    if ((st = ensure(c, c->parts, rce_qmm::gemm_f16_parts_bytes(), nullptr))) {
+    if ((st = ensure(c, c->parts, rce_qmm::gemm_f16_parts_bytes(), nullptr)) ||
+        (st = ensure(c, c->kv_parts, rce_qmm::kv_attention_parts_bytes(), nullptr))) {
         context_release(c);
         return st;
     }
@@ -360,7 +362,7 @@ void rce_qmm_abi::context_release(rce_qmm_context *ctx) {
     if (ctx->refs.fetch_sub(1) != 1) return;
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
-    for (Scratch *s : {&ctx->a_in, &ctx->a_f32, &ctx->out, &ctx->a_f16, &ctx->parts, &ctx->act_q, &ctx->moe_meta, &ctx->moe_wtab, &ctx->moe_x,
+    for (Scratch *s : {&ctx->a_in, &ctx->a_f32, &ctx->out, &ctx->a_f16, &ctx->parts, &ctx->kv_parts, &ctx->act_q, &ctx->moe_meta, &ctx->moe_wtab, &ctx->moe_x,
                        &ctx->moe_h, &ctx->moe_h16, &ctx->moe_y, &ctx->moe_u})
         if (s->p) (void)hipFree(s->p);
     if (ctx->moe_grouped) (void)hipEventDestroy(ctx->moe_grouped);
