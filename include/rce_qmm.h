@@ -422,8 +422,8 @@ rce_qmm_status rce_qmm_kv_append_dev(rce_qmm_context *ctx, const rce_qmm_kv_cach
                                      const void *v_dev, size_t v_stride, uint32_t dtype, const rce_qmm_rope *rope,
                                      void *stream);
 
-/* The cached values (code * scale, rounded to dtype F32, F16 or BF16) of the
- * batch's rows into k_out, v_out [n_rows][n_kv_heads][d_head] (either may be
+/* The cached values (code * scale in f32, then rounded to dtype F32, F16 or
+ * BF16) of the batch's rows into k_out, v_out [n_rows][n_kv_heads][d_head] (either may be
  * NULL); what rce_qmm_dequant_row is to a weight.  Rows left out keep their
  * bytes. */
 rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache, const rce_qmm_kv_batch *batch,

@@ -240,8 +240,12 @@ __global__ __launch_bounds__(256) void k_kv_append(KvPool P, KvRows B, const T *
     else append_keys<T, D, false>(P, t, k + (size_t)h * D, k_stride, rope);
 }
 
+// x, a product rounded to f32, in T: the empty asm keeps the two roundings
+// apart (else product and conversion become one v_fma_mix instruction, in
+// some places and not in others).
 template <class T>
 __device__ __forceinline__ T narrow(float x) {
+    asm("" : "+v"(x));
     return (T)x;
 }
 template <>

@@ -164,6 +164,28 @@ def test_read(ctx, d, dtype):
     dev.free()
 
 
+@pytest.mark.parametrize("dtype", [G.F16, G.BF16])
+def test_read_rounds_the_f32_product(ctx, dtype):
+    """A million values: about one in 30000 tells the product rounded to f32 and
+    then to 16 bits from the product rounded once."""
+    rng = np.random.default_rng(2)
+    rows = 4096
+    batch, n_pages = kc.make_batch(rng, [rows], [rows], 64)
+    pool = kc.Pool(n_pages, 64, 2, 128, rng)
+    dev = kc.Device(ctx, pool, batch)
+    out = [rce_amd.DeviceBuffer(ctx, rows * 256 * 2) for _ in range(2)]
+    rce_amd.kv_read_dev(ctx, dev.cache, dev.b, out[0].ptr, out[1].ptr, dtype)
+    ctx.synchronize()
+    pg = batch.pages[0]
+    k = pool.k[pg].astype(F32) * pool.k_scale[pg][..., None, None]  # [pages, heads, blocks, 16, d]
+    v = pool.v[pg].transpose(0, 1, 2, 4, 3).astype(F32) * pool.v_scale[pg][..., None, None]
+    for o, x in zip(out, (k, v)):
+        want = kc.to_bits(x.transpose(0, 2, 3, 1, 4).reshape(-1), dtype)
+        assert np.array_equal(o.download(kc.np_type(dtype), rows * 256).view(np.uint16), want.view(np.uint16))
+        o.free()
+    dev.free()
+
+
 # ---- attention --------------------------------------------------------------------
 
 class Attn:
