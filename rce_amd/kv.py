@@ -7,6 +7,7 @@ asynchronous on the given stream (None: the context's); there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
@@ -16,47 +17,48 @@ from .qmm import Context, DeviceBuffer, _ptr
 __all__ = ["KvCache", "KvBatch", "Rope", "kv_append_dev", "kv_read_dev", "kv_attention_dev", "sample_dev"]
 
 
-class _Cache(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
-               [(n, ctypes.c_size_t) for n in ("n_pages", "page_tokens", "n_kv_heads", "d_head")]
+# The header's structs as bytes: made once per object, passed as they are (a
+# decode step makes several calls of a few microseconds each).
+_CACHE = struct.Struct("@PPPPNNNN")
+_BATCH = struct.Struct("@PPPNNN")
+_ROPE = struct.Struct("@PNN")
+_SAMPLING = struct.Struct("@PPPPP")
 
 
-class _Batch(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("row_offsets", "seq_lens", "pages")] + \
-               [(n, ctypes.c_size_t) for n in ("n_seqs", "n_rows", "max_pages")]
-
-
-class _Rope(ctypes.Structure):
-    _fields_ = [("cs", ctypes.c_void_p), ("dim", ctypes.c_size_t), ("n_pos", ctypes.c_size_t)]
-
-
-class _Sampling(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("u", "temperature", "top_k", "top_p", "min_p")]
+def _pack(fmt: struct.Struct, *values: int) -> bytes:
+    try:
+        return fmt.pack(*values)
+    except struct.error as e:
+        raise QmmError(2, f"an address or a size is out of range: {e}") from None
 
 
 class KvCache:
     """A pool of pages (rce_qmm_kv_cache): device addresses of the key and
     value codes and their scales, in the layout the header gives."""
 
+    __slots__ = ("raw", "d_head", "buffers")
+
     def __init__(self, n_pages: int, page_tokens: int, n_kv_heads: int, d_head: int, k: int = 0, v: int = 0,
                  k_scale: int = 0, v_scale: int = 0):
-        self.c = _Cache(k or None, v or None, k_scale or None, v_scale or None, n_pages, page_tokens, n_kv_heads, d_head)
+        self.raw = _pack(_CACHE, k, v, k_scale, v_scale, n_pages, page_tokens, n_kv_heads, d_head)
+        self.d_head = d_head
         self.buffers: tuple = ()
 
     @classmethod
     def allocate(cls, ctx: Context, n_pages: int, page_tokens: int, n_kv_heads: int, d_head: int) -> "KvCache":
         """A pool in device memory of its own (contents undefined), freed by
         ``free`` or with the object."""
-        c = cls(n_pages, page_tokens, n_kv_heads, d_head)
-        codes, scales = c.sizes()
-        c.buffers = tuple(DeviceBuffer(ctx, n) for n in (codes, codes, 4 * scales, 4 * scales))
-        c.c.k, c.c.v, c.c.k_scale, c.c.v_scale = (b.ptr for b in c.buffers)
+        shape = (n_pages, page_tokens, n_kv_heads, d_head)
+        codes, scales = cls(*shape).sizes()
+        buffers = tuple(DeviceBuffer(ctx, n) for n in (codes, codes, 4 * scales, 4 * scales))
+        c = cls(*shape, *(b.ptr for b in buffers))
+        c.buffers = buffers
         return c
 
     def sizes(self) -> tuple[int, int]:
         """(bytes of the key codes, and of the value codes; scales of each)."""
         b, n = ctypes.c_size_t(), ctypes.c_size_t()
-        check(lib().rce_qmm_kv_sizes(ctypes.byref(self.c), ctypes.byref(b), ctypes.byref(n)))
+        check(lib().rce_qmm_kv_sizes(self.raw, ctypes.byref(b), ctypes.byref(n)))
         return b.value, n.value
 
     def free(self) -> None:
@@ -70,15 +72,19 @@ class KvBatch:
     addresses of row_offsets [n_seqs + 1], seq_lens [n_seqs] and pages
     [n_seqs][max_pages], all int32."""
 
+    __slots__ = ("raw",)
+
     def __init__(self, row_offsets: int, seq_lens: int, pages: int, n_seqs: int, n_rows: int, max_pages: int):
-        self.c = _Batch(row_offsets or None, seq_lens or None, pages or None, n_seqs, n_rows, max_pages)
+        self.raw = _pack(_BATCH, row_offsets, seq_lens, pages, n_seqs, n_rows, max_pages)
 
 
 class Rope:
     """A rotation table on the device (rce_qmm_rope)."""
 
+    __slots__ = ("raw", "buffer")
+
     def __init__(self, cs: int, dim: int, n_pos: int):
-        self.c = _Rope(cs or None, dim, n_pos)
+        self.raw = _pack(_ROPE, cs, dim, n_pos)
         self.buffer: DeviceBuffer | None = None
 
     @staticmethod
@@ -98,26 +104,26 @@ class Rope:
         return r
 
 
-def _p(a: int | None) -> ctypes.c_void_p:
-    return ctypes.c_void_p(a or None)
-
-
-def _ref(x):
-    return ctypes.byref(x.c) if x is not None else None
+def _raw(x) -> bytes | None:
+    return None if x is None else x.raw
 
 
 def kv_append_dev(ctx: Context, cache: KvCache, batch: KvBatch, k_dev: int, v_dev: int, dtype, k_stride: int,
                   v_stride: int, rope: Rope | None = None, stream: int | None = None) -> None:
     """Quantize and append the batch's rows of keys (rotated) and values
     (rce_qmm_kv_append_dev); strides in values from row to row."""
-    check(lib().rce_qmm_kv_append_dev(ctx.handle, _ref(cache), _ref(batch), _p(k_dev), k_stride, _p(v_dev), v_stride,
-                                      int(dtype), _ref(rope), _p(stream)))
+    st = lib().rce_qmm_kv_append_dev(ctx.handle, _raw(cache), _raw(batch), k_dev, k_stride, v_dev, v_stride, dtype,
+                                     _raw(rope), stream)
+    if st:
+        check(st)
 
 
 def kv_read_dev(ctx: Context, cache: KvCache, batch: KvBatch, k_out: int | None, v_out: int | None, dtype,
                 stream: int | None = None) -> None:
     """The cached values of the batch's rows (rce_qmm_kv_read_dev)."""
-    check(lib().rce_qmm_kv_read_dev(ctx.handle, _ref(cache), _ref(batch), _p(k_out), _p(v_out), int(dtype), _p(stream)))
+    st = lib().rce_qmm_kv_read_dev(ctx.handle, _raw(cache), _raw(batch), k_out, v_out, dtype, stream)
+    if st:
+        check(st)
 
 
 def kv_attention_dev(ctx: Context, cache: KvCache, batch: KvBatch, q_dev: int, q_dtype, q_stride: int, n_q_heads: int,
@@ -125,9 +131,12 @@ def kv_attention_dev(ctx: Context, cache: KvCache, batch: KvBatch, q_dev: int, q
                      out_stride: int | None = None, stream: int | None = None) -> None:
     """Causal attention of the batch's query rows over the cache
     (rce_qmm_kv_attention_dev); out_stride None: rows without gaps."""
-    check(lib().rce_qmm_kv_attention_dev(ctx.handle, _ref(cache), _ref(batch), _p(q_dev), int(q_dtype), q_stride, n_q_heads,
-                                         _ref(rope), scale, window, _p(out_dev), int(out_dtype),
-                                         n_q_heads * cache.c.d_head if out_stride is None else out_stride, _p(stream)))
+    if out_stride is None and cache is not None:
+        out_stride = n_q_heads * cache.d_head
+    st = lib().rce_qmm_kv_attention_dev(ctx.handle, _raw(cache), _raw(batch), q_dev, q_dtype, q_stride, n_q_heads, _raw(rope),
+                                        scale, window, out_dev, out_dtype, out_stride or 0, stream)
+    if st:
+        check(st)
 
 
 def sample_dev(ctx: Context, logits_dev: int, dtype, n_rows: int, vocab: int, row_stride: int, u_dev: int, ids_dev: int,
@@ -135,6 +144,7 @@ def sample_dev(ctx: Context, logits_dev: int, dtype, n_rows: int, vocab: int, ro
                top_p_dev: int | None = None, min_p_dev: int | None = None, stream: int | None = None) -> None:
     """One token per row from its logits and its uniform number
     (rce_qmm_sample_dev); a filter without an array is off."""
-    s = _Sampling(u_dev or None, temperature_dev or None, top_k_dev or None, top_p_dev or None, min_p_dev or None)
-    check(lib().rce_qmm_sample_dev(ctx.handle, _p(logits_dev), int(dtype), n_rows, vocab, row_stride, ctypes.byref(s),
-                                   _p(ids_dev), _p(probs_dev), _p(stream)))
+    s = _pack(_SAMPLING, u_dev or 0, temperature_dev or 0, top_k_dev or 0, top_p_dev or 0, min_p_dev or 0)
+    st = lib().rce_qmm_sample_dev(ctx.handle, logits_dev, dtype, n_rows, vocab, row_stride, s, ids_dev, probs_dev, stream)
+    if st:
+        check(st)

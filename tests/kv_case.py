@@ -236,11 +236,16 @@ class Device:
                      up(np.asarray(batch.lens, np.int32)), up(batch.pages)]
         k, v, ks, vs, off, ln, pg = (b.ptr for b in self.bufs)
         self.cache = rce_amd.KvCache(pool.n_pages, pool.page, pool.heads, pool.d, k=k, v=v, k_scale=ks, v_scale=vs)
-        self.b = rce_amd.KvBatch(off, ln, pg, len(batch.lens), batch.n_rows, batch.pages.shape[1])
+        self.at = (off, ln, pg)
+        self.rows(batch.n_rows)
         self.rope = None
         if cs is not None:
             self.bufs.append(up(cs))
             self.rope = rce_amd.Rope(self.bufs[-1].ptr, cs.shape[1] * 2, cs.shape[0])
+
+    def rows(self, n):
+        """The batch with n rows."""
+        self.b = rce_amd.KvBatch(*self.at, len(self.batch.lens), n, self.batch.pages.shape[1])
 
     def download(self):
         p = self.pool.copy()

@@ -125,7 +125,7 @@ def test_append_token_by_token(ctx, d, heads, page, dtype):
         b = kc.Batch([at, at], [m, m], full.pages, page)
         for buf, a in zip(dev.bufs[4:6], (b.offsets, np.asarray(b.lens, np.int32))):
             buf.upload(a)
-        dev.b.c.n_rows = b.n_rows
+        dev.rows(b.n_rows)
         raw, stride, ka, va, k, v = fused(rng, b.n_rows, heads, d, dtype)
         run_append(ctx, dev, raw, stride, ka, va, dtype)
         kc.append(want, b, k, v, cs)

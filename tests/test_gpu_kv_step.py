@@ -45,7 +45,7 @@ def test_step(ctx):
         rows = b.n_rows
         dev.bufs[4].upload(b.offsets)
         dev.bufs[5].upload(np.asarray(lens, np.int32))
-        dev.b.c.n_rows = rows
+        dev.rows(rows)
         xin = embd[tokens]
         x.upload(xin)
         uu = rng.random(n).astype(F32)
