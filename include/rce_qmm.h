@@ -471,8 +471,9 @@ typedef struct rce_qmm_sampling {
  * of ids 0 .. i sum to more than u times their total; probs_dev[r] (may be
  * NULL) = its share of that total.  A row without any weight gives id -1,
  * probability 0.  vocab at most 2^24.
- * Weights are double-precision exponentials as whole numbers (the largest weight
- * is 2^(62 - ceil(log2 vocab))), so every sum is exact in any order: run-to-run identical. */
+ * Weights are exponentials to 2^-46 as whole numbers, the largest 2^S, S = min(50,
+ * 62 - ceil(log2 vocab)), so every sum is exact in any order: run-to-run
+ * identical. */
 rce_qmm_status rce_qmm_sample_dev(rce_qmm_context *ctx, const void *logits_dev, uint32_t dtype, size_t n_rows,
                                   size_t vocab, size_t row_stride, const rce_qmm_sampling *sampling, int32_t *ids_dev,
                                   float *probs_dev, void *stream);

@@ -2,65 +2,91 @@
 // the draw from given uniform numbers (include/rce_qmm.h rce_qmm_sample_dev).
 //
 // A block per row.  Weights are whole numbers, rint(exp((l - max) / T) 2^S)
-// with S = 62 - ceil(log2 vocab): a row's sum fits 63 bits, every sum is exact
-// and no order of additions matters, so histograms by LDS atomics are
-// deterministic.
-// The filters keep a prefix of the order (l falling, id rising), which a
-// threshold says: keys above `key`, and the first `ties` ids at `key`.  It
-// is found by radix descent over the order-preserving bits of l, 8 at a
-// time: by counts for top-k, by weights for top-p.
+// with S = min(50, 62 - ceil(log2 vocab)): a row's sum fits 63 bits, every sum
+// is exact and no order of additions matters, so the histograms, made with LDS
+// atomics, are deterministic.
+//
+// The filters keep a prefix of the order (l falling, id rising): it is told by
+// its last element, a 64-bit number ~key(l) << 32 | id that is smaller or equal for what
+// is kept (key: the bits of l in an order-preserving form).  To find it, a
+// histogram over BINS equal intervals of l says which bin holds the end (by
+// counts for top-k, by weights for top-p); that bin's elements are collected,
+// sorted, and cut where the count or the sum is reached.  A bin of more than NT
+// elements (many equal logits) goes through a radix descent over the 64-bit
+// numbers instead, 8 bits a pass.
+//
+// The draw: each wave owns runs of q * 64 consecutive ids (run r of the row
+// belongs to wave r % 16); the runs' kept weights are summed and scanned, and the
+// wave whose run the draw falls into walks it.
+//
+// What bounds it: one CU per row, so the row's passes (two to six, from
+// registers up to 32768 ids, else from L2) and their double-precision exponentials,
+// which only elements that a pass keeps pay for.
 #include "kv_cache.h"
+
+#include <type_traits>
 
 namespace rce_qmm {
 namespace {
 
-constexpr int NT = 1024, NW = NT / 64;
-
 typedef unsigned long long u64;
 
-struct Row {
-    const void *p;
-    uint32_t dtype;
-    int n;
-};
+constexpr int NT = 1024, NW = NT / 64;
+constexpr int BINS = 4096;
+constexpr int SEGS = 64;    // runs of a wave, at most
+constexpr int CACHED = 32;  // ids per thread held in registers
 
-// l in f32, NaN as -inf, -0 as 0.
-__device__ __forceinline__ float logit(const Row &r, int i) {
-    float x;
-    if (r.dtype == T_F32) x = static_cast<const float *>(r.p)[i];
-    else if (r.dtype == T_F16) x = (float)static_cast<const _Float16 *>(r.p)[i];
-    else x = __uint_as_float((uint32_t)static_cast<const uint16_t *>(r.p)[i] << 16);
-    return x == x ? x + 0.0f : -INFINITY;
-}
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+// position in the order: smaller comes first
+__device__ __forceinline__ u64 place(float l, int id) { return (u64)(~key_of(l)) << 32 | (uint32_t)id; }
 
-struct Weights {
+struct bf16_bits {
+    uint16_t u;
+};
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float widen(bf16_bits x) { return __uint_as_float((uint32_t)x.u << 16); }
+
+struct Shared {
+    u64 hist[BINS];
+    u64 sums[SEGS * NW];
+    u64 list[NT];
+    u64 wave[NW + 1];
+    double exp2_[128];  // 2^(j / 128)
+    float red[2 * NW];
+    u64 at;      // a place, or an id
+    u64 before;  // count or weight in front of a bin
+    int bin, n;
+};
+
+// 2^S exp((l - max) / T) as a double: t = (l - max) log2e / T = k / 128 + r, k a whole
+// number, 2^(k / 128) from the table and the exponent, 2^r by its Taylor series to degree 4
+// (|r ln 2| <= 2.71e-3: within 2^-49).
+struct Weight {
     float max;
-    double inv_t, scale, min_p;  // scale = 2^S
-    __device__ __forceinline__ u64 operator()(float l) const {
-        if (l == max) return (u64)scale;
-        if (l == -INFINITY) return 0;
-        const double w = exp(((double)l - (double)max) * inv_t);
-        return w > 0.0 ? (u64)rint(w * scale) : 0;  // not above 0: NaN where both max l and T are infinite
+    double c;  // log2e / T
+    int S;
+    double low;  // t below it: weight 0
+    __device__ __forceinline__ double value(const Shared &sh, float l) const {
+        if (l == max) return __builtin_ldexp(1.0, S);
+        const double t = ((double)l - (double)max) * c;
+        if (!(t > low)) return 0.0;  // NaN too, of an infinite max and T
+        const double k = __builtin_rint(t * 128.0), r = __builtin_fma(k, -1.0 / 128, t);
+        const int i = (int)k;
+        double p = 0x1.3b2ab6fba4e77p-7;
+        p = __builtin_fma(p, r, 0x1.c6b08d704a0bfp-5);
+        p = __builtin_fma(p, r, 0x1.ebfbdff82c58ep-3);
+        p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);
+        p = __builtin_fma(p, r, 1.0);
+        return __builtin_ldexp(sh.exp2_[i & 127] * p, (i >> 7) + S);
     }
-};
-
-struct Keep {
-    uint32_t key;  // keys above it are kept,
-    int ties;      // and the first ids with this key
-};
-
-struct Sh {
-    u64 hist[256];
-    u64 wave[NW];
-    int cnt[NW];
-    u64 acc;
-    uint32_t key;
-    int ties, idx;
+    // rounded to a whole number: at most 2^50, so adding 2^52 leaves it in the low bits
+    __device__ __forceinline__ static u64 whole(double w) {
+        return (u64)(__builtin_bit_cast(long long, w + 0x1p52) - __builtin_bit_cast(long long, 0x1p52));
+    }
 };
 
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
@@ -68,203 +94,350 @@ __device__ __forceinline__ u64 wave_sum64(u64 v) {
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
     return v;
 }
-
-}  // namespace
-
-__global__ __launch_bounds__(NT) void k_sample(SampleRows R, int shift) {
-    __shared__ Sh sh;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t size = R.dtype == T_F32 ? 4 : 2;
-    const Row r{static_cast<const char *>(R.logits) + (size_t)row * R.stride * size, R.dtype, (int)R.vocab};
-    // the largest key
-    uint32_t top = 0;
-    for (int i = tid; i < r.n; i += NT) top = max(top, key_of(logit(r, i)));
-    if (tid == 0) {
-        sh.key = 0;
-        sh.idx = r.n;
+__device__ __forceinline__ u64 wave_scan64(u64 v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = __shfl_up(v, o);
+        if (lane >= o) v += y;
     }
+    return v;
+}
+// Exclusive prefix sum over the block's threads; total in every thread.
+__device__ __forceinline__ u64 block_scan(Shared &sh, u64 v, u64 &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const u64 incl = wave_scan64(v);
     __syncthreads();
-    atomicMax(&sh.key, top);
+    if (lane == 63) sh.wave[wave] = incl;
     __syncthreads();
-    top = sh.key;
-    const float max_l = of_key(top);
-    if (max_l == -INFINITY) {
-        if (tid == 0) {
-            R.ids[row] = -1;
-            if (R.probs) R.probs[row] = 0.0f;
-        }
-        return;
-    }
-    const float t = R.temperature ? R.temperature[row] : 1.0f;
-    const float min_p = R.min_p ? R.min_p[row] : 0.0f;
-    float top_p = R.top_p ? R.top_p[row] : 1.0f;
-    const int top_k = R.top_k ? R.top_k[row] : 0;
-    if (!(t > 0.0f) || min_p > 1.0f || top_p <= 0.0f || top_k == 1) {  // the most likely token
-        int at = r.n;
-        for (int i = tid; i < r.n; i += NT)
-            if (key_of(logit(r, i)) == top) {
-                at = i;
-                break;
-            }
-        atomicMin(&sh.idx, at);
-        __syncthreads();
-        if (tid == 0) {
-            R.ids[row] = sh.idx;
-            if (R.probs) R.probs[row] = 1.0f;
-        }
-        return;
-    }
-    Weights W;
-    W.max = max_l;
-    W.inv_t = 1.0 / (double)t;
-    W.scale = (double)(1ull << shift);
-
-    Keep keep{key_of(-INFINITY), 0};
-    if (top_k > 0 && top_k < r.n) {
-        uint32_t prefix = 0;
-        int left = top_k;
-        for (int s = 24; s >= 0; s -= 8) {
-            if (tid < 256) sh.hist[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < r.n; i += NT) {
-                const uint32_t k = key_of(logit(r, i));
-                if (s == 24 || (k >> (s + 8)) == (prefix >> (s + 8))) atomicAdd(&sh.hist[(k >> s) & 255u], 1ull);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int b = 255, c = left;
-                for (; b > 0 && c > (int)sh.hist[b]; b--) c -= (int)sh.hist[b];
-                sh.key = prefix | (uint32_t)b << s;
-                sh.ties = c;
-            }
-            __syncthreads();
-            prefix = sh.key;
-            left = sh.ties;
-            __syncthreads();
-        }
-        keep = {prefix, left};
-    }
-    // sum of what is kept: above the threshold, and its ties
-    if (top_p < 1.0f) {
-        u64 s = 0;
-        for (int i = tid; i < r.n; i += NT) {
-            const float l = logit(r, i);
-            if (key_of(l) > keep.key) s += W(l);
-        }
-        s = wave_sum64(s);
-        if (lane == 0) sh.wave[wave] = s;
-        __syncthreads();
-        u64 total = (u64)keep.ties * W(of_key(keep.key));
-        for (int w = 0; w < NW; w++) total += sh.wave[w];
-        const double want = (double)top_p * (double)total;
-        uint32_t prefix = 0;
-        u64 acc = 0;
-        for (int s2 = 24; s2 >= 0; s2 -= 8) {
-            __syncthreads();
-            if (tid < 256) sh.hist[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < r.n; i += NT) {
-                const float l = logit(r, i);
-                const uint32_t k = key_of(l);
-                if (k > keep.key && (s2 == 24 || (k >> (s2 + 8)) == (prefix >> (s2 + 8))))
-                    atomicAdd(&sh.hist[(k >> s2) & 255u], W(l));
-            }
-            __syncthreads();
-            if (tid == 0) {
-                if (keep.ties && (s2 == 24 || (keep.key >> (s2 + 8)) == (prefix >> (s2 + 8))))
-                    sh.hist[(keep.key >> s2) & 255u] += (u64)keep.ties * W(of_key(keep.key));
-                // from the top: the first bin that reaches `want`, else the lowest with weight
-                int b = 0;
-                u64 a = acc, before = acc;
-                for (int c = 255; c >= 0; c--) {
-                    if (!sh.hist[c]) continue;
-                    b = c;
-                    before = a;
-                    a += sh.hist[c];
-                    if ((double)a >= want) break;
-                }
-                sh.acc = before;
-                sh.key = prefix | (uint32_t)b << s2;
-            }
-            __syncthreads();
-            prefix = sh.key;
-            acc = sh.acc;
-        }
-        const u64 w = W(of_key(prefix));
-        const double m = ceil((want - (double)acc) / (double)w);
-        const int most = prefix == keep.key ? keep.ties : r.n;
-        keep = {prefix, max(1, (int)fmin(m, (double)most))};
-    }
-    // draw: a wave per contiguous part of the ids, then 64 at a time in the wave the draw falls into
-    const int part = (r.n + NW - 1) / NW, a0 = min(r.n, wave * part), a1 = min(r.n, a0 + part);
-    auto passes = [&](float l) { return l == max_l || !(min_p > 0.0f) || exp(((double)l - (double)max_l) * W.inv_t) >= (double)min_p; };
-    const u64 wk = passes(of_key(keep.key)) ? W(of_key(keep.key)) : 0;
-    u64 sum = 0;
-    int ties = 0;
-    for (int i = a0 + lane; i < a1; i += 64) {
-        const float l = logit(r, i);
-        const uint32_t k = key_of(l);
-        if (k > keep.key) sum += passes(l) ? W(l) : 0;
-        else if (k == keep.key) ties++;
-    }
-    sum = wave_sum64(sum);
-    for (int o = 1; o < 64; o <<= 1) ties += __shfl_xor(ties, o);
-    __syncthreads();
-    if (lane == 0) {
-        sh.wave[wave] = sum;
-        sh.cnt[wave] = ties;
-    }
-    __syncthreads();
-    u64 total = 0, before = 0;
-    int left = keep.ties, my_left = 0;
+    u64 run = 0;
+    total = 0;
+#pragma unroll
     for (int w = 0; w < NW; w++) {
-        if (w == wave) {
-            before = total;
-            my_left = left;
-        }
-        const int c = min(left, sh.cnt[w]);
-        total += sh.wave[w] + (u64)c * wk;
-        left -= c;
+        if (w == wave) run = total;
+        total += sh.wave[w];
     }
-    const u64 mine = sum + (u64)min(my_left, ties) * wk;
-    float u = R.u[row];
-    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    u64 want = (u64)((double)u * (double)total);
-    if (want >= total) want = total - 1;
-    if (!(want >= before && want < before + mine)) return;
-    u64 run = before;
-    for (int b = a0; b < a1; b += 64) {
-        const int i = b + lane;
-        const float l = i < a1 ? logit(r, i) : -INFINITY;
-        const uint32_t k = i < a1 ? key_of(l) : 0;
-        const bool tie = i < a1 && k == keep.key;
-        const unsigned long long tm = __ballot(tie);
-        const int rank = __popcll(tm & ((1ull << lane) - 1));
-        u64 w = k > keep.key ? (passes(l) ? W(l) : 0) : tie && rank < my_left ? wk : 0;
-        my_left = max(0, my_left - __popcll(tm));
-        u64 c = w;
-        for (int o = 1; o < 64; o <<= 1) {
-            const u64 y = __shfl_up(c, o);
-            if (lane >= o) c += y;
+    return run + incl - v;
+}
+
+// The row's logits.  Run r = seg * NW + wave holds ids r * q * 64 ...; lane
+// and step j of a run: id (r * q + j) * 64 + lane.
+template <class T, bool REGS>
+struct Row {
+    const T *p;
+    int n, q, segs;
+    float x[REGS ? CACHED : 1];
+
+    __device__ __forceinline__ float load(int i) const {
+        const float v = i < n ? widen(p[i]) : -INFINITY;
+        return v == v ? v + 0.0f : -INFINITY;  // NaN as -inf, -0 as 0
+    }
+    __device__ __forceinline__ void fill() {
+        if constexpr (REGS) {
+#pragma unroll
+            for (int s = 0; s < CACHED; s++) x[s] = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < CACHED; s++)
+                if (s < segs) x[s] = load(s * NT + (int)threadIdx.x);
         }
-        const unsigned long long hit = __ballot(run + c > want);
+    }
+    // f(seg, id, l) for this thread's ids, l = -inf past the row's end.
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        if constexpr (REGS) {
+            // opaque, and one after the other: else the passes share 32 keys, ids
+            // and places in registers, and spill
+            int id = (int)threadIdx.x, m = segs;
+            asm volatile("" : "+v"(id), "+s"(m));
+#pragma unroll
+            for (int s = 0; s < CACHED; s++)
+                if (s < m) {
+                    float v = x[s];
+                    asm volatile("" : "+v"(v), "+v"(id));
+                    f(s, id, v);
+                    id += NT;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        } else {
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            for (int s = 0; s < segs; s++) {
+                const int first = (s * NW + wave) * q * 64 + lane;
+                for (int j = 0; j < q; j += 4) {  // q is a multiple of 4
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = load(first + (j + e) * 64);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f(s, first + (j + e) * 64, v[e]);
+                }
+            }
+        }
+    }
+};
+
+// In double: no difference of two logits overflows, none is lost.
+struct Bins {
+    float max;
+    double f;
+    __device__ __forceinline__ int of(float l) const {
+        return l == max ? 0 : (int)fmin(((double)max - (double)l) * f, (double)(BINS - 1));  // the last one of NaN
+    }
+};
+
+// The last place to keep: what is kept so far is `keep`, of it only a prefix: the
+// first `want` elements (WEIGHTS false), or the shortest one whose weights reach the
+// share `p` of theirs.  limited: the last bin holds only weights of 0.  At
+// most one of the row's elements is at any place.
+template <bool WEIGHTS, class R>
+__device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, const Weight &W, u64 keep, u64 count, double p,
+                                   bool limited) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    for (int b = tid; b < BINS; b += NT) sh.hist[b] = 0;
+    if (tid == 0) sh.bin = -1;
+    __syncthreads();
+    row.each([&](int, int id, float l) {
+        if (l > -INFINITY && place(l, id) <= keep)
+            atomicAdd(&sh.hist[bins.of(l)], WEIGHTS ? Weight::whole(W.value(sh, l)) : 1ull);
+    });
+    __syncthreads();
+    constexpr int PER = BINS / NT;
+    u64 h[PER], mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; i++) mine += h[i] = sh.hist[PER * tid + i];
+    u64 run = block_scan(sh, mine, total);
+    const double want = WEIGHTS ? p * (double)total : (double)count;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if ((double)run < want && (double)(run + h[i]) >= want) {  // one bin of the row
+            sh.bin = PER * tid + i;
+            sh.before = run;
+        }
+        run += h[i];
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    const int bin = sh.bin;
+    if (bin < 0 || (limited && bin == BINS - 1)) return keep;  // fewer elements than wanted, or only weights of 0 beyond
+    const u64 before = sh.before;
+    // the bin's elements
+    row.each([&](int, int id, float l) {
+        if (l > -INFINITY && bins.of(l) == bin && place(l, id) <= keep) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < NT) sh.list[at] = place(l, id);
+        }
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= NT) {
+        // a bitonic sort, one element per thread; steps within a wave by lane exchanges
+        u64 v = tid < n ? sh.list[tid] : ~0ull;
+        for (int size = 2; size < 2 * n; size <<= 1) {
+            for (int d = size >> 1; d > 0; d >>= 1) {
+                u64 o;
+                if (d >= 64) {
+                    __syncthreads();
+                    sh.list[tid] = v;
+                    __syncthreads();
+                    o = sh.list[tid ^ d];
+                } else {
+                    o = __shfl_xor(v, d);
+                }
+                const bool up = (tid & size) == 0, low = (tid & d) == 0;
+                v = (low == up) == (o < v) ? o : v;
+            }
+        }
+        u64 w = 0;
+        if (tid < n) w = WEIGHTS ? Weight::whole(W.value(sh, __uint_as_float([&] {
+                             const uint32_t k = ~(uint32_t)(v >> 32);
+                             return k & 0x80000000u ? k ^ 0x80000000u : ~k;
+                         }()))) : 1;
+        u64 all;
+        const u64 ahead = before + block_scan(sh, w, all);
+        if (tid < n && (double)ahead < want && (double)(ahead + w) >= want) sh.at = v;
+        __syncthreads();
+        return sh.at;
+    }
+    // radix descent over the places
+    u64 prefix = 0, acc = before;
+    for (int s = 56; s >= 0; s -= 8) {
+        __syncthreads();
+        if (tid < 256) sh.hist[tid] = 0;
+        __syncthreads();
+        row.each([&](int, int id, float l) {
+            const u64 v = place(l, id);
+            if (l > -INFINITY && bins.of(l) == bin && v <= keep && (s == 56 || v >> (s + 8) == prefix >> (s + 8)))
+                atomicAdd(&sh.hist[(v >> s) & 255u], WEIGHTS ? Weight::whole(W.value(sh, l)) : 1ull);
+        });
+        __syncthreads();
+        const u64 c = tid < 256 ? sh.hist[tid] : 0;
+        u64 all;
+        const u64 ahead = acc + block_scan(sh, c, all);
+        if ((double)ahead < want && (double)(ahead + c) >= want) {
+            sh.at = prefix | (u64)tid << s;
+            sh.before = ahead;
+        }
+        __syncthreads();
+        prefix = sh.at;
+        acc = sh.before;
+    }
+    return prefix;
+}
+
+template <class T, bool REGS>
+__global__ __launch_bounds__(NT) void k_sample(SampleRows R, int S) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Row<T, REGS> row;
+    row.p = static_cast<const T *>(R.logits) + (size_t)r * R.stride;
+    row.n = (int)R.vocab;
+    row.q = REGS ? 1 : (row.n + SEGS * NT * 4 - 1) / (SEGS * NT * 4) * 4;
+    row.segs = (row.n + row.q * NT - 1) / (row.q * NT);
+    row.fill();
+    if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
+    const float temp = R.temperature ? R.temperature[r] : 1.0f;
+    const float min_p = R.min_p ? R.min_p[r] : 0.0f;
+    const float top_p = R.top_p ? R.top_p[r] : 1.0f;
+    const int top_k = R.top_k ? R.top_k[r] : 0;
+    const float u_in = R.u[r];
+
+    // the largest and the smallest finite logit
+    float hi = -INFINITY, lo = INFINITY;
+    row.each([&](int, int, float l) {
+        hi = fmaxf(hi, l);
+        lo = fminf(lo, l > -INFINITY ? l : INFINITY);
+    });
+    hi = wave_max(hi);
+    lo = -wave_max(-lo);
+    if (lane == 0) {
+        sh.red[wave] = hi;
+        sh.red[NW + wave] = lo;
+    }
+    if (tid == 0) sh.at = ~0ull;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        hi = fmaxf(hi, sh.red[w]);
+        lo = fminf(lo, sh.red[NW + w]);
+    }
+    if (hi == -INFINITY) {  // nothing to draw
+        if (tid == 0) {
+            R.ids[r] = -1;
+            if (R.probs) R.probs[r] = 0.0f;
+        }
+        return;
+    }
+    if (!(temp > 0.0f) || min_p > 1.0f || top_p <= 0.0f || top_k == 1) {  // the most likely token
+        u64 at = ~0ull;
+        row.each([&](int, int id, float l) {
+            if (l == hi && at == ~0ull) at = (u64)id;
+        });
+        if (at != ~0ull) atomicMin(&sh.at, at);
+        __syncthreads();
+        if (tid == 0) {
+            R.ids[r] = (int)sh.at;
+            if (R.probs) R.probs[r] = 1.0f;
+        }
+        return;
+    }
+    Weight W;
+    W.max = hi;
+    W.c = 1.4426950408889634 / (double)temp;
+    W.S = S;
+    W.low = -(double)(S + 2);
+    // Bins over the logits that have weight, or all of them if those span less.
+    const double span = (double)(S + 3) / W.c, range = (double)hi - (double)lo;
+    const bool limited = !(range < span);
+    const Bins bins{hi, (double)BINS / (limited ? span : range > 0.0 ? range : 1.0)};
+
+    u64 keep = ~0ull;
+    if (top_k > 0 && top_k < row.n) keep = cut<false>(sh, row, bins, W, keep, (u64)top_k, 0.0, limited);
+    if (top_p < 1.0f) keep = cut<true>(sh, row, bins, W, keep, 0, (double)top_p, limited);
+
+    // the runs' kept weights
+    const double least = min_p > 0.0f ? __builtin_ldexp((double)min_p, S) : 0.0;
+    auto kept = [&](int id, float l) -> u64 {
+        if (!(l > -INFINITY) || place(l, id) > keep) return 0;
+        const double w = W.value(sh, l);
+        return w >= least ? Weight::whole(w) : 0;
+    };
+    __syncthreads();
+    sh.sums[tid] = 0;
+    __syncthreads();
+    {
+        u64 sum = 0;
+        int at = 0;
+        row.each([&](int s, int id, float l) {
+            if constexpr (REGS) {
+                u64 w = kept(id, l);
+                if (__ballot(w != 0)) {
+                    w = wave_sum64(w);
+                    if (lane == 0) sh.sums[s * NW + wave] = w;
+                }
+            } else {
+                if (s != at) {
+                    if (__ballot(sum != 0)) {
+                        sum = wave_sum64(sum);
+                        if (lane == 0) sh.sums[at * NW + wave] = sum;
+                    }
+                    sum = 0;
+                    at = s;
+                }
+                sum += kept(id, l);
+            }
+        });
+        if constexpr (!REGS) {
+            sum = wave_sum64(sum);
+            if (lane == 0) sh.sums[at * NW + wave] = sum;
+        }
+    }
+    __syncthreads();
+    static_assert(SEGS * NW == NT, "a thread per run");
+    const u64 mine = sh.sums[tid];
+    u64 total;
+    const u64 ahead = block_scan(sh, mine, total);
+    const float u = u_in > 0.0f ? fminf(u_in, 0x1.fffffep-1f) : 0.0f;
+    u64 want = (u64)((double)u * (double)total);
+    want = want < total ? want : total - 1;
+    if (want >= ahead && want < ahead + mine) {
+        sh.bin = tid;
+        sh.before = ahead;
+    }
+    __syncthreads();
+    const int run = sh.bin;
+    if (wave != run % NW) return;
+    u64 acc = sh.before;
+    for (int j = 0; j < row.q; j++) {
+        const int id = (run * row.q + j) * 64 + lane;
+        const float l = row.load(id);
+        const u64 w = kept(id, l), c = wave_scan64(w);
+        const u64 hit = __ballot(acc + c > want);
         if (hit) {
-            const int at = __builtin_ctzll(hit);
-            if (lane == at) {
-                R.ids[row] = i;
-                if (R.probs) R.probs[row] = (float)((double)w / (double)total);
+            if (lane == __builtin_ctzll(hit)) {
+                R.ids[r] = id;
+                if (R.probs) R.probs[r] = (float)((double)w / (double)total);
             }
             return;
         }
-        run += __shfl(c, 63);
+        acc += __shfl(c, 63);
     }
 }
+
+}  // namespace
 
 hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
     if (!r.n_rows) return hipSuccess;
     int lg = 0;
     while ((1ull << lg) < r.vocab) lg++;
-    hipLaunchKernelGGL(k_sample, dim3((unsigned)r.n_rows), dim3(NT), 0, s, r, 62 - lg);
+    const int S = 62 - lg < 50 ? 62 - lg : 50;
+    auto go = [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (r.vocab <= (size_t)CACHED * NT)
+            hipLaunchKernelGGL((k_sample<T, true>), dim3((unsigned)r.n_rows), dim3(NT), 0, s, r, S);
+        else hipLaunchKernelGGL((k_sample<T, false>), dim3((unsigned)r.n_rows), dim3(NT), 0, s, r, S);
+    };
+    if (r.dtype == T_F32) go((float *)nullptr);
+    else if (r.dtype == T_F16) go((_Float16 *)nullptr);
+    else go((bf16_bits *)nullptr);
     return hipGetLastError();
 }
 

@@ -130,6 +130,16 @@ def test_infinities_and_nan(ctx):
     for par in ({}, {"top_k": 4}, {"top_p": 0.5}, {"temperature": 0.0}, {"temperature": 1e-30}, {"min_p": 0.1, "top_k": 299},
                 {"temperature": 3e38}):
         Call(ctx, x, G.F32, u, **par).check()
+    # more infinite logits than are kept; the whole range of f32
+    y = x[:3].copy()
+    y[:] = -3
+    y[:, 20:30] = np.inf
+    for par in ({"top_k": 3}, {"top_p": 0.25}, {"top_k": 7, "top_p": 0.5}):
+        Call(ctx, y, G.F32, [0.0, 0.5, 0.99], **par).check()
+    y = np.linspace(-3.4e38, 3.4e38, 300, dtype=F32)[None].repeat(3, 0)
+    for par in ({"top_k": 30}, {"top_p": 0.25}, {"top_k": 70, "top_p": 0.5}):
+        Call(ctx, y, G.F32, [0.0, 0.5, 0.99], temperature=3e38, **par).check()
+        Call(ctx, (y / F32(1e38)) * F32(1e-44), G.F32, [0.0, 0.5, 0.99], temperature=1e-44, **par).check()
     # an infinite temperature: every finite logit alike
     y = np.where(np.isinf(x), 0, x)[4:6].copy()
     Call(ctx, y, G.F32, u[4:6], temperature=np.inf).check()
