@@ -7,13 +7,12 @@
 // atomics, are deterministic.
 //
 // The filters keep a prefix of the order (l falling, id rising): it is told by
-// its last element, a 64-bit number ~key(l) << 32 | id that is smaller or equal for what
-// is kept (key: the bits of l in an order-preserving form).  To find it, a
+// its last element.  To find it, a
 // histogram over BINS equal intervals of l says which bin holds the end (by
 // counts for top-k, by weights for top-p); that bin's elements are collected,
 // sorted, and cut where the count or the sum is reached.  A bin of more than NT
-// elements (many equal logits) goes through a radix descent over the 64-bit
-// numbers instead, 8 bits a pass.
+// elements (many equal logits) goes through a radix descent over (order-preserving bits
+// of l, id), 64 bits, 8 a pass.
 //
 // The draw: each wave owns runs of q * 64 consecutive ids (run r of the row
 // belongs to wave r % 16); the runs' kept weights are summed and scanned, and the
@@ -89,20 +88,29 @@ struct Weight {
     }
 };
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    return v;
+// v of the lane CTRL names (0 where there is none, or for rows outside ROWS).
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (u64)hi << 32 | lo;
 }
+// Inclusive prefix sum over the lanes: within rows of 16 (shifts by 1, 2, 4, 8), then
+// lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
 __device__ __forceinline__ u64 wave_scan64(u64 v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(v, o);
-        if (lane >= o) v += y;
-    }
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xA>(v);
+    v += dpp64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ u64 lane64(u64 v, int l) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return lane64(wave_scan64(v), 63); }
 // Exclusive prefix sum over the block's threads; total in every thread.
 __device__ __forceinline__ u64 block_scan(Shared &sh, u64 v, u64 &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -128,17 +136,26 @@ struct Row {
     int n, q, segs;
     float x[REGS ? CACHED : 1];
 
-    __device__ __forceinline__ float load(int i) const {
-        const float v = i < n ? widen(p[i]) : -INFINITY;
-        return v == v ? v + 0.0f : -INFINITY;  // NaN as -inf, -0 as 0
+    // id i's logit as loaded, any for ids past the end: the load is not under a
+    // condition, so that several are in flight
+    __device__ __forceinline__ T raw(int i) const { return p[min(i, n - 1)]; }
+    // NaN and ids past the end as -inf, -0 as 0
+    __device__ __forceinline__ float value(int i, T t) const {
+        const float v = widen(t) + 0.0f;
+        return i < n && v == v ? v : -INFINITY;
     }
+    __device__ __forceinline__ float load(int i) const { return value(i, raw(i)); }
     __device__ __forceinline__ void fill() {
         if constexpr (REGS) {
+            T t[CACHED];
 #pragma unroll
-            for (int s = 0; s < CACHED; s++) x[s] = -INFINITY;
+            for (int s = 0; s < CACHED; s += 8) {
+                if (s >= segs) break;
 #pragma unroll
-            for (int s = 0; s < CACHED; s++)
-                if (s < segs) x[s] = load(s * NT + (int)threadIdx.x);
+                for (int e = 0; e < 8; e++) t[s + e] = raw((s + e) * NT + (int)threadIdx.x);
+            }
+#pragma unroll
+            for (int s = 0; s < CACHED; s++) x[s] = s < segs ? value(s * NT + (int)threadIdx.x, t[s]) : -INFINITY;
         }
     }
     // f(seg, id, l) for this thread's ids, l = -inf past the row's end.
@@ -163,47 +180,60 @@ struct Row {
             for (int s = 0; s < segs; s++) {
                 const int first = (s * NW + wave) * q * 64 + lane;
                 for (int j = 0; j < q; j += 4) {  // q is a multiple of 4
-                    float v[4];
+                    T t[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = load(first + (j + e) * 64);
+                    for (int e = 0; e < 4; e++) t[e] = raw(first + (j + e) * 64);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) f(s, first + (j + e) * 64, v[e]);
+                    for (int e = 0; e < 4; e++) f(s, first + (j + e) * 64, value(first + (j + e) * 64, t[e]));
                 }
             }
         }
     }
 };
 
-// In double: no difference of two logits overflows, none is lost.
+// f is between 2^-118 and 2^100, so that the product is neither NaN nor lost: past the
+// range it is the last bin, and logits of a range below 2^-88 share the first.
 struct Bins {
-    float max;
-    double f;
+    float max, f;
     __device__ __forceinline__ int of(float l) const {
-        return l == max ? 0 : (int)fmin(((double)max - (double)l) * f, (double)(BINS - 1));  // the last one of NaN
+        return l == max ? 0 : (int)fminf((max - l) * f, (float)(BINS - 1));
     }
 };
 
-// The last place to keep: what is kept so far is `keep`, of it only a prefix: the
-// first `want` elements (WEIGHTS false), or the shortest one whose weights reach the
-// share `p` of theirs.  limited: the last bin holds only weights of 0.  At
-// most one of the row's elements is at any place.
+// Bin b's place in the histogram: a thread's PER bins lie NT apart (no bank conflicts).
+constexpr int PER = BINS / NT;
+__device__ __forceinline__ int slot_of(int b) { return b % PER * NT + b / PER; }
+
+// The end of what is kept, in the order (l falling, id rising).
+struct Keep {
+    float l;
+    int id;
+    __device__ __forceinline__ bool has(float x, int i) const { return x > l || (x == l && i <= id); }
+};
+__device__ __forceinline__ float logit_of(u64 place) {
+    const uint32_t k = ~(uint32_t)(place >> 32);
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ Keep keep_to(u64 place) { return {logit_of(place), (int)(uint32_t)place}; }
+
+// The new end: of what is kept so far only a prefix, the first `want` elements (WEIGHTS false), or the shortest one whose weights reach the
+// share `p` of theirs.  limited: the last bin holds only weights of 0.
 template <bool WEIGHTS, class R>
-__device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, const Weight &W, u64 keep, u64 count, double p,
-                                   bool limited) {
+__device__ __forceinline__ Keep cut(Shared &sh, const R &row, const Bins &bins, const Weight &W, Keep keep, u64 count,
+                                    double p, bool limited) {
     const int tid = threadIdx.x;
     __syncthreads();
     for (int b = tid; b < BINS; b += NT) sh.hist[b] = 0;
     if (tid == 0) sh.bin = -1;
     __syncthreads();
     row.each([&](int, int id, float l) {
-        if (l > -INFINITY && place(l, id) <= keep)
-            atomicAdd(&sh.hist[bins.of(l)], WEIGHTS ? Weight::whole(W.value(sh, l)) : 1ull);
+        if (keep.has(l, id))
+            atomicAdd(&sh.hist[slot_of(bins.of(l))], WEIGHTS ? Weight::whole(W.value(sh, l)) : 1ull);
     });
     __syncthreads();
-    constexpr int PER = BINS / NT;
     u64 h[PER], mine = 0, total;
 #pragma unroll
-    for (int i = 0; i < PER; i++) mine += h[i] = sh.hist[PER * tid + i];
+    for (int i = 0; i < PER; i++) mine += h[i] = sh.hist[i * NT + tid];
     u64 run = block_scan(sh, mine, total);
     const double want = WEIGHTS ? p * (double)total : (double)count;
 #pragma unroll
@@ -221,7 +251,7 @@ __device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, c
     const u64 before = sh.before;
     // the bin's elements
     row.each([&](int, int id, float l) {
-        if (l > -INFINITY && bins.of(l) == bin && place(l, id) <= keep) {
+        if (bins.of(l) == bin && keep.has(l, id)) {
             const int at = atomicAdd(&sh.n, 1);
             if (at < NT) sh.list[at] = place(l, id);
         }
@@ -247,15 +277,12 @@ __device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, c
             }
         }
         u64 w = 0;
-        if (tid < n) w = WEIGHTS ? Weight::whole(W.value(sh, __uint_as_float([&] {
-                             const uint32_t k = ~(uint32_t)(v >> 32);
-                             return k & 0x80000000u ? k ^ 0x80000000u : ~k;
-                         }()))) : 1;
+        if (tid < n) w = WEIGHTS ? Weight::whole(W.value(sh, logit_of(v))) : 1;
         u64 all;
         const u64 ahead = before + block_scan(sh, w, all);
         if (tid < n && (double)ahead < want && (double)(ahead + w) >= want) sh.at = v;
         __syncthreads();
-        return sh.at;
+        return keep_to(sh.at);
     }
     // radix descent over the places
     u64 prefix = 0, acc = before;
@@ -265,7 +292,7 @@ __device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, c
         __syncthreads();
         row.each([&](int, int id, float l) {
             const u64 v = place(l, id);
-            if (l > -INFINITY && bins.of(l) == bin && v <= keep && (s == 56 || v >> (s + 8) == prefix >> (s + 8)))
+            if (bins.of(l) == bin && keep.has(l, id) && (s == 56 || v >> (s + 8) == prefix >> (s + 8)))
                 atomicAdd(&sh.hist[(v >> s) & 255u], WEIGHTS ? Weight::whole(W.value(sh, l)) : 1ull);
         });
         __syncthreads();
@@ -280,7 +307,7 @@ __device__ __forceinline__ u64 cut(Shared &sh, const R &row, const Bins &bins, c
         prefix = sh.at;
         acc = sh.before;
     }
-    return prefix;
+    return keep_to(prefix);
 }
 
 template <class T, bool REGS>
@@ -347,16 +374,16 @@ __global__ __launch_bounds__(NT) void k_sample(SampleRows R, int S) {
     // Bins over the logits that have weight, or all of them if those span less.
     const double span = (double)(S + 3) / W.c, range = (double)hi - (double)lo;
     const bool limited = !(range < span);
-    const Bins bins{hi, (double)BINS / (limited ? span : range > 0.0 ? range : 1.0)};
+    const Bins bins{hi, (float)fmin(fmax((double)BINS / (limited ? span : range), 0x1p-118), 0x1p100)};
 
-    u64 keep = ~0ull;
+    Keep keep{-INFINITY, -1};  // everything finite
     if (top_k > 0 && top_k < row.n) keep = cut<false>(sh, row, bins, W, keep, (u64)top_k, 0.0, limited);
     if (top_p < 1.0f) keep = cut<true>(sh, row, bins, W, keep, 0, (double)top_p, limited);
 
     // the runs' kept weights
     const double least = min_p > 0.0f ? __builtin_ldexp((double)min_p, S) : 0.0;
     auto kept = [&](int id, float l) -> u64 {
-        if (!(l > -INFINITY) || place(l, id) > keep) return 0;
+        if (!keep.has(l, id)) return 0;
         const double w = W.value(sh, l);
         return w >= least ? Weight::whole(w) : 0;
     };
@@ -368,9 +395,8 @@ __global__ __launch_bounds__(NT) void k_sample(SampleRows R, int S) {
         int at = 0;
         row.each([&](int s, int id, float l) {
             if constexpr (REGS) {
-                u64 w = kept(id, l);
-                if (__ballot(w != 0)) {
-                    w = wave_sum64(w);
+                if (__ballot(keep.has(l, id))) {
+                    const u64 w = wave_sum64(kept(id, l));
                     if (lane == 0) sh.sums[s * NW + wave] = w;
                 }
             } else {
@@ -382,7 +408,7 @@ __global__ __launch_bounds__(NT) void k_sample(SampleRows R, int S) {
                     sum = 0;
                     at = s;
                 }
-                sum += kept(id, l);
+                if (__ballot(keep.has(l, id))) sum += kept(id, l);
             }
         });
         if constexpr (!REGS) {
@@ -418,7 +444,7 @@ __global__ __launch_bounds__(NT) void k_sample(SampleRows R, int S) {
             }
             return;
         }
-        acc += __shfl(c, 63);
+        acc += lane64(c, 63);
     }
 }
 
