@@ -36,5 +36,6 @@ hipError_t q6_prepare_lds();
 hipError_t gemm_prepare_lds();
 hipError_t gemm_wide_prepare_lds();  // gemm_wide.hip
 hipError_t q8_mfma_prepare_lds();    // gemv_q8_mfma.hip
+hipError_t sample_prepare_lds();     // sample.hip
 
 }  // namespace rce_qmm

@@ -331,6 +331,7 @@ rce_qmm_status rce_qmm_context_create(int device, rce_qmm_context **out) {
     if (st) return st;
     HIP_TRY(rce_qmm::chain_prepare_lds());
     HIP_TRY(rce_qmm::q6_prepare_lds());
+    HIP_TRY(rce_qmm::sample_prepare_lds());
     HIP_TRY(rce_qmm::gemm_prepare_lds());
     HIP_TRY(rce_qmm::gemm_wide_prepare_lds());
     HIP_TRY(rce_qmm::q8_mfma_prepare_lds());
