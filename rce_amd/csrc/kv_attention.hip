@@ -45,6 +45,7 @@ constexpr int WAVES = 4;    // of a block
 constexpr int TILE = 64;    // positions of a wave's step
 constexpr int TARGET = 512;   // blocks that a call's tiles are spread over (two per CU)
 constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
+constexpr int FEW = 32;       // query rows per kv head up to which a sequence is served in units of ROWS
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -52,16 +53,21 @@ struct Args {
     KvPool P;
     KvRows B;
     KvAttention a;
-    int G;  // query heads per kv head
+    int G;          // query heads per kv head
+    int rows;       // query rows of a unit
+    int lo_x, hi_x; // the call's part: sequences of lo_x .. hi_x query rows per kv head
+    int target;     // blocks that the part's tiles are spread over
+    int vec;        // query rows (1) and rotation table (2) can be read 16 bytes at a time
 };
 
-// The units of a sequence (per kv head) and the tiles of its longest one.
+// The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one.
 struct Span {
     int units, t0, tiles;
 };
 __device__ __forceinline__ Span span_of(const Args &A, const KvSeq &q) {
     Span s;
-    s.units = (int)(((long long)(q.r1 - q.r0) * A.G + ROWS - 1) / ROWS);
+    const int x = (q.r1 - q.r0) * A.G;
+    s.units = x >= A.lo_x && x <= A.hi_x ? (x + A.rows - 1) / A.rows : 0;
     const int lo = max(0, q.lo() - (A.a.window - 1));
     s.t0 = lo / TILE;
     s.tiles = q.hi(A.B) > q.lo() ? (q.hi(A.B) + TILE - 1) / TILE - s.t0 : 0;
@@ -77,7 +83,7 @@ __device__ __forceinline__ int chunk_of(const Args &A) {
         total += (float)p.units * (float)p.tiles;
     }
     total = wave_sum(total) * (float)A.P.heads;
-    return max(MIN_CHUNK, (int)fminf(ceilf(total / (float)TARGET), 1e9f));
+    return max(MIN_CHUNK, (int)fminf(ceilf(total / (float)A.target), 1e9f));
 }
 
 __device__ __forceinline__ int ranges(int tiles, int chunk) { return tiles ? (tiles + chunk - 1) / chunk : 1; }
@@ -164,6 +170,30 @@ __device__ __forceinline__ void codes4(uint32_t x, half2v &lo, half2v &hi) {
     hi = as_h2(__builtin_amdgcn_perm(b, 0x64646464u, 0x00070006u)) + off;
 }
 
+// 16 values as LIMBS signed bytes each of rint(x * id), the highest first: one operand register
+// group per limb.
+template <int LIMBS>
+__device__ __forceinline__ void limbs_of(const float (&x)[16], float id, i32x4 (&out)[LIMBS]) {
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        uint32_t limb[LIMBS];
+#pragma unroll
+        for (int b = 0; b < LIMBS; b++) limb[b] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            int i = id == 0.0f ? 0 : (int)__builtin_rintf(x[4 * v + e] * id);
+#pragma unroll
+            for (int b = LIMBS - 1; b >= 0; b--) {  // signed bytes, the lowest first
+                const int c = (int)(int8_t)i;
+                limb[b] |= ((uint32_t)c & 255u) << (8 * e);
+                i = (i - c) >> 8;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < LIMBS; b++) out[b][v] = (int)limb[b];
+    }
+}
+
 // LDS: the query rows in f32 before the loop, the waves' results after it (at
 // most 128 dimensions at a time: 34 KB).
 template <int D>
@@ -242,26 +272,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
         const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
         qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
 #pragma unroll
-        for (int s = 0; s < NQ; s++)
+        for (int s = 0; s < NQ; s++) {
+            float x[16];
 #pragma unroll
-            for (int v = 0; v < 4; v++) {
-                uint32_t limb[LIMBS];
-#pragma unroll
-                for (int b = 0; b < LIMBS; b++) limb[b] = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = sh.q[n][64 * s + 16 * g + 4 * v + e];
-                    int i = id == 0.0f ? 0 : (int)__builtin_rintf(x * id);
-#pragma unroll
-                    for (int b = LIMBS - 1; b >= 0; b--) {  // signed bytes, the lowest first
-                        const int c = (int)(int8_t)i;
-                        limb[b] |= ((uint32_t)c & 255u) << (8 * e);
-                        i = (i - c) >> 8;
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < LIMBS; b++) qf[s][b][v] = (int)limb[b];
-            }
+            for (int j = 0; j < 16; j++) x[j] = sh.q[n][64 * s + 16 * g + j];
+            limbs_of<LIMBS>(x, id, qf[s]);
+        }
     }
     __syncthreads();  // sh.q is read; sh.o may be written
 
@@ -426,75 +442,461 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
     }
 }
 
-// The split units' ranges, in range order: a wave per (unit, head, row).
+// ---- many query rows ------------------------------------------------------
+//
+// A block of four waves takes 128 query rows; a wave 32 of them as the columns
+// of 32x32 MFMAs.  The block shares each tile of 64 positions through LDS: the key
+// codes as they are, the values converted to binary16 once, both with their
+// 16-byte pieces in another order per row (row r's piece c lies at c ^ (r % 8): the
+// rows are 128 bytes, and reads of one piece of 32 rows would fall on the same banks).
+// The next tile's codes travel to registers meanwhile.
+//   S^T = K Q^T (int8, 32x32x32): operand row r of tile half t is position
+//         32 t + 16 (r / 4 % 2) + 4 (r / 8) + r % 4, so that lane (n, g = lane / 32)
+//         gets the 16 scores of one block, 2 t + g.
+//   O^T += V^T P^T (binary16, 32x32x16): again the lane's scores in order are its
+//         operand.
+// O stays in the MFMAs' accumulators, in units of `ref`, the largest value
+// scale so far, and of the row's m.  m moves, and O and l are rescaled, only when a
+// score passes it by more than LAG (base 2): weights are then at most 2^LAG,
+// times UP in binary16 at most 2^15.
+constexpr int P_ROWS = 128, P_WAVES = 4;
+constexpr float LAG = 6.0f, UP = 512.0f;  // UP = 2^9
+
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float half_max(float x) {  // over the lanes n and n + 32
+    const unsigned w = __builtin_bit_cast(unsigned, x);
+    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned)q[0]), __builtin_bit_cast(float, (unsigned)q[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const unsigned w = __builtin_bit_cast(unsigned, x);
+    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return __builtin_bit_cast(float, (unsigned)q[0]) + __builtin_bit_cast(float, (unsigned)q[1]);
+}
+
+// 16 consecutive values from value index i; vec: the address is a multiple of 16 bytes.
+__device__ __forceinline__ void load16(const void *p, uint32_t t, size_t i, bool vec, float (&x)[16]) {
+    if (vec && t == T_F32) {
+        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float4 v = q[k];
+            x[4 * k] = v.x;
+            x[4 * k + 1] = v.y;
+            x[4 * k + 2] = v.z;
+            x[4 * k + 3] = v.w;
+        }
+    } else if (vec) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+        const uint4 a = q[0], b = q[1];
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (t == T_F16) {
+                const half2v h = as_h2(w[k]);
+                x[2 * k] = (float)h.x;
+                x[2 * k + 1] = (float)h.y;
+            } else {
+                x[2 * k] = __uint_as_float(w[k] << 16);
+                x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 16; k++) x[k] = load_any(p, t, i + k);
+    }
+}
+
+template <int D>
+struct PShared {
+    alignas(16) int8_t k[TILE * D];      // row: a position, pieces of 16 codes
+    alignas(16) _Float16 v[D * TILE];    // row: a dimension, pieces of 8 positions
+    float ks[4], vs[4];                  // of the tile's blocks; 0 and unseen where ok is 0
+    int ok[4];
+};
+
+template <int D, bool HILO>
+__global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_kv_prompt(Args A) {
+    constexpr int NQ = D / 32, NT = D / 32;
+    constexpr int LIMBS = HILO ? 3 : 2;
+    constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
+    constexpr int SWAP = D % 128 == 0 ? 7 : 3;  // a key row's pieces change places within groups of 8 or 4
+    constexpr int NK = TILE * D / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
+    __shared__ PShared<D> sh;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x % A.P.heads;
+    const int chunk = chunk_of(A);
+    Work w;
+    if (!find_work(A, blockIdx.x / A.P.heads, chunk, w)) return;
+    const KvSeq &q = w.q;
+    const int G = A.G, first = q.first();
+    const int x0 = w.unit * P_ROWS, n_x = min(P_ROWS, (q.r1 - q.r0) * G - x0);
+    const int xr = wave * 32 + n;  // this lane's row of the unit
+    const int tok = (x0 + xr) / G, pos = first + tok;
+    const bool is = xr < n_x && pos >= 0 && pos < A.B.cap;
+
+    i32x4 qf[NQ][LIMBS];
+    float qs;
+    {
+        float x[NQ][16];
+        const size_t at = (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + xr) % G) * D;
+#pragma unroll
+        for (int s = 0; s < NQ; s++) {
+            const int d = 32 * s + 16 * g;
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[s][j] = 0.0f;
+            if (!is) continue;
+            load16(A.a.q, A.a.q_dtype, at + d, A.vec & 1, x[s]);
+            const int half = A.a.rope.half;
+            if (!A.a.rope.cs || d >= 2 * half) continue;
+            const float *cs = A.a.rope.cs + (size_t)pos * half * 2;
+            float y[16], c[32];
+            if ((A.vec & 2) && half % 16 == 0) {  // the partners and the table's entries are whole pieces too
+                const bool lo = d < half;
+                const int k = lo ? d : d - half;
+                load16(A.a.q, A.a.q_dtype, at + (lo ? d + half : k), A.vec & 1, y);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 v = reinterpret_cast<const float4 *>(cs + 2 * k)[j];
+                    c[4 * j] = v.x;
+                    c[4 * j + 1] = v.y;
+                    c[4 * j + 2] = v.z;
+                    c[4 * j + 3] = v.w;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float xc = x[s][j] * c[2 * j], ys = y[j] * c[2 * j + 1];
+                    x[s][j] = lo ? xc - ys : ys + xc;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int dd = d + j;
+                    if (dd >= 2 * half) continue;
+                    const bool lo = dd < half;
+                    const int k = lo ? dd : dd - half;
+                    const float p = load_any(A.a.q, A.a.q_dtype, at + (lo ? dd + half : k));
+                    const float xc = x[s][j] * cs[2 * k], ys = p * cs[2 * k + 1];
+                    x[s][j] = lo ? xc - ys : ys + xc;
+                }
+            }
+        }
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < NQ; s++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                amax = fmaxf(amax, fabsf(x[s][j]));
+                bad |= !(fabsf(x[s][j]) < __builtin_inff());
+            }
+        amax = half_max(amax);
+        bad = half_max(bad ? 1.0f : 0.0f) != 0.0f;
+        const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
+        qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
+#pragma unroll
+        for (int s = 0; s < NQ; s++) limbs_of<LIMBS>(x[s], id, qf[s]);
+    }
+
+    const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;
+    // the wave's rows: positions that all of them see, or that any of them sees
+    const int w0 = wave * 32, w_n = min(32, n_x - w0);  // rows (none: w_n <= 0)
+    const int f0 = first + (x0 + w0) / G, f1 = first + (x0 + w0 + max(w_n, 1) - 1) / G;
+    const bool placed = w_n > 0 && f0 >= 0 && f1 < A.B.cap;
+    const int w_lo = max(0, f0 - (A.a.window - 1)), w_hi = w_n > 0 ? min(f1, A.B.cap - 1) : -1;
+    const int all_lo = max(0, f1 - (A.a.window - 1)), all_hi = f0;
+    // the block's tiles
+    const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
+    int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
+    t_lo = max(t_lo, w.sp.t0 + w.range * chunk);
+    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * chunk);
+    const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
+    const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
+
+    // What this thread moves: piece tid + 256 i of the tile's keys (position / (D / 16), 16
+    // codes) and of its values (dimension and block: 16 positions).
+    u32x4 kr[NK], vr[NK];
+    float ksr = 0.0f, vsr = 0.0f;
+    int okr = 0;
+    auto block_at = [&](int t, int b, bool &ok) -> size_t {  // block b of tile t, 0 where there is none
+        const int blk = min(4 * t + b, max_block);
+        const int pg = pages[blk >> A.P.lg_b];
+        ok = (unsigned)pg < (unsigned)A.P.n_pages;
+        return (((size_t)(ok ? pg : 0) * A.P.heads + h) << A.P.lg_b) + (blk & bmask);
+    };
+    constexpr int BP = D;  // pieces of a block: 16 positions x D codes / 16
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int e = tid + 64 * P_WAVES * i, b = e / BP, r = e % BP;
+            bool ok;
+            const size_t at = (block_at(t, b, ok) * BP + r) * 16;
+            kr[i] = *reinterpret_cast<const u32x4 *>(A.P.k + at);
+            vr[i] = *reinterpret_cast<const u32x4 *>(A.P.v + at);
+        }
+        if (tid < 4) {
+            bool ok;
+            const size_t blk = block_at(t, tid, ok);
+            ksr = A.P.k_scale[blk];
+            vsr = A.P.v_scale[blk];
+            okr = ok;
+        }
+    };
+    auto place = [&] {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int e = tid + 64 * P_WAVES * i, b = e / BP, r = e % BP;
+            {  // keys: position 16 b + r / (D / 16), piece r % (D / 16)
+                const int p = 16 * b + r / (D / 16), c = r % (D / 16);
+                *reinterpret_cast<u32x4 *>(sh.k + p * D + (c ^ (p & SWAP)) * 16) = kr[i];
+            }
+            {  // values: dimension r, positions 16 b .. + 15: pieces 2 b, 2 b + 1
+                half2v a[8];
+#pragma unroll
+                for (int k = 0; k < 4; k++) codes4(vr[i][k], a[2 * k], a[2 * k + 1]);
+                _Float16 *row = sh.v + r * TILE;
+                *reinterpret_cast<half8 *>(row + ((2 * b) ^ (r & 7)) * 8) = join8(a[0], a[1], a[2], a[3]);
+                *reinterpret_cast<half8 *>(row + ((2 * b + 1) ^ (r & 7)) * 8) = join8(a[4], a[5], a[6], a[7]);
+            }
+        }
+        if (tid < 4) {
+            sh.ks[tid] = ksr;
+            sh.vs[tid] = vsr;
+            sh.ok[tid] = okr;
+        }
+    };
+
+    f32x16 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f, ref = 0.0f;
+    // K operand row n of tile half t: its position there
+    const int kpos = 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3);
+    if (t_lo < t_hi) fetch(t_lo);
+    for (int t = t_lo; t < t_hi; t++) {
+        __syncthreads();  // the tile before is read
+        place();
+        __syncthreads();
+        if (t + 1 < t_hi) fetch(t + 1);
+        if (TILE * t > w_hi || TILE * t + TILE - 1 < w_lo) continue;  // no row of the wave sees it (the same in all lanes)
+
+        int xi[2][16];
+        float xf[HILO ? 2 : 1][16];  // HILO: scores as floats
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            i32x16 c[LIMBS];
+#pragma unroll
+            for (int b = 0; b < LIMBS; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) c[b][e] = 0;
+            const int p = 32 * u + kpos;
+#pragma unroll
+            for (int s = 0; s < NQ; s++) {
+                const int piece = 2 * s + g;
+                const i32x4 a = *reinterpret_cast<const i32x4 *>(sh.k + p * D + (piece ^ (p & SWAP)) * 16);
+#pragma unroll
+                for (int b = 0; b < LIMBS; b++) c[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qf[s][b], c[b], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                xi[u][e] = c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e];
+                if constexpr (HILO) xf[u][e] = (float)c[0][e] * 65536.0f + (float)xi[u][e];
+            }
+        }
+        const float f[2] = {sh.ks[g] * qs, sh.ks[2 + g] * qs};
+        float sv[2] = {sh.vs[g], sh.vs[2 + g]};
+        const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
+        const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
+        // scores in base 2 and their maximum
+        float x[2][16], top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const bool v_ok = sh.ok[2 * u + g];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                x[u][e] = (HILO ? xf[HILO ? u : 0][e] : (float)xi[u][e]) * f[u];
+                if (masked) {
+                    const int p = TILE * t + 32 * u + 16 * g + e;
+                    const bool see = v_ok && p >= p_lo && p <= p_hi;
+                    any |= see;
+                    x[u][e] = see ? x[u][e] : -INFINITY;
+                }
+                top = fmaxf(top, x[u][e]);
+            }
+            if (masked) {  // a block that no row of the wave sees may hold anything
+                const unsigned long long b = __ballot(any);
+                if (!((b >> (32 * g)) & 0xFFFFFFFFull)) sv[u] = 0.0f;
+            }
+        }
+        top = half_max(top);
+        // a score above m + LAG, a larger value scale: rescale
+        const float ref_new = fmaxf(ref, half_max(fmaxf(sv[0] < __builtin_inff() ? sv[0] : 0.0f, sv[1] < __builtin_inff() ? sv[1] : 0.0f)));
+        if (__ballot(top > m + LAG) || ref_new > ref) {
+            const float m_new = top > m + LAG ? top : m;
+            const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
+            l *= alpha;
+            const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][e] *= back;
+            m = m_new;
+            ref = ref_new;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        half8 ph[2][2], pl[2][2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            // an infinite or NaN scale makes NaN of the rows that see its block, no others
+            const float pw = ref > 0.0f ? sv[u] / ref * UP : sv[u] < __builtin_inff() ? 0.0f : sv[u];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float y = exp2_(x[u][e] - base);
+                sum += y;
+                const float p = masked && x[u][e] == -INFINITY ? 0.0f : y * pw;
+                const _Float16 hi = (_Float16)p;
+                ph[u][e >> 3][e & 7] = hi;
+                if constexpr (HILO) pl[u][e >> 3][e & 7] = (_Float16)(p - (float)hi);
+            }
+        }
+        l += sum;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const int d = 32 * i + n, piece = 4 * u + 2 * g + k;
+                    const half8 a = *reinterpret_cast<const half8 *>(sh.v + d * TILE + (piece ^ (d & 7)) * 8);
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[u][k], acc[i], 0, 0, 0);
+                    if constexpr (HILO) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[u][k], acc[i], 0, 0, 0);
+                }
+    }
+    // lane (n, g) holds dimensions 32 i + 8 j + 4 g + e of its row
+    l = half_sum(l);
+    if (xr >= n_x) return;
+    const float unit = ref * (1.0f / UP);
+    if (w.n_ranges == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l * unit;
+        const size_t at = (size_t)(q.r0 + tok) * A.a.out_stride + (size_t)(h * G + (x0 + xr) % G) * D + 4 * g;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                store_any(A.a.out, A.a.out_dtype, at + 32 * i + 8 * (e >> 2) + (e & 3), l == 0.0f ? 0.0f : acc[i][e] * inv);
+    } else {
+        float *part = A.a.parts + ((size_t)(w.slot + w.range) * A.P.heads + h) * (P_ROWS * (D + 2));
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) part[xr * D + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3)] = acc[i][e] * unit;
+        if (g == 0) {
+            part[P_ROWS * D + xr] = m;
+            part[P_ROWS * D + P_ROWS + xr] = l;
+        }
+    }
+}
+
+// The split units' ranges, in range order: a wave per (unit, head, row), every
+// wave of the grid the next one.
+constexpr int JOIN_BLOCKS = 512;
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_join(Args A) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunk = chunk_of(A);
-    const int task = blockIdx.x * 4 + wave, r = task % ROWS, rest = task / ROWS, h = rest % A.P.heads;
-    const int item = rest / A.P.heads;
-    int seq, unit;
-    if (!kv_find(A.B, item, [&](const KvSeq &q) {
-            const Span p = span_of(A, q);
-            return ranges(p.tiles, chunk) > 1 ? p.units : 0;
-        }, seq, unit))
-        return;
-    // the ranges before this unit's
-    int slot = 0;
-    for (int s = lane; s < seq; s += 64) {
-        const Span p = span_of(A, kv_seq(A.B, s));
-        const int n = ranges(p.tiles, chunk);
-        slot += n > 1 ? p.units * n : 0;
-    }
-    slot = __builtin_amdgcn_readlane(wave_scan(slot), 63);
-    const KvSeq q = kv_seq(A.B, seq);
-    const int nr = ranges(span_of(A, q).tiles, chunk), x = unit * ROWS + r;
-    if (x >= (q.r1 - q.r0) * A.G) return;
-    slot += unit * nr;
-    const size_t step = (size_t)A.P.heads * (ROWS * (D + 2));
-    const float *part = A.a.parts + ((size_t)slot * A.P.heads + h) * (ROWS * (D + 2));
-    float top = -INFINITY;
-    for (int k = lane; k < nr; k += 64) top = fmaxf(top, part[k * step + ROWS * D + r]);
-    top = wave_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float o[D / 64], sum = 0.0f;
+    const int rows = A.rows;
+    for (int task = blockIdx.x * 4 + wave;; task += gridDim.x * 4) {
+        const int r = task % rows, rest = task / rows, h = rest % A.P.heads;
+        int seq, unit;
+        if (!kv_find(A.B, rest / A.P.heads, [&](const KvSeq &q) {
+                const Span p = span_of(A, q);
+                return ranges(p.tiles, chunk) > 1 ? p.units : 0;
+            }, seq, unit))
+            return;
+        // the ranges before this unit's
+        int slot = 0;
+        for (int s = lane; s < seq; s += 64) {
+            const Span p = span_of(A, kv_seq(A.B, s));
+            const int n = ranges(p.tiles, chunk);
+            slot += n > 1 ? p.units * n : 0;
+        }
+        slot = __builtin_amdgcn_readlane(wave_scan(slot), 63);
+        const KvSeq q = kv_seq(A.B, seq);
+        const int nr = ranges(span_of(A, q).tiles, chunk), x = unit * rows + r;
+        if (x >= (q.r1 - q.r0) * A.G) continue;
+        slot += unit * nr;
+        const size_t step = (size_t)A.P.heads * (rows * (D + 2));
+        const float *part = A.a.parts + ((size_t)slot * A.P.heads + h) * (rows * (D + 2));
+        float top = -INFINITY;
+        for (int k = lane; k < nr; k += 64) top = fmaxf(top, part[k * step + rows * D + r]);
+        top = wave_max(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float o[D / 64], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) o[i] = 0.0f;
+        for (int i = 0; i < D / 64; i++) o[i] = 0.0f;
 #pragma unroll 4
-    for (int k = 0; k < nr; k++) {
-        const float *p = part + k * step;
-        const float f = exp2_(p[ROWS * D + r] - base);
-        sum = __builtin_fmaf(f, p[ROWS * D + ROWS + r], sum);
+        for (int k = 0; k < nr; k++) {
+            const float *p = part + k * step;
+            const float f = exp2_(p[rows * D + r] - base);
+            sum = __builtin_fmaf(f, p[rows * D + rows + r], sum);
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) o[i] = __builtin_fmaf(f, p[r * D + lane + 64 * i], o[i]);
+            for (int i = 0; i < D / 64; i++) o[i] = __builtin_fmaf(f, p[r * D + lane + 64 * i], o[i]);
+        }
+        const size_t at = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D;
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+            store_any(A.a.out, A.a.out_dtype, at + lane + 64 * i, sum == 0.0f ? 0.0f : o[i] / sum);
     }
-    const size_t at = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++)
-        store_any(A.a.out, A.a.out_dtype, at + lane + 64 * i, sum == 0.0f ? 0.0f : o[i] / sum);
 }
 
 }  // namespace
 
-// Split units have at least two ranges, all but the last of `chunk` tiles, so
-// there are at most twice TARGET of them (heads included), and a rounding
-// of the total adds less than one in 2^20.
-size_t kv_attention_parts_bytes() { return (size_t)(2 * TARGET + 64) * (ROWS * (256 + 2)) * sizeof(float); }
+// A part's split units have at least two ranges, all but the last of `chunk` tiles, so that
+// there are at most twice `target` of them (heads included); a rounding of the total
+// adds less than one in 2^10 (n_seqs is at most 2^20).
+constexpr int slots(int target) { return 2 * target + target / 16; }
+constexpr size_t PARTS = (size_t)34 << 20;
+static_assert((size_t)slots(TARGET) * ROWS * (256 + 2) * sizeof(float) <= PARTS, "room for the split ranges");
+size_t kv_attention_parts_bytes() { return PARTS; }
 
 hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_head, const KvAttention &a, hipStream_t s) {
     if (!rows.n_rows) return hipSuccess;
-    Args A{pool, rows, a, a.n_q / pool.heads};
-    // units of the call at most, and their split ranges
-    const size_t x = (size_t)rows.n_rows * A.G, units = x / ROWS + (size_t)rows.n_seqs;
-    const size_t u = units < x ? units : x;
-    const bool split = rows.cap > MIN_CHUNK * TILE;
-    const size_t items = (u + (split ? (2 * TARGET + 64) / pool.heads + 1 : 0)) * pool.heads;
-    const dim3 grid((unsigned)items), join((unsigned)((TARGET + 64) * ROWS / 4));
+    const int G = a.n_q / pool.heads;
+    // units of the call at most
+    const size_t x = (size_t)rows.n_rows * G;
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (a.out_dtype == T_F32) hipLaunchKernelGGL((k_kv_attention<D, true>), grid, dim3(64 * WAVES), 0, s, A);
-        else hipLaunchKernelGGL((k_kv_attention<D, false>), grid, dim3(64 * WAVES), 0, s, A);
-        if (split) hipLaunchKernelGGL((k_kv_join<D>), join, dim3(256), 0, s, A);
+        auto part = [&](bool many, int lo, int hi) {
+            Args A{pool, rows, a, G, many ? P_ROWS : ROWS, lo, hi, TARGET, 0};
+            if (many) {
+                const size_t fit = PARTS / ((size_t)P_ROWS * (D + 2) * sizeof(float));  // slots
+                A.target = (int)(fit * 16 / 33);
+                const int size = a.q_dtype == T_F32 ? 4 : 2;
+                if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
+                if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
+            }
+            const size_t units = x / A.rows + (size_t)rows.n_seqs, u = units < x ? units : x;
+            const bool split = rows.cap > MIN_CHUNK * TILE;
+            const dim3 grid((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
+            const bool f32 = a.out_dtype == T_F32;
+            if (many && f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A);
+            else if (many) hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A);
+            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, true>), grid, dim3(64 * WAVES), 0, s, A);
+            else hipLaunchKernelGGL((k_kv_attention<D, false>), grid, dim3(64 * WAVES), 0, s, A);
+            if (split) hipLaunchKernelGGL((k_kv_join<D>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
+        };
+        if (x > (size_t)FEW * rows.n_seqs) {
+            part(true, FEW + 1, INT_MAX);
+            part(false, 0, FEW);
+        } else {
+            part(false, 0, INT_MAX);
+        }
     };
     switch (d_head) {
     case 64: go(std::integral_constant<int, 64>{}); break;
