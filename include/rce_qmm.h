@@ -368,7 +368,8 @@ rce_qmm_status rce_qmm_llama_check(rce_qmm_llama *m);
  *   k code of dimension d  k[(((p * n_kv_heads + h) * B + b) * 16 + i) * d_head + d]
  *   v code of dimension d  v[(((p * n_kv_heads + h) * B + b) * d_head + d) * 16 + i]
  *   scales                 k_scale, v_scale[(p * n_kv_heads + h) * B + b]
- * d_head: 64, 128, 192 or 256.  k and v 16-byte aligned, the scales 4. */
+ * d_head: 64, 128, 192 or 256; fewer than 2^32 blocks.  k and v 16-byte
+ * aligned, the scales 4. */
 typedef struct rce_qmm_kv_cache {
     int8_t *k, *v;
     float *k_scale, *v_scale;

@@ -49,6 +49,9 @@ rce_qmm_status check_pool(const rce_qmm_kv_cache *c, KvPool &p) {
         return fail(RCE_QMM_BAD_SHAPE, "d_head must be 64, 128, 192 or 256");
     if (c->n_kv_heads == 0 || c->n_kv_heads > 65536) return fail(RCE_QMM_BAD_SHAPE, "n_kv_heads must be 1 to 65536");
     if (c->n_pages == 0 || c->n_pages > (size_t)INT_MAX) return fail(RCE_QMM_BAD_SHAPE, "n_pages must be 1 to 2^31 - 1");
+    // blocks are numbered in 32 bits (at 64 dimensions 2^32 of them are 8 TiB)
+    if (c->n_pages * c->n_kv_heads > (((size_t)1 << 32) - 1) / (pt / 16))
+        return fail(RCE_QMM_BAD_SHAPE, "n_pages * n_kv_heads * page_tokens / 16 must be below 2^32");
     p.n_pages = (int)c->n_pages;
     p.heads = (int)c->n_kv_heads;
     p.lg_b = 0;

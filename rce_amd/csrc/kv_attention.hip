@@ -30,7 +30,9 @@
 //                 normal in binary16); HILO adds a second binary16 term.
 #include "kv_cache.h"
 
+#include <algorithm>
 #include <climits>
+#include <cstdlib>
 #include <type_traits>
 
 #include "mfma_util.h"
@@ -43,7 +45,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int ROWS = 16;    // query rows of a unit
 constexpr int WAVES = 4;    // of a block
 constexpr int TILE = 64;    // positions of a wave's step
-constexpr int TARGET = 512;   // blocks that a call's tiles are spread over (two per CU)
+static int envi(const char*n,int d){const char*e=getenv(n);return e?atoi(e):d;}
+#define TARGET envi("KT",512)
+#define P_TARGET envi("PT",512)
 constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
 constexpr int FEW = 32;       // query rows per kv head up to which a sequence is served in units of ROWS
 
@@ -87,12 +91,14 @@ __device__ __forceinline__ int chunk_of(const Args &A) {
 }
 
 __device__ __forceinline__ int ranges(int tiles, int chunk) { return tiles ? (tiles + chunk - 1) / chunk : 1; }
+// Tiles of each of a unit's ranges but the last: the ranges are as long as each other.
+__device__ __forceinline__ int range_tiles(int tiles, int n) { return (tiles + n - 1) / n; }
 
 // A unit's split ranges are numbered within the call: parts slot (range number * heads + head).
 struct Work {
     KvSeq q;
     Span sp;
-    int seq, unit, range, n_ranges, slot;  // slot of the unit's range 0, before the head
+    int seq, unit, range, n_ranges, step, slot;  // step: tiles of a range; slot of the unit's range 0, before the head
 };
 
 // Range `item` of the list (sequence, unit, range).
@@ -117,8 +123,10 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
             w.q = kv_seq(A.B, w.seq);
             w.sp = span_of(A, w.q);
             w.n_ranges = ranges(w.sp.tiles, chunk);
-            w.unit = at / w.n_ranges;
-            w.range = at - w.unit * w.n_ranges;
+            w.step = range_tiles(w.sp.tiles, w.n_ranges);
+            const int u = at / w.n_ranges;
+            w.unit = w.sp.units - 1 - u;  // the units with the most keys first
+            w.range = at - u * w.n_ranges;
             w.slot = srun + __builtin_amdgcn_readlane(sincl - sc, l) + w.unit * w.n_ranges;
             return true;
         }
@@ -286,8 +294,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
     const int u_hi = min(A.B.cap - 1, first + u_tok1), u_first = first + u_tok0;
     const int all_lo = max(0, max(0, u_hi) - (A.a.window - 1)), all_hi = u_first;  // seen by every row (if all have positions)
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-    t_lo = max(t_lo, w.sp.t0 + w.range * chunk);
-    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * chunk);
+    t_lo = max(t_lo, w.sp.t0 + w.range * w.step);
+    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * w.step);
     const bool placed = u_first >= 0 && first + u_tok1 < A.B.cap;  // every row has a position
     const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1;
@@ -512,8 +520,8 @@ template <int D>
 struct PShared {
     alignas(16) int8_t k[TILE * D];      // row: a position, pieces of 16 codes
     alignas(16) _Float16 v[D * TILE];    // row: a dimension, pieces of 8 positions
-    float ks[4], vs[4];                  // of the tile's blocks; 0 and unseen where ok is 0
-    int ok[4];
+    float ks[4], vs[4];                  // of the tile's blocks
+    int ok[4];                           // 0: no page
 };
 
 template <int D, bool HILO>
@@ -523,7 +531,8 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
     constexpr int SWAP = D % 128 == 0 ? 7 : 3;  // a key row's pieces change places within groups of 8 or 4
     constexpr int NK = TILE * D / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
-    __shared__ PShared<D> sh;
+    constexpr int BUFS = D <= 128 ? 2 : 1;  // two where they fit 64 KB
+    __shared__ PShared<D> buf[BUFS];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.P.heads;
@@ -610,61 +619,67 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     // the block's tiles
     const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-    t_lo = max(t_lo, w.sp.t0 + w.range * chunk);
-    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * chunk);
+    t_lo = max(t_lo, w.sp.t0 + w.range * w.step);
+    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * w.step);
     const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
 
     // What this thread moves: piece tid + 256 i of the tile's keys (position / (D / 16), 16
-    // codes) and of its values (dimension and block: 16 positions).
+    // codes) and of its values (dimension and block: 16 positions); pieces i of
+    // all threads lie in one block for D = 256, in 4 / NK of them else.
+    constexpr int BP = D;  // pieces of a block: 16 positions x D codes / 16
     u32x4 kr[NK], vr[NK];
     float ksr = 0.0f, vsr = 0.0f;
-    int okr = 0;
-    auto block_at = [&](int t, int b, bool &ok) -> size_t {  // block b of tile t, 0 where there is none
-        const int blk = min(4 * t + b, max_block);
-        const int pg = pages[blk >> A.P.lg_b];
-        ok = (unsigned)pg < (unsigned)A.P.n_pages;
-        return (((size_t)(ok ? pg : 0) * A.P.heads + h) << A.P.lg_b) + (blk & bmask);
+    int pg[NK], pgs = 0, oks = 0;  // the next tile's page ids, loaded a tile ahead
+    auto block_of = [&](int t, int b) { return min(4 * t + b, max_block); };
+    auto look = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) pg[i] = pages[block_of(t, (tid + 64 * P_WAVES * i) / BP) >> A.P.lg_b];
+        if (tid < 4) pgs = pages[block_of(t, tid) >> A.P.lg_b];
     };
-    constexpr int BP = D;  // pieces of a block: 16 positions x D codes / 16
+    auto block_at = [&](int page, int blk) -> uint32_t {  // page 0 where there is none
+        const uint32_t p = (unsigned)page < (unsigned)A.P.n_pages ? page : 0;
+        return ((p * (uint32_t)A.P.heads + (uint32_t)h) << A.P.lg_b) + (uint32_t)(blk & bmask);
+    };
+    const int8_t *const k_at = A.P.k + tid % BP * 16, *const v_at = A.P.v + tid % BP * 16;
+    static_assert(64 * P_WAVES % BP == 0 || D == 192, "a thread's pieces lie at one place of their blocks");
     auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int e = tid + 64 * P_WAVES * i, b = e / BP, r = e % BP;
-            bool ok;
-            const size_t at = (block_at(t, b, ok) * BP + r) * 16;
-            kr[i] = *reinterpret_cast<const u32x4 *>(A.P.k + at);
-            vr[i] = *reinterpret_cast<const u32x4 *>(A.P.v + at);
+            const int e = tid + 64 * P_WAVES * i, b = e / BP;
+            size_t at = (size_t)block_at(pg[i], block_of(t, b)) * (16 * D);
+            if constexpr (64 * P_WAVES % BP != 0) at += (e % BP - tid % BP) * 16;
+            kr[i] = *reinterpret_cast<const u32x4 *>(k_at + at);
+            vr[i] = *reinterpret_cast<const u32x4 *>(v_at + at);
         }
         if (tid < 4) {
-            bool ok;
-            const size_t blk = block_at(t, tid, ok);
+            const size_t blk = block_at(pgs, block_of(t, tid));
             ksr = A.P.k_scale[blk];
             vsr = A.P.v_scale[blk];
-            okr = ok;
+            oks = (unsigned)pgs < (unsigned)A.P.n_pages;
         }
     };
-    auto place = [&] {
+    auto place = [&](PShared<D> &to) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int e = tid + 64 * P_WAVES * i, b = e / BP, r = e % BP;
             {  // keys: position 16 b + r / (D / 16), piece r % (D / 16)
                 const int p = 16 * b + r / (D / 16), c = r % (D / 16);
-                *reinterpret_cast<u32x4 *>(sh.k + p * D + (c ^ (p & SWAP)) * 16) = kr[i];
+                *reinterpret_cast<u32x4 *>(to.k + p * D + (c ^ (p & SWAP)) * 16) = kr[i];
             }
             {  // values: dimension r, positions 16 b .. + 15: pieces 2 b, 2 b + 1
                 half2v a[8];
 #pragma unroll
                 for (int k = 0; k < 4; k++) codes4(vr[i][k], a[2 * k], a[2 * k + 1]);
-                _Float16 *row = sh.v + r * TILE;
+                _Float16 *row = to.v + r * TILE;
                 *reinterpret_cast<half8 *>(row + ((2 * b) ^ (r & 7)) * 8) = join8(a[0], a[1], a[2], a[3]);
                 *reinterpret_cast<half8 *>(row + ((2 * b + 1) ^ (r & 7)) * 8) = join8(a[4], a[5], a[6], a[7]);
             }
         }
         if (tid < 4) {
-            sh.ks[tid] = ksr;
-            sh.vs[tid] = vsr;
-            sh.ok[tid] = okr;
+            to.ks[tid] = ksr;
+            to.vs[tid] = vsr;
+            to.ok[tid] = oks;
         }
     };
 
@@ -673,110 +688,137 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
-    float m = -INFINITY, l = 0.0f, ref = 0.0f;
+    float m = -INFINITY, l = 0.0f, ref = 0.0f, inv_ref = 0.0f;
     // K operand row n of tile half t: its position there
     const int kpos = 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3);
-    if (t_lo < t_hi) fetch(t_lo);
+    if (t_lo < t_hi) {
+        look(t_lo);
+        fetch(t_lo);
+        look(t_lo + 1);
+        place(buf[0]);
+        if (t_lo + 1 < t_hi) fetch(t_lo + 1);
+        look(t_lo + 2);
+    }
+    __syncthreads();
     for (int t = t_lo; t < t_hi; t++) {
-        __syncthreads();  // the tile before is read
-        place();
+        const PShared<D> &sh = buf[(t - t_lo) & (BUFS - 1)];
+        if (TILE * t <= w_hi && TILE * t + TILE - 1 >= w_lo) {  // some row of the wave sees it (the same in all lanes)
+            const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
+            const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {  // 32 positions at a time: half the registers
+                int xi[16];  // scores as whole numbers (HILO: without the highest limb)
+                float xh[HILO ? 16 : 1];
+                {
+                    i32x16 c[LIMBS];
+#pragma unroll
+                    for (int b = 0; b < LIMBS; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) c[b][e] = 0;
+                    const int p = 32 * u + kpos;
+#pragma unroll
+                    for (int s = 0; s < NQ; s++) {
+                        const i32x4 a = *reinterpret_cast<const i32x4 *>(sh.k + p * D + ((2 * s + g) ^ (p & SWAP)) * 16);
+#pragma unroll
+                        for (int b = 0; b < LIMBS; b++) c[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qf[s][b], c[b], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        xi[e] = c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e];
+                        if constexpr (HILO) xh[e] = (float)c[0][e] * 65536.0f;
+                    }
+                }
+                auto score = [&](int e) { return HILO ? xh[HILO ? e : 0] + (float)xi[e] : (float)xi[e]; };
+                const float f = sh.ks[2 * u + g] * qs;
+                float sv = sh.vs[2 * u + g], top;
+                uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
+                if (HILO || masked) {
+                    if (masked) {
+                        const int p = TILE * t + 32 * u + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
+                        seen = sh.ok[2 * u + g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
+                        // a block that no row of the wave sees may hold anything
+                        if (!((__ballot(seen != 0) >> (32 * g)) & 0xFFFFFFFFull)) sv = 0.0f;
+                    }
+                    asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
+                    top = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+                } else {
+                    int x = xi[0];
+#pragma unroll
+                    for (int e = 1; e < 16; e++) x = max(x, xi[e]);
+                    top = (float)x * f;
+                }
+                top = half_max(top);
+                // `top` above m + LAG, or a larger value scale: rescale
+                const bool fin = sv < __builtin_inff();
+                const float scale = half_max(fin ? sv : 0.0f);
+                if (__ballot(top > m + LAG) || scale > ref) {
+                    const float m_new = top > m + LAG ? top : m, ref_new = fmaxf(ref, scale);
+                    const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
+                    const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
+                    l *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) acc[i][e] *= back;
+                    m = m_new;
+                    ref = ref_new;
+                    inv_ref = ref > 0.0f ? UP / ref : 0.0f;
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                // what the values' scale makes of the weights; an infinite or NaN one makes NaN
+                // of the rows that see its block, no others
+                const float pw = fin ? sv * inv_ref : sv;
+                half8 ph[2], pl[2];
+                // The ordinary case: no mask, value scales above 2^-12 of `ref`.  The scale goes
+                // into the exponent, l gets the sum of the rounded weights (dot products with
+                // ones) over it.  Two terms (HILO) and all else take the longer way.
+                if (!HILO && !masked && !__ballot(!(pw >= 0.125f && pw < 2.0f * UP))) {
+                    const float lw = __builtin_amdgcn_logf(pw), off = lw - base;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const half2v p = {(_Float16)exp2_(__builtin_fmaf((float)xi[e], f, off)),
+                                          (_Float16)exp2_(__builtin_fmaf((float)xi[e + 1], f, off))};
+                        sum = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                        ph[e >> 3][e & 7] = p.x;
+                        ph[e >> 3][(e & 7) + 1] = p.y;
+                    }
+                    l = __builtin_fmaf(sum, exp2_(-lw), l);
+                } else {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const bool see = seen >> e & 1;
+                        const float y = see ? exp2_(score(e) * f - base) : 0.0f, p = see ? y * pw : 0.0f;
+                        sum += y;
+                        const _Float16 hi = (_Float16)p;
+                        ph[e >> 3][e & 7] = hi;
+                        if constexpr (HILO) pl[e >> 3][e & 7] = (_Float16)(p - (float)hi);
+                    }
+                    l += sum;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) {  // 16 positions: 32 u + 16 g + 8 k ...
+                    const int piece = 4 * u + 2 * g + k;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const int d = 32 * i + n;
+                        const half8 a = *reinterpret_cast<const half8 *>(sh.v + d * TILE + (piece ^ (d & 7)) * 8);
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[k], acc[i], 0, 0, 0);
+                        if constexpr (HILO) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[k], acc[i], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if constexpr (BUFS == 1) __syncthreads();
+        if (t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
+            place(buf[(t + 1 - t_lo) & (BUFS - 1)]);
+            if (t + 2 < t_hi) fetch(t + 2);
+            look(t + 3);
+        }
         __syncthreads();
-        if (t + 1 < t_hi) fetch(t + 1);
-        if (TILE * t > w_hi || TILE * t + TILE - 1 < w_lo) continue;  // no row of the wave sees it (the same in all lanes)
-
-        int xi[2][16];
-        float xf[HILO ? 2 : 1][16];  // HILO: scores as floats
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            i32x16 c[LIMBS];
-#pragma unroll
-            for (int b = 0; b < LIMBS; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) c[b][e] = 0;
-            const int p = 32 * u + kpos;
-#pragma unroll
-            for (int s = 0; s < NQ; s++) {
-                const int piece = 2 * s + g;
-                const i32x4 a = *reinterpret_cast<const i32x4 *>(sh.k + p * D + (piece ^ (p & SWAP)) * 16);
-#pragma unroll
-                for (int b = 0; b < LIMBS; b++) c[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qf[s][b], c[b], 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                xi[u][e] = c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e];
-                if constexpr (HILO) xf[u][e] = (float)c[0][e] * 65536.0f + (float)xi[u][e];
-            }
-        }
-        const float f[2] = {sh.ks[g] * qs, sh.ks[2 + g] * qs};
-        float sv[2] = {sh.vs[g], sh.vs[2 + g]};
-        const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
-        const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
-        // scores in base 2 and their maximum
-        float x[2][16], top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const bool v_ok = sh.ok[2 * u + g];
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                x[u][e] = (HILO ? xf[HILO ? u : 0][e] : (float)xi[u][e]) * f[u];
-                if (masked) {
-                    const int p = TILE * t + 32 * u + 16 * g + e;
-                    const bool see = v_ok && p >= p_lo && p <= p_hi;
-                    any |= see;
-                    x[u][e] = see ? x[u][e] : -INFINITY;
-                }
-                top = fmaxf(top, x[u][e]);
-            }
-            if (masked) {  // a block that no row of the wave sees may hold anything
-                const unsigned long long b = __ballot(any);
-                if (!((b >> (32 * g)) & 0xFFFFFFFFull)) sv[u] = 0.0f;
-            }
-        }
-        top = half_max(top);
-        // a score above m + LAG, a larger value scale: rescale
-        const float ref_new = fmaxf(ref, half_max(fmaxf(sv[0] < __builtin_inff() ? sv[0] : 0.0f, sv[1] < __builtin_inff() ? sv[1] : 0.0f)));
-        if (__ballot(top > m + LAG) || ref_new > ref) {
-            const float m_new = top > m + LAG ? top : m;
-            const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
-            l *= alpha;
-            const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[i][e] *= back;
-            m = m_new;
-            ref = ref_new;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        half8 ph[2][2], pl[2][2];
-        float sum = 0.0f;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            // an infinite or NaN scale makes NaN of the rows that see its block, no others
-            const float pw = ref > 0.0f ? sv[u] / ref * UP : sv[u] < __builtin_inff() ? 0.0f : sv[u];
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float y = exp2_(x[u][e] - base);
-                sum += y;
-                const float p = masked && x[u][e] == -INFINITY ? 0.0f : y * pw;
-                const _Float16 hi = (_Float16)p;
-                ph[u][e >> 3][e & 7] = hi;
-                if constexpr (HILO) pl[u][e >> 3][e & 7] = (_Float16)(p - (float)hi);
-            }
-        }
-        l += sum;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const int d = 32 * i + n, piece = 4 * u + 2 * g + k;
-                    const half8 a = *reinterpret_cast<const half8 *>(sh.v + d * TILE + (piece ^ (d & 7)) * 8);
-                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[u][k], acc[i], 0, 0, 0);
-                    if constexpr (HILO) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[u][k], acc[i], 0, 0, 0);
-                }
     }
     // lane (n, g) holds dimensions 32 i + 8 j + 4 g + e of its row
     l = half_sum(l);
@@ -812,12 +854,12 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
     const int chunk = chunk_of(A);
     const int rows = A.rows;
     for (int task = blockIdx.x * 4 + wave;; task += gridDim.x * 4) {
-        const int r = task % rows, rest = task / rows, h = rest % A.P.heads;
-        int seq, unit;
-        if (!kv_find(A.B, rest / A.P.heads, [&](const KvSeq &q) {
+        const int h = task % A.P.heads;
+        int seq, x;  // query row x of the sequence
+        if (!kv_find(A.B, task / A.P.heads, [&](const KvSeq &q) {
                 const Span p = span_of(A, q);
-                return ranges(p.tiles, chunk) > 1 ? p.units : 0;
-            }, seq, unit))
+                return p.units && ranges(p.tiles, chunk) > 1 ? (q.r1 - q.r0) * A.G : 0;
+            }, seq, x))
             return;
         // the ranges before this unit's
         int slot = 0;
@@ -828,9 +870,8 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
         }
         slot = __builtin_amdgcn_readlane(wave_scan(slot), 63);
         const KvSeq q = kv_seq(A.B, seq);
-        const int nr = ranges(span_of(A, q).tiles, chunk), x = unit * rows + r;
-        if (x >= (q.r1 - q.r0) * A.G) continue;
-        slot += unit * nr;
+        const int nr = ranges(span_of(A, q).tiles, chunk), r = x % rows;
+        slot += x / rows * nr;
         const size_t step = (size_t)A.P.heads * (rows * (D + 2));
         const float *part = A.a.parts + ((size_t)slot * A.P.heads + h) * (rows * (D + 2));
         float top = -INFINITY;
@@ -862,26 +903,26 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
 // adds less than one in 2^10 (n_seqs is at most 2^20).
 constexpr int slots(int target) { return 2 * target + target / 16; }
 constexpr size_t PARTS = (size_t)34 << 20;
-static_assert((size_t)slots(TARGET) * ROWS * (256 + 2) * sizeof(float) <= PARTS, "room for the split ranges");
 size_t kv_attention_parts_bytes() { return PARTS; }
 
 hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_head, const KvAttention &a, hipStream_t s) {
     if (!rows.n_rows) return hipSuccess;
     const int G = a.n_q / pool.heads;
-    // units of the call at most
     const size_t x = (size_t)rows.n_rows * G;
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
         auto part = [&](bool many, int lo, int hi) {
-            Args A{pool, rows, a, G, many ? P_ROWS : ROWS, lo, hi, TARGET, 0};
+            Args A{pool, rows, a, G, many ? P_ROWS : ROWS, lo, hi, 0, 0};
+            const size_t fit = PARTS / ((size_t)A.rows * (D + 2) * sizeof(float));  // slots
+            A.target = std::min(many ? P_TARGET : TARGET, (int)(fit * 16 / 33));
             if (many) {
-                const size_t fit = PARTS / ((size_t)P_ROWS * (D + 2) * sizeof(float));  // slots
-                A.target = (int)(fit * 16 / 33);
                 const int size = a.q_dtype == T_F32 ? 4 : 2;
                 if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
                 if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
             }
-            const size_t units = x / A.rows + (size_t)rows.n_seqs, u = units < x ? units : x;
+            // units of the part at most
+            size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
+            if (hi != INT_MAX) u = std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
             const bool split = rows.cap > MIN_CHUNK * TILE;
             const dim3 grid((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
             const bool f32 = a.out_dtype == T_F32;

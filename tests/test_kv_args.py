@@ -42,7 +42,7 @@ def refused(status, f, *args, **kw):
 
 BAD_CACHES = [(dict(page_tokens=8), BAD), (dict(page_tokens=48), BAD), (dict(page_tokens=8192), BAD), (dict(page_tokens=0), BAD),
               (dict(d_head=80), BAD), (dict(d_head=0), BAD), (dict(d_head=512), BAD), (dict(n_kv_heads=0), BAD),
-              (dict(n_kv_heads=1 << 40), BAD), (dict(n_pages=0), BAD), (dict(n_pages=1 << 31), BAD), (dict(k=0), NULL),
+              (dict(n_kv_heads=1 << 40), BAD), (dict(n_pages=0), BAD), (dict(n_pages=1 << 31), BAD), (dict(n_pages=1 << 20, page_tokens=4096, n_kv_heads=16), BAD), (dict(k=0), NULL),
               (dict(v=0), NULL), (dict(k_scale=0), NULL), (dict(v_scale=0), NULL), (dict(k=(1 << 20) + 8), BAD),
               (dict(v=(1 << 20) + 1), BAD), (dict(k_scale=(1 << 20) + 2), BAD), (dict(v_scale=(1 << 20) + 1), BAD)]
 BAD_BATCHES = [(dict(row_offsets=0), NULL), (dict(seq_lens=0), NULL), (dict(pages=0), NULL), (dict(pages=(1 << 20) + 2), BAD),
