@@ -61,7 +61,7 @@ struct Args {
     int rows;       // query rows of a unit
     int lo_x, hi_x; // the call's part: sequences of lo_x .. hi_x query rows per kv head
     int target;     // blocks that the part's tiles are spread over
-    int vec;        // query rows (1) and rotation table (2) can be read 16 bytes at a time
+    int vec;        // query rows (1) and rotation table (2) can be read, output rows (4) written 16 bytes at a time
 };
 
 // The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one.
@@ -160,13 +160,14 @@ __device__ __forceinline__ float load_any(const void *p, uint32_t t, size_t i) {
     if (t == T_F16) return (float)static_cast<const _Float16 *>(p)[i];
     return __uint_as_float((uint32_t)static_cast<const uint16_t *>(p)[i] << 16);
 }
+__device__ __forceinline__ uint32_t bf16_of(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return x != x ? 0x7FC0u : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
 __device__ __forceinline__ void store_any(void *p, uint32_t t, size_t i, float x) {
     if (t == T_F32) static_cast<float *>(p)[i] = x;
     else if (t == T_F16) static_cast<_Float16 *>(p)[i] = (_Float16)x;
-    else {
-        const uint32_t u = __float_as_uint(x);
-        static_cast<uint16_t *>(p)[i] = (uint16_t)(x != x ? 0x7FC0u : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-    }
+    else static_cast<uint16_t *>(p)[i] = (uint16_t)bf16_of(x);
 }
 
 // Four codes as two binary16 pairs: bytes offset to 0 .. 255 become the low
@@ -483,36 +484,71 @@ __device__ __forceinline__ float half_sum(float x) {
     return __builtin_bit_cast(float, (unsigned)q[0]) + __builtin_bit_cast(float, (unsigned)q[1]);
 }
 
-// 16 consecutive values from value index i; vec: the address is a multiple of 16 bytes.
-__device__ __forceinline__ void load16(const void *p, uint32_t t, size_t i, bool vec, float (&x)[16]) {
-    if (vec && t == T_F32) {
+// Pieces of 16 values from value index i, one every 32: D / 32 of them, at multiples of 16 bytes.
+template <int D>
+__device__ __forceinline__ void load_row(const void *p, uint32_t t, size_t i, float (&x)[D / 32][16]) {
+    if (t == T_F32) {
         const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        float4 v[D / 32][4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float4 v = q[k];
-            x[4 * k] = v.x;
-            x[4 * k + 1] = v.y;
-            x[4 * k + 2] = v.z;
-            x[4 * k + 3] = v.w;
-        }
-    } else if (vec) {
-        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-        const uint4 a = q[0], b = q[1];
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        for (int s = 0; s < D / 32; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[s][k] = q[8 * s + k];
+#pragma unroll
+        for (int s = 0; s < D / 32; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[s][4 * k] = v[s][k].x;
+                x[s][4 * k + 1] = v[s][k].y;
+                x[s][4 * k + 2] = v[s][k].z;
+                x[s][4 * k + 3] = v[s][k].w;
+            }
+        return;
+    }
+    const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i);
+    u32x4 v[D / 32][2];
+#pragma unroll
+    for (int s = 0; s < D / 32; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) v[s][k] = q[4 * s + k];
+    const bool f16 = t == T_F16;
+#pragma unroll
+    for (int s = 0; s < D / 32; s++)
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            if (t == T_F16) {
-                const half2v h = as_h2(w[k]);
-                x[2 * k] = (float)h.x;
-                x[2 * k + 1] = (float)h.y;
-            } else {
-                x[2 * k] = __uint_as_float(w[k] << 16);
-                x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-            }
+            const uint32_t w = v[s][k >> 2][k & 3];
+            const half2v e = as_h2(w);
+            x[s][2 * k] = f16 ? (float)e.x : __uint_as_float(w << 16);
+            x[s][2 * k + 1] = f16 ? (float)e.y : __uint_as_float(w & 0xFFFF0000u);
         }
-    } else {
+}
+
+// A lane's accumulators times f: four consecutive values every 8 from value index i; vec: at
+// multiples of their size.
+template <int NT>
+__device__ __forceinline__ void store_row(void *p, uint32_t t, size_t i, bool vec, const f32x16 (&acc)[NT], float f, bool zero) {
+    auto at = [&](int k, int e) { return zero ? 0.0f : acc[k >> 2][4 * (k & 3) + e] * f; };
+    if (!vec) {
 #pragma unroll
-        for (int k = 0; k < 16; k++) x[k] = load_any(p, t, i + k);
+        for (int k = 0; k < 4 * NT; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) store_any(p, t, i + 8 * k + e, at(k, e));
+    } else if (t == T_F32) {
+        float *o = static_cast<float *>(p) + i;
+#pragma unroll
+        for (int k = 0; k < 4 * NT; k++) *reinterpret_cast<float4 *>(o + 8 * k) = make_float4(at(k, 0), at(k, 1), at(k, 2), at(k, 3));
+    } else if (t == T_F16) {
+        _Float16 *o = static_cast<_Float16 *>(p) + i;
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int k = 0; k < 4 * NT; k++)
+            *reinterpret_cast<half4 *>(o + 8 * k) = half4{(_Float16)at(k, 0), (_Float16)at(k, 1), (_Float16)at(k, 2), (_Float16)at(k, 3)};
+    } else {
+        uint16_t *o = static_cast<uint16_t *>(p) + i;
+#pragma unroll
+        for (int k = 0; k < 4 * NT; k++)
+            *reinterpret_cast<uint2 *>(o + 8 * k) =
+                make_uint2(bf16_of(at(k, 0)) | bf16_of(at(k, 1)) << 16, bf16_of(at(k, 2)) | bf16_of(at(k, 3)) << 16);
     }
 }
 
@@ -550,48 +586,56 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     float qs;
     {
         float x[NQ][16];
-        const size_t at = (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + xr) % G) * D;
+        const int half = A.a.rope.cs ? A.a.rope.half : 0;
+        // a row without a position reads row 0 of its call and the table, and is zeroed after: no
+        // load stands under a condition of its lane, all are in flight together
+        const size_t at = is ? (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + xr) % G) * D : 0;
+        const float *cs = A.a.rope.cs + (size_t)(is ? pos : 0) * half * 2;
+        if ((A.vec & 3) == 3 && half % 32 == 0) {
+            // pieces of 16 values: piece s of this lane turns with its own piece s + half / 32
+            load_row<D>(A.a.q, A.a.q_dtype, at + 16 * g, x);
+            if (half) {
+                float4 c[NQ / 2][8];
 #pragma unroll
-        for (int s = 0; s < NQ; s++) {
-            const int d = 32 * s + 16 * g;
+                for (int s = 0; s < NQ / 2; s++)
+                    if (s < half / 32)
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[s][j] = 0.0f;
-            if (!is) continue;
-            load16(A.a.q, A.a.q_dtype, at + d, A.vec & 1, x[s]);
-            const int half = A.a.rope.half;
-            if (!A.a.rope.cs || d >= 2 * half) continue;
-            const float *cs = A.a.rope.cs + (size_t)pos * half * 2;
-            float y[16], c[32];
-            if ((A.vec & 2) && half % 16 == 0) {  // the partners and the table's entries are whole pieces too
-                const bool lo = d < half;
-                const int k = lo ? d : d - half;
-                load16(A.a.q, A.a.q_dtype, at + (lo ? d + half : k), A.vec & 1, y);
+                        for (int j = 0; j < 8; j++) c[s][j] = reinterpret_cast<const float4 *>(cs + 2 * (32 * s + 16 * g))[j];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float4 v = reinterpret_cast<const float4 *>(cs + 2 * k)[j];
-                    c[4 * j] = v.x;
-                    c[4 * j + 1] = v.y;
-                    c[4 * j + 2] = v.z;
-                    c[4 * j + 3] = v.w;
-                }
+                for (int hs = 1; hs <= NQ / 2; hs++)  // half / 32, known in each copy
+                    if (half == 32 * hs)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const float xc = x[s][j] * c[2 * j], ys = y[j] * c[2 * j + 1];
-                    x[s][j] = lo ? xc - ys : ys + xc;
-                }
-            } else {
+                        for (int s = 0; s < hs; s++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int dd = d + j;
-                    if (dd >= 2 * half) continue;
-                    const bool lo = dd < half;
-                    const int k = lo ? dd : dd - half;
-                    const float p = load_any(A.a.q, A.a.q_dtype, at + (lo ? dd + half : k));
-                    const float xc = x[s][j] * cs[2 * k], ys = p * cs[2 * k + 1];
-                    x[s][j] = lo ? xc - ys : ys + xc;
-                }
+                            for (int j = 0; j < 16; j++) {
+                                const float4 v = c[s][j >> 1];
+                                const float co = j & 1 ? v.z : v.x, si = j & 1 ? v.w : v.y;
+                                const float p = x[s][j], r = x[s + hs][j];
+                                const float pc = p * co, rs = r * si, ps = p * si, rc = r * co;
+                                x[s][j] = pc - rs;
+                                x[s + hs][j] = ps + rc;
+                            }
             }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NQ; s++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int d = 32 * s + 16 * g + j;
+                    x[s][j] = load_any(A.a.q, A.a.q_dtype, at + d);
+                    if (d < 2 * half) {
+                        const bool lo = d < half;
+                        const int k = lo ? d : d - half;
+                        const float p = load_any(A.a.q, A.a.q_dtype, at + (lo ? d + half : k));
+                        const float xc = x[s][j] * cs[2 * k], ys = p * cs[2 * k + 1];
+                        x[s][j] = lo ? xc - ys : ys + xc;
+                    }
+                }
         }
+#pragma unroll
+        for (int s = 0; s < NQ; s++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[s][j] = is ? x[s][j] : 0.0f;
         float amax = 0.0f;
         bool bad = false;
 #pragma unroll
@@ -827,17 +871,10 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     if (w.n_ranges == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l * unit;
         const size_t at = (size_t)(q.r0 + tok) * A.a.out_stride + (size_t)(h * G + (x0 + xr) % G) * D + 4 * g;
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                store_any(A.a.out, A.a.out_dtype, at + 32 * i + 8 * (e >> 2) + (e & 3), l == 0.0f ? 0.0f : acc[i][e] * inv);
+        store_row<NT>(A.a.out, A.a.out_dtype, at, A.vec & 4, acc, inv, l == 0.0f);
     } else {
         float *part = A.a.parts + ((size_t)(w.slot + w.range) * A.P.heads + h) * (P_ROWS * (D + 2));
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) part[xr * D + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3)] = acc[i][e] * unit;
+        store_row<NT>(part, T_F32, (size_t)xr * D + 4 * g, (D + 2) * P_ROWS % 4 == 0, acc, unit, false);
         if (g == 0) {
             part[P_ROWS * D + xr] = m;
             part[P_ROWS * D + P_ROWS + xr] = l;
@@ -919,6 +956,7 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
                 const int size = a.q_dtype == T_F32 ? 4 : 2;
                 if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
                 if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
+                if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride * (a.out_dtype == T_F32 ? 4 : 2) % 16 == 0) A.vec |= 4;
             }
             // units of the part at most
             size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
