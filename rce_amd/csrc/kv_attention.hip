@@ -453,49 +453,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
 
 // ---- many query rows ------------------------------------------------------
 //
-// A block of four waves takes 128 query rows; a wave 32 of them as the columns
-// of 32x32 MFMAs.  The block shares each tile of 64 positions through LDS: the key
-// codes as they are, the values converted to binary16 once, both with their
-// 16-byte pieces in another order per row (row r's piece c lies at c ^ (r % 8): the
-// rows are 128 bytes, and reads of one piece of 32 rows would fall on the same banks).
-// The next tile's codes travel to registers meanwhile.
-//   S^T = K Q^T (int8, 32x32x32): operand row r of tile half t is position
-//         32 t + 16 (r / 4 % 2) + 4 (r / 8) + r % 4, so that lane (n, g = lane / 32)
-//         gets the 16 scores of one block, 2 t + g.
-//   O^T += V^T P^T (binary16, 32x32x16): again the lane's scores in order are its
-//         operand.
+// A block of eight waves takes 128 query rows, a wave 16 of them, with the
+// operand layouts of k_kv_attention.  The block shares each tile of 64 positions
+// through LDS: the key codes as they are, the values converted to binary16 once, both
+// with their 16-byte pieces in another order per row (else reads of one piece of
+// 16 rows would fall on the same banks).  The next tile's codes travel to registers meanwhile.
 // O stays in the MFMAs' accumulators, in units of `ref`, the largest value
 // scale so far, and of the row's m.  m moves, and O and l are rescaled, only when a
 // score passes it by more than LAG (base 2): weights are then at most 2^LAG,
 // times UP in binary16 at most 2^15.
-constexpr int P_ROWS = 128, P_WAVES = 4;
+// 16 rows and not 32 per wave: MFMAs, exponentials and the vector unit overlap only across
+// waves, and 16 rows fit 128 registers (four waves per SIMD; at the price of twice
+// the LDS reads per product).
+constexpr int P_ROWS = 128, P_WAVES = 8;
 constexpr float LAG = 6.0f, UP = 512.0f;  // UP = 2^9
 
-typedef int i32x16 __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ float half_max(float x) {  // over the lanes n and n + 32
-    const unsigned w = __builtin_bit_cast(unsigned, x);
-    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__builtin_bit_cast(float, (unsigned)q[0]), __builtin_bit_cast(float, (unsigned)q[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-    const unsigned w = __builtin_bit_cast(unsigned, x);
-    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return __builtin_bit_cast(float, (unsigned)q[0]) + __builtin_bit_cast(float, (unsigned)q[1]);
-}
-
-// Pieces of 16 values from value index i, one every 32: D / 32 of them, at multiples of 16 bytes.
-template <int D>
-__device__ __forceinline__ void load_row(const void *p, uint32_t t, size_t i, float (&x)[D / 32][16]) {
+// N pieces of 16 values from the value indexes i: at multiples of 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_pieces(const void *p, uint32_t t, const size_t (&i)[N], float (&x)[N][16]) {
     if (t == T_F32) {
-        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        float4 v[D / 32][4];
+        float4 v[N][4];
 #pragma unroll
-        for (int s = 0; s < D / 32; s++)
+        for (int s = 0; s < N; s++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[s][k] = q[8 * s + k];
+            for (int k = 0; k < 4; k++) v[s][k] = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i[s])[k];
 #pragma unroll
-        for (int s = 0; s < D / 32; s++)
+        for (int s = 0; s < N; s++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 x[s][4 * k] = v[s][k].x;
@@ -505,15 +488,14 @@ __device__ __forceinline__ void load_row(const void *p, uint32_t t, size_t i, fl
             }
         return;
     }
-    const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i);
-    u32x4 v[D / 32][2];
+    u32x4 v[N][2];
 #pragma unroll
-    for (int s = 0; s < D / 32; s++)
+    for (int s = 0; s < N; s++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) v[s][k] = q[4 * s + k];
+        for (int k = 0; k < 2; k++) v[s][k] = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i[s])[k];
     const bool f16 = t == T_F16;
 #pragma unroll
-    for (int s = 0; s < D / 32; s++)
+    for (int s = 0; s < N; s++)
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const uint32_t w = v[s][k >> 2][k & 3];
@@ -523,31 +505,31 @@ __device__ __forceinline__ void load_row(const void *p, uint32_t t, size_t i, fl
         }
 }
 
-// A lane's accumulators times f: four consecutive values every 8 from value index i; vec: at
-// multiples of their size.
+// A lane's accumulators times f: four consecutive values every 16 from value index i; vec:
+// at multiples of their size.
 template <int NT>
-__device__ __forceinline__ void store_row(void *p, uint32_t t, size_t i, bool vec, const f32x16 (&acc)[NT], float f, bool zero) {
-    auto at = [&](int k, int e) { return zero ? 0.0f : acc[k >> 2][4 * (k & 3) + e] * f; };
+__device__ __forceinline__ void store_row(void *p, uint32_t t, size_t i, bool vec, const f32x4 (&acc)[NT], float f, bool zero) {
+    auto at = [&](int k, int e) { return zero ? 0.0f : acc[k][e] * f; };
     if (!vec) {
 #pragma unroll
-        for (int k = 0; k < 4 * NT; k++)
+        for (int k = 0; k < NT; k++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) store_any(p, t, i + 8 * k + e, at(k, e));
+            for (int e = 0; e < 4; e++) store_any(p, t, i + 16 * k + e, at(k, e));
     } else if (t == T_F32) {
         float *o = static_cast<float *>(p) + i;
 #pragma unroll
-        for (int k = 0; k < 4 * NT; k++) *reinterpret_cast<float4 *>(o + 8 * k) = make_float4(at(k, 0), at(k, 1), at(k, 2), at(k, 3));
+        for (int k = 0; k < NT; k++) *reinterpret_cast<float4 *>(o + 16 * k) = make_float4(at(k, 0), at(k, 1), at(k, 2), at(k, 3));
     } else if (t == T_F16) {
         _Float16 *o = static_cast<_Float16 *>(p) + i;
         typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int k = 0; k < 4 * NT; k++)
-            *reinterpret_cast<half4 *>(o + 8 * k) = half4{(_Float16)at(k, 0), (_Float16)at(k, 1), (_Float16)at(k, 2), (_Float16)at(k, 3)};
+        for (int k = 0; k < NT; k++)
+            *reinterpret_cast<half4 *>(o + 16 * k) = half4{(_Float16)at(k, 0), (_Float16)at(k, 1), (_Float16)at(k, 2), (_Float16)at(k, 3)};
     } else {
         uint16_t *o = static_cast<uint16_t *>(p) + i;
 #pragma unroll
-        for (int k = 0; k < 4 * NT; k++)
-            *reinterpret_cast<uint2 *>(o + 8 * k) =
+        for (int k = 0; k < NT; k++)
+            *reinterpret_cast<uint2 *>(o + 16 * k) =
                 make_uint2(bf16_of(at(k, 0)) | bf16_of(at(k, 1)) << 16, bf16_of(at(k, 2)) | bf16_of(at(k, 3)) << 16);
     }
 }
@@ -560,16 +542,21 @@ struct PShared {
     int ok[4];                           // 0: no page
 };
 
+// Where piece c of a key row of position p lies: the 16 rows of an operand are 16 (m / 4) + m % 4 (+ 4 t).
+template <int D>
+__device__ __forceinline__ int key_piece(int p, int c) {
+    return D % 128 == 0 ? c ^ ((p & 3) | (p >> 2 & 4)) : c ^ ((p >> 1 & 1) | (p >> 3 & 2));
+}
+
 template <int D, bool HILO>
-__global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_kv_prompt(Args A) {
-    constexpr int NQ = D / 32, NT = D / 32;
+__global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k_kv_prompt(Args A, const int32_t *__restrict__ page_table) {
+    constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
     constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
-    constexpr int SWAP = D % 128 == 0 ? 7 : 3;  // a key row's pieces change places within groups of 8 or 4
-    constexpr int NK = TILE * D / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
+    constexpr int NK = (TILE * D + 16 * 64 * P_WAVES - 1) / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
     constexpr int BUFS = D <= 128 ? 2 : 1;  // two where they fit 64 KB
     __shared__ PShared<D> buf[BUFS];
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.P.heads;
     const int chunk = chunk_of(A);
@@ -578,7 +565,7 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     const KvSeq &q = w.q;
     const int G = A.G, first = q.first();
     const int x0 = w.unit * P_ROWS, n_x = min(P_ROWS, (q.r1 - q.r0) * G - x0);
-    const int xr = wave * 32 + n;  // this lane's row of the unit
+    const int xr = wave * 16 + n;  // this lane's row of the unit
     const int tok = (x0 + xr) / G, pos = first + tok;
     const bool is = xr < n_x && pos >= 0 && pos < A.B.cap;
 
@@ -587,41 +574,44 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     {
         float x[NQ][16];
         const int half = A.a.rope.cs ? A.a.rope.half : 0;
-        // a row without a position reads row 0 of its call and the table, and is zeroed after: no
-        // load stands under a condition of its lane, all are in flight together
+        // A row without a position reads row 0 of the call and of the table, and is zeroed after:
+        // no load stands under a condition of its lane, all are in flight together.
         const size_t at = is ? (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + xr) % G) * D : 0;
         const float *cs = A.a.rope.cs + (size_t)(is ? pos : 0) * half * 2;
-        if ((A.vec & 3) == 3 && half % 32 == 0) {
-            // pieces of 16 values: piece s of this lane turns with its own piece s + half / 32
-            load_row<D>(A.a.q, A.a.q_dtype, at + 16 * g, x);
+        if ((A.vec & 3) == 3 && half % 16 == 0) {  // the pieces' partners are whole pieces too
+            size_t own[NQ], other[NQ];
+#pragma unroll
+            for (int s = 0; s < NQ; s++) {
+                const int d = 64 * s + 16 * g;
+                own[s] = at + d;
+                other[s] = at + (d < half ? d + half : d < 2 * half ? d - half : d);
+            }
+            load_pieces<NQ>(A.a.q, A.a.q_dtype, own, x);
             if (half) {
-                float4 c[NQ / 2][8];
+                float y[NQ][16];
+                load_pieces<NQ>(A.a.q, A.a.q_dtype, other, y);
 #pragma unroll
-                for (int s = 0; s < NQ / 2; s++)
-                    if (s < half / 32)
+                for (int s = 0; s < NQ; s++) {
+                    const int d = 64 * s + 16 * g;
+                    const bool lo = d < half, turns = d < 2 * half;
+                    const float4 *c = reinterpret_cast<const float4 *>(cs + 2 * (lo ? d : turns ? d - half : 0));
 #pragma unroll
-                        for (int j = 0; j < 8; j++) c[s][j] = reinterpret_cast<const float4 *>(cs + 2 * (32 * s + 16 * g))[j];
-#pragma unroll
-                for (int hs = 1; hs <= NQ / 2; hs++)  // half / 32, known in each copy
-                    if (half == 32 * hs)
-#pragma unroll
-                        for (int s = 0; s < hs; s++)
-#pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                const float4 v = c[s][j >> 1];
-                                const float co = j & 1 ? v.z : v.x, si = j & 1 ? v.w : v.y;
-                                const float p = x[s][j], r = x[s + hs][j];
-                                const float pc = p * co, rs = r * si, ps = p * si, rc = r * co;
-                                x[s][j] = pc - rs;
-                                x[s + hs][j] = ps + rc;
-                            }
+                    for (int j = 0; j < 8; j++) {
+                        const float4 v = c[j];
+                        const float ac = x[s][2 * j] * v.x, as = y[s][2 * j] * v.y;
+                        const float bc = x[s][2 * j + 1] * v.z, bs = y[s][2 * j + 1] * v.w;
+                        const float a = lo ? ac - as : as + ac, b = lo ? bc - bs : bs + bc;
+                        x[s][2 * j] = turns ? a : x[s][2 * j];
+                        x[s][2 * j + 1] = turns ? b : x[s][2 * j + 1];
+                    }
+                }
             }
         } else {
 #pragma unroll
             for (int s = 0; s < NQ; s++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const int d = 32 * s + 16 * g + j;
+                    const int d = 64 * s + 16 * g + j;
                     x[s][j] = load_any(A.a.q, A.a.q_dtype, at + d);
                     if (d < 2 * half) {
                         const bool lo = d < half;
@@ -632,21 +622,18 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
                     }
                 }
         }
-#pragma unroll
-        for (int s = 0; s < NQ; s++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[s][j] = is ? x[s][j] : 0.0f;
         float amax = 0.0f;
         bool bad = false;
 #pragma unroll
         for (int s = 0; s < NQ; s++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
+                x[s][j] = is ? x[s][j] : 0.0f;
                 amax = fmaxf(amax, fabsf(x[s][j]));
                 bad |= !(fabsf(x[s][j]) < __builtin_inff());
             }
-        amax = half_max(amax);
-        bad = half_max(bad ? 1.0f : 0.0f) != 0.0f;
+        amax = swap_max(amax);
+        bad = swap_max(bad ? 1.0f : 0.0f) != 0.0f;
         const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
         qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
 #pragma unroll
@@ -655,7 +642,7 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
 
     const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;
     // the wave's rows: positions that all of them see, or that any of them sees
-    const int w0 = wave * 32, w_n = min(32, n_x - w0);  // rows (none: w_n <= 0)
+    const int w0 = wave * 16, w_n = min(16, n_x - w0);  // rows (none: w_n <= 0)
     const int f0 = first + (x0 + w0) / G, f1 = first + (x0 + w0 + max(w_n, 1) - 1) / G;
     const bool placed = w_n > 0 && f0 >= 0 && f1 < A.B.cap;
     const int w_lo = max(0, f0 - (A.a.window - 1)), w_hi = w_n > 0 ? min(f1, A.B.cap - 1) : -1;
@@ -665,39 +652,42 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
     t_lo = max(t_lo, w.sp.t0 + w.range * w.step);
     t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * w.step);
-    const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
+    const int32_t *__restrict__ pages = page_table + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
 
     // What this thread moves: piece tid + 256 i of the tile's keys (position / (D / 16), 16
-    // codes) and of its values (dimension and block: 16 positions); pieces i of
-    // all threads lie in one block for D = 256, in 4 / NK of them else.
+    // codes) and of its values (dimension and block: 16 positions).  A wave's pieces i lie in one
+    // block: page ids and block addresses are scalar.
     constexpr int BP = D;  // pieces of a block: 16 positions x D codes / 16
+    static_assert(BP % 64 == 0, "a wave's pieces lie in one block");
     u32x4 kr[NK], vr[NK];
     float ksr = 0.0f, vsr = 0.0f;
     int pg[NK], pgs = 0, oks = 0;  // the next tile's page ids, loaded a tile ahead
+    auto mine = [&](int i) { return 4 * BP % (64 * P_WAVES) == 0 || wave * 64 + 64 * P_WAVES * i < 4 * BP; };  // the same in a wave
     auto block_of = [&](int t, int b) { return min(4 * t + b, max_block); };
     auto look = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < NK; i++) pg[i] = pages[block_of(t, (tid + 64 * P_WAVES * i) / BP) >> A.P.lg_b];
+        for (int i = 0; i < NK; i++)
+            if (mine(i)) pg[i] = pages[block_of(t, (wave * 64 + 64 * P_WAVES * i) / BP) >> A.P.lg_b];
         if (tid < 4) pgs = pages[block_of(t, tid) >> A.P.lg_b];
     };
     auto block_at = [&](int page, int blk) -> uint32_t {  // page 0 where there is none
         const uint32_t p = (unsigned)page < (unsigned)A.P.n_pages ? page : 0;
         return ((p * (uint32_t)A.P.heads + (uint32_t)h) << A.P.lg_b) + (uint32_t)(blk & bmask);
     };
-    const int8_t *const k_at = A.P.k + tid % BP * 16, *const v_at = A.P.v + tid % BP * 16;
-    static_assert(64 * P_WAVES % BP == 0 || D == 192, "a thread's pieces lie at one place of their blocks");
     auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int e = tid + 64 * P_WAVES * i, b = e / BP;
-            size_t at = (size_t)block_at(pg[i], block_of(t, b)) * (16 * D);
-            if constexpr (64 * P_WAVES % BP != 0) at += (e % BP - tid % BP) * 16;
-            kr[i] = *reinterpret_cast<const u32x4 *>(k_at + at);
-            vr[i] = *reinterpret_cast<const u32x4 *>(v_at + at);
+            if (!mine(i)) continue;
+            const int e = wave * 64 + 64 * P_WAVES * i, b = e / BP;
+            const size_t at = (size_t)block_at(pg[i], block_of(t, b)) * (16 * D) + e % BP * 16;
+            kr[i] = *reinterpret_cast<const u32x4 *>(A.P.k + at + 16u * lane);
+            vr[i] = *reinterpret_cast<const u32x4 *>(A.P.v + at + 16u * lane);
         }
         if (tid < 4) {
-            const size_t blk = block_at(pgs, block_of(t, tid));
+            int b = tid;
+            asm volatile("" : "+v"(b));  // as below
+            const uint32_t blk = block_at(pgs, block_of(t, b));
             ksr = A.P.k_scale[blk];
             vsr = A.P.v_scale[blk];
             oks = (unsigned)pgs < (unsigned)A.P.n_pages;
@@ -706,10 +696,11 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
     auto place = [&](PShared<D> &to) {
 #pragma unroll
         for (int i = 0; i < NK; i++) {
+            if (!mine(i)) continue;
             const int e = tid + 64 * P_WAVES * i, b = e / BP, r = e % BP;
             {  // keys: position 16 b + r / (D / 16), piece r % (D / 16)
                 const int p = 16 * b + r / (D / 16), c = r % (D / 16);
-                *reinterpret_cast<u32x4 *>(to.k + p * D + (c ^ (p & SWAP)) * 16) = kr[i];
+                *reinterpret_cast<u32x4 *>(to.k + p * D + key_piece<D>(p, c) * 16) = kr[i];
             }
             {  // values: dimension r, positions 16 b .. + 15: pieces 2 b, 2 b + 1
                 half2v a[8];
@@ -727,14 +718,14 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
         }
     };
 
-    f32x16 acc[NT];
+    f32x4 acc[NT];
 #pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
+    for (int i = 0; i < NT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f, ref = 0.0f, inv_ref = 0.0f;
-    // K operand row n of tile half t: its position there
-    const int kpos = 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3);
+    // This lane's operands in LDS: key position 16 (n / 4) + n % 4 + 4 i, piece 4 s + g, and value
+    // row n + 16 i, piece 2 g + u.
+    const int k_pos = 16 * (n >> 2) + (n & 3);
+    const int k_row0 = k_pos * D + key_piece<D>(k_pos, g) * 16, v_row0 = n * TILE + (2 * g ^ (n & 7)) * 8;
     if (t_lo < t_hi) {
         look(t_lo);
         fetch(t_lo);
@@ -749,112 +740,111 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
         if (TILE * t <= w_hi && TILE * t + TILE - 1 >= w_lo) {  // some row of the wave sees it (the same in all lanes)
             const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
             const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
+            // opaque: what is formed from them would be kept over the loop, in registers that spill
+            int k_row = k_row0, v_row = v_row0, my = lane;
+            asm volatile("" : "+v"(k_row), "+v"(v_row), "+v"(my));
+            int xi[16];  // scores as whole numbers (HILO: without the highest limb, which is xh)
+            float xh[HILO ? 16 : 1];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {  // 32 positions at a time: half the registers
-                int xi[16];  // scores as whole numbers (HILO: without the highest limb)
-                float xh[HILO ? 16 : 1];
-                {
-                    i32x16 c[LIMBS];
+            for (int i = 0; i < 4; i++) {
+                i32x4 c[LIMBS];
 #pragma unroll
-                    for (int b = 0; b < LIMBS; b++)
+                for (int b = 0; b < LIMBS; b++) c[b] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int e = 0; e < 16; e++) c[b][e] = 0;
-                    const int p = 32 * u + kpos;
+                for (int s = 0; s < NQ; s++) {
+                    // key_piece of a row 4 i on is the same, of a piece 4 s on 64 s bytes on (all but bit 2 of
+                    // the piece stays)
+                    const int8_t *at = sh.k + (D % 128 == 0 ? (k_row ^ (s & 1) * 64) + (s >> 1) * 128 : k_row + 64 * s) + 4 * i * D;
+                    const i32x4 a = *reinterpret_cast<const i32x4 *>(at);
 #pragma unroll
-                    for (int s = 0; s < NQ; s++) {
-                        const i32x4 a = *reinterpret_cast<const i32x4 *>(sh.k + p * D + ((2 * s + g) ^ (p & SWAP)) * 16);
-#pragma unroll
-                        for (int b = 0; b < LIMBS; b++) c[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, qf[s][b], c[b], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        xi[e] = c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e];
-                        if constexpr (HILO) xh[e] = (float)c[0][e] * 65536.0f;
-                    }
-                }
-                auto score = [&](int e) { return HILO ? xh[HILO ? e : 0] + (float)xi[e] : (float)xi[e]; };
-                const float f = sh.ks[2 * u + g] * qs;
-                float sv = sh.vs[2 * u + g], top;
-                uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
-                if (HILO || masked) {
-                    if (masked) {
-                        const int p = TILE * t + 32 * u + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
-                        seen = sh.ok[2 * u + g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
-                        // a block that no row of the wave sees may hold anything
-                        if (!((__ballot(seen != 0) >> (32 * g)) & 0xFFFFFFFFull)) sv = 0.0f;
-                    }
-                    asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
-                    top = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
-                } else {
-                    int x = xi[0];
-#pragma unroll
-                    for (int e = 1; e < 16; e++) x = max(x, xi[e]);
-                    top = (float)x * f;
-                }
-                top = half_max(top);
-                // `top` above m + LAG, or a larger value scale: rescale
-                const bool fin = sv < __builtin_inff();
-                const float scale = half_max(fin ? sv : 0.0f);
-                if (__ballot(top > m + LAG) || scale > ref) {
-                    const float m_new = top > m + LAG ? top : m, ref_new = fmaxf(ref, scale);
-                    const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
-                    const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
-                    l *= alpha;
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) acc[i][e] *= back;
-                    m = m_new;
-                    ref = ref_new;
-                    inv_ref = ref > 0.0f ? UP / ref : 0.0f;
-                }
-                const float base = m == -INFINITY ? 0.0f : m;
-                // what the values' scale makes of the weights; an infinite or NaN one makes NaN
-                // of the rows that see its block, no others
-                const float pw = fin ? sv * inv_ref : sv;
-                half8 ph[2], pl[2];
-                // The ordinary case: no mask, value scales above 2^-12 of `ref`.  The scale goes
-                // into the exponent, l gets the sum of the rounded weights (dot products with
-                // ones) over it.  Two terms (HILO) and all else take the longer way.
-                if (!HILO && !masked && !__ballot(!(pw >= 0.125f && pw < 2.0f * UP))) {
-                    const float lw = __builtin_amdgcn_logf(pw), off = lw - base;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const half2v p = {(_Float16)exp2_(__builtin_fmaf((float)xi[e], f, off)),
-                                          (_Float16)exp2_(__builtin_fmaf((float)xi[e + 1], f, off))};
-                        sum = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
-                        ph[e >> 3][e & 7] = p.x;
-                        ph[e >> 3][(e & 7) + 1] = p.y;
-                    }
-                    l = __builtin_fmaf(sum, exp2_(-lw), l);
-                } else {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const bool see = seen >> e & 1;
-                        const float y = see ? exp2_(score(e) * f - base) : 0.0f, p = see ? y * pw : 0.0f;
-                        sum += y;
-                        const _Float16 hi = (_Float16)p;
-                        ph[e >> 3][e & 7] = hi;
-                        if constexpr (HILO) pl[e >> 3][e & 7] = (_Float16)(p - (float)hi);
-                    }
-                    l += sum;
+                    for (int b = 0; b < LIMBS; b++) c[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, qf[s][b], c[b], 0, 0, 0);
                 }
 #pragma unroll
-                for (int k = 0; k < 2; k++) {  // 16 positions: 32 u + 16 g + 8 k ...
-                    const int piece = 4 * u + 2 * g + k;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        const int d = 32 * i + n;
-                        const half8 a = *reinterpret_cast<const half8 *>(sh.v + d * TILE + (piece ^ (d & 7)) * 8);
-                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[k], acc[i], 0, 0, 0);
-                        if constexpr (HILO) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[k], acc[i], 0, 0, 0);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    xi[4 * i + e] = c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e];
+                    if constexpr (HILO) xh[4 * i + e] = (float)c[0][e] * 65536.0f;
                 }
             }
+            auto score = [&](int e) { return HILO ? xh[HILO ? e : 0] + (float)xi[e] : (float)xi[e]; };
+            const float f = sh.ks[g] * qs;
+            float sv = sh.vs[g], top = -INFINITY;
+            uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
+            if (HILO || masked) {
+                if (masked) {
+                    const int p = TILE * t + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
+                    seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
+                    // a block that no row of the wave sees may hold anything
+                    const unsigned long long b = __ballot(seen != 0);
+                    const uint32_t half = my < 32 ? (uint32_t)b : (uint32_t)(b >> 32);
+                    if (!(half >> (my & 16) & 0xFFFFu)) sv = 0.0f;
+                }
+                asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+            } else {
+                int x = xi[0];
+#pragma unroll
+                for (int e = 1; e < 16; e++) x = max(x, xi[e]);
+                top = (float)x * f;
+            }
+            top = swap_max(top);
+            // `top` above m + LAG, or a larger value scale: rescale
+            const bool fin = sv < __builtin_inff();
+            const float scale = swap_max(fin ? sv : 0.0f);
+            if (__ballot(top > m + LAG) || scale > ref) {
+                const float m_new = top > m + LAG ? top : m, ref_new = fmaxf(ref, scale);
+                const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
+                const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][e] *= back;
+                m = m_new;
+                ref = ref_new;
+                inv_ref = ref > 0.0f ? UP / ref : 0.0f;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            // what the values' scale makes of the weights; an infinite or NaN one makes NaN of the
+            // rows that see its block, no others
+            const float pw = fin ? sv * inv_ref : sv;
+            half8 ph[2], pl[2];
+            // The ordinary tile: no mask, value scales above 2^-12 of `ref`.  The scale goes into the
+            // exponent, l gets the sum of the rounded weights (dot products with ones) over it.
+            // Two terms (HILO) and all else take the longer way.
+            if (!HILO && !masked && !__ballot(!(pw >= 0.125f && pw < 2.0f * UP))) {
+                const float lw = __builtin_amdgcn_logf(pw), off = lw - base;
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const half2v p = {(_Float16)exp2_(__builtin_fmaf((float)xi[e], f, off)),
+                                      (_Float16)exp2_(__builtin_fmaf((float)xi[e + 1], f, off))};
+                    sum = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                    ph[e >> 3][e & 7] = p.x;
+                    ph[e >> 3][(e & 7) + 1] = p.y;
+                }
+                l = __builtin_fmaf(sum, exp2_(-lw), l);
+            } else {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const bool see = seen >> e & 1;
+                    const float y = see ? exp2_(score(e) * f - base) : 0.0f, p = see ? y * pw : 0.0f;
+                    sum += y;
+                    const _Float16 hi = (_Float16)p;
+                    ph[e >> 3][e & 7] = hi;
+                    if constexpr (HILO) pl[e >> 3][e & 7] = (_Float16)(p - (float)hi);
+                }
+                l += sum;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)  // positions 16 g + 8 u ...
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const half8 a = *reinterpret_cast<const half8 *>(sh.v + (v_row ^ u * 8) + 16 * i * TILE);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[u], acc[i], 0, 0, 0);
+                    if constexpr (HILO) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[u], acc[i], 0, 0, 0);
+                }
         }
         if constexpr (BUFS == 1) __syncthreads();
         if (t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
@@ -864,8 +854,8 @@ __global__ __launch_bounds__(64 * P_WAVES, (D <= 128 && !HILO) ? 2 : 1) void k_k
         }
         __syncthreads();
     }
-    // lane (n, g) holds dimensions 32 i + 8 j + 4 g + e of its row
-    l = half_sum(l);
+    // lane (n, g) holds dimensions 16 i + 4 g + e of its row
+    l = swap_sum(l);
     if (xr >= n_x) return;
     const float unit = ref * (1.0f / UP);
     if (w.n_ranges == 1) {
@@ -964,8 +954,8 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
             const bool split = rows.cap > MIN_CHUNK * TILE;
             const dim3 grid((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
             const bool f32 = a.out_dtype == T_F32;
-            if (many && f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A);
-            else if (many) hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A);
+            if (many && f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
+            else if (many) hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
             else if (f32) hipLaunchKernelGGL((k_kv_attention<D, true>), grid, dim3(64 * WAVES), 0, s, A);
             else hipLaunchKernelGGL((k_kv_attention<D, false>), grid, dim3(64 * WAVES), 0, s, A);
             if (split) hipLaunchKernelGGL((k_kv_join<D>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
