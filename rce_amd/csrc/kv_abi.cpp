@@ -278,7 +278,7 @@ rce_qmm_status rce_qmm_sample_dev(rce_qmm_context *ctx, const void *logits_dev, 
                               (const void *)p.min_p, (const void *)ids_dev, (const void *)probs_dev})
             if (!aligned(x, 4)) return fail(RCE_QMM_BAD_SHAPE, "arrays of one value per row must be 4-byte aligned");
         const SampleRows r{logits_dev, dtype, n_rows, vocab, row_stride, p.u, p.temperature, p.top_p, p.min_p, p.top_k,
-                           ids_dev, probs_dev};
+                           ids_dev, probs_dev, ctx->kv_parts.p};
         OnDevice dev(ctx->device);
         HIP_TRY(dev.error());
         HIP_TRY(launch_sample(r, stream ? static_cast<hipStream_t>(stream) : ctx->stream));

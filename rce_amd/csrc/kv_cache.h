@@ -57,7 +57,10 @@ struct SampleRows {
     const int32_t *top_k;
     int32_t *ids;
     float *probs;
+    void *split;  // sample_split_bytes(), 16-byte aligned
 };
+// Room for rows that several blocks share, whatever the call.
+size_t sample_split_bytes();
 hipError_t launch_sample(const SampleRows &r, hipStream_t s);
 
 #ifdef __HIPCC__

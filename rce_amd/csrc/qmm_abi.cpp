@@ -345,7 +345,7 @@ rce_qmm_status rce_qmm_context_create(int device, rce_qmm_context **out) {
     c->device = device;
     c->stream = s;
     if ((st = ensure(c, c->parts, rce_qmm::gemm_f16_parts_bytes(), nullptr)) ||
-        (st = ensure(c, c->kv_parts, rce_qmm::kv_attention_parts_bytes(), nullptr))) {
+        (st = ensure(c, c->kv_parts, std::max(rce_qmm::kv_attention_parts_bytes(), rce_qmm::sample_split_bytes()), nullptr))) {
         context_release(c);
         return st;
     }

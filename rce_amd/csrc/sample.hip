@@ -25,6 +25,8 @@
 #include "kv_cache.h"
 #include "lds_limit.h"
 
+#include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace rce_qmm {
@@ -165,12 +167,16 @@ struct Weight {
     __device__ __forceinline__ u64 operator()(const Shared &sh, float l) const { return whole(value(sh, l)); }
 };
 
+// Steps of a run: so many that a row has at most RUNS.
+__host__ __device__ constexpr int row_q(size_t vocab) { return (int)((vocab + RUNS * 64 * STEP - 1) / (RUNS * 64 * STEP)); }
+
 // The row's logits.  A lane's step is STEP consecutive ids, a run q steps of a wave;
-// run s * NW + wave is the wave's s-th.
+// run run0 + s * NW + wave is the wave's s-th.
 template <class T, bool LDS>
 struct Row {
     T *copy;  // in LDS: NaN as -inf, -0 as 0, -inf past the end up to a whole number of steps
     int n, q, segs;
+    int run0;  // of the block's slice of the row
     // In device memory, as a buffer whose loads return 0 past the row's end (a 16-bit row's end
     // rounded up to a dword).  words: the row starts at a dword.
     __amdgpu_buffer_rsrc_t mem;
@@ -221,16 +227,16 @@ struct Row {
         const int wave = threadIdx.x >> 6;
         float l[STEP];
         if constexpr (LDS) {
-            int id = first(wave, 0);
+            int id = first(run0 + wave, 0);
             for (int s = 0; s < segs; s++, id += NT * STEP) {
-                g(s * NW + wave);
+                g(run0 + s * NW + wave);
                 values(id, l);
                 f(id, l);
             }
         } else {
-            Quad next = load(first(wave, 0));
+            Quad next = load(first(run0 + wave, 0));
             for (int s = 0; s < segs; s++) {
-                const int run = s * NW + wave;
+                const int run = run0 + s * NW + wave;
                 g(run);
                 for (int j = 0; j < q; j++) {
                     const int id = first(run, j);
@@ -240,7 +246,7 @@ struct Row {
                 }
             }
         }
-        g(segs * NW + wave);
+        g(run0 + segs * NW + wave);
     }
     template <class F>
     __device__ __forceinline__ void each(F f) const {
@@ -337,6 +343,18 @@ struct Kept {
     double want;
 };
 
+// The last kept one of a bin's n elements, v of thread tid by place: where the sum passes `want`.
+template <bool WEIGHTS>
+__device__ __forceinline__ Keep end_of(Shared &sh, const Weight &W, u64 v, int n, u64 before, double want) {
+    const int tid = threadIdx.x;
+    const u64 w = tid < n ? (WEIGHTS ? W(sh, logit_of(v)) : 1) : 0;
+    u64 sum;
+    const u64 ahead = before + block_scan(sh, w, sum);
+    if (tid < n && (double)ahead < want && (double)(ahead + w) >= want) sh.at = v;
+    __syncthreads();
+    return keep_to(sh.at);
+}
+
 // Keep only a prefix: the first `count` elements (WEIGHTS false), or the shortest one whose
 // weights reach the share `p` of all kept ones'.  limited: the last bin holds only
 // weights of 0.  Where the result is a list, it holds more: the cut is still to be made.
@@ -397,12 +415,7 @@ __device__ __forceinline__ void cut(Shared &sh, const R &row, const Bins &bins, 
     }
     if (n <= NT) {
         const u64 v = block_sort(sh, tid < n ? sh.list[tid] : ~0ull, n);
-        const u64 w = tid < n ? (WEIGHTS ? W(sh, logit_of(v)) : 1) : 0;
-        u64 sum;
-        const u64 ahead = before + block_scan(sh, w, sum);
-        if (tid < n && (double)ahead < want && (double)(ahead + w) >= want) sh.at = v;
-        __syncthreads();
-        K.keep = keep_to(sh.at);
+        K.keep = end_of<WEIGHTS>(sh, W, v, n, before, want);
         return;
     }
     // radix descent over the places
@@ -441,40 +454,62 @@ __device__ __forceinline__ u64 target(float u, u64 total) {
     return t < total ? t : total - 1;
 }
 
-template <class T, bool LDS>
-__global__ __launch_bounds__(NT, LDS ? 8 : 4) void k_sample(SampleRows R, int S) {
-    extern __shared__ __align__(16) unsigned char lds[];
-    Shared &sh = *reinterpret_cast<Shared *>(lds);
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Row<T, LDS> row;
-    row.copy = reinterpret_cast<T *>(lds + sizeof(Shared));
-    row.n = (int)R.vocab;
-    row.q = LDS ? 1 : (row.n + RUNS * 64 * STEP - 1) / (RUNS * 64 * STEP);
-    row.segs = (row.n + row.q * NT * STEP - 1) / (row.q * NT * STEP);
-    row.bind(static_cast<const T *>(R.logits) + (size_t)r * R.stride);
-    const float temp = R.temperature ? R.temperature[r] : 1.0f;
-    const float min_p = R.min_p ? R.min_p[r] : 0.0f;
-    const float top_p = R.top_p ? R.top_p[r] : 1.0f;
-    const int top_k = R.top_k ? R.top_k[r] : 0;
-    const float u = R.u[r];
+// A row's filters, and what follows from its largest and smallest logit.
+struct Filters {
+    float temp, min_p, top_p;
+    int top_k;
+    bool by_count, by_weight, limited;  // limited: the last bin holds only weights of 0
+    Weight W;
+    Bins bins;
+    double least;
+    __device__ __forceinline__ void read(const SampleRows &R, int r) {
+        temp = R.temperature ? R.temperature[r] : 1.0f;
+        min_p = R.min_p ? R.min_p[r] : 0.0f;
+        top_p = R.top_p ? R.top_p[r] : 1.0f;
+        top_k = R.top_k ? R.top_k[r] : 0;
+        by_count = top_k > 0 && (size_t)top_k < R.vocab;
+        by_weight = top_p < 1.0f;
+    }
+    // the most likely token
+    __device__ __forceinline__ bool greedy() const { return !(temp > 0.0f) || min_p > 1.0f || top_p <= 0.0f || top_k == 1; }
+    __device__ __forceinline__ void range(float hi, float lo, int S) {
+        W.max = hi;
+        W.c = 1.4426950408889634 / (double)temp;
+        W.S = S;
+        W.low = -(double)(S + 2);
+        // Bins over the logits that have weight, or all of them if those span less.
+        const double span = (double)(S + 3) / W.c, wide = (double)hi - (double)lo;
+        limited = !(wide < span);
+        bins = {hi, (float)fmin(fmax((double)BINS / (limited ? span : wide), 0x1p-118), 0x1p100)};
+        least = min_p > 0.0f ? __builtin_ldexp((double)min_p, S) : 0.0;
+    }
+};
 
-    // the largest and the smallest finite logit
-    float hi = -INFINITY, lo = INFINITY;
-    constexpr int U = 8;
+// The largest and the smallest finite logit of this thread's (in all, of the row or
+// slice); id: the lowest of the largest (ID).  A row kept in LDS is copied there.
+template <bool ID, class T, bool LDS>
+__device__ __forceinline__ void extremes(const Row<T, LDS> &row, float &hi, float &lo, int &id_hi) {
+    const int tid = threadIdx.x;
+    hi = -INFINITY;
+    lo = INFINITY;
+    id_hi = INT_MAX;
+    constexpr int U = ID ? 4 : 8;
     using Quad = typename Row<T, LDS>::Quad;
-    const int steps = row.segs * row.q;
+    const int steps = row.segs * row.q, id0 = row.run0 * row.q * (64 * STEP);
+    auto id_of = [&](int step) { return !ID || step < steps ? id0 + (step * NT + tid) * STEP : row.n; };  // past the row's end: nothing
     for (int s = 0; s < steps; s += U) {
         Quad v[U];
 #pragma unroll
-        for (int k = 0; k < U; k++) v[k] = row.load(((s + k) * NT + tid) * STEP);
+        for (int k = 0; k < U; k++) v[k] = row.load(id_of(s + k));
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            const int id = ((s + k) * NT + tid) * STEP;
+            const int id = id_of(s + k);
             float l[STEP];
             row.unpack(id, v[k], l);
             Quad c;
 #pragma unroll
             for (int e = 0; e < STEP; e++) {
+                if constexpr (ID) id_hi = l[e] > hi ? id + e : id_hi;
                 hi = fmaxf(hi, l[e]);
                 lo = fminf(lo, l[e] > -INFINITY ? l[e] : INFINITY);
                 narrow(l[e], c.t[e]);
@@ -483,20 +518,253 @@ __global__ __launch_bounds__(NT, LDS ? 8 : 4) void k_sample(SampleRows R, int S)
                 if (s + k < steps) *reinterpret_cast<Quad *>(row.copy + id) = c;
         }
     }
-    if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
-    const float hi_t = hi;  // this thread's
+}
+
+template <class T, bool LDS>
+__device__ __forceinline__ void bind_row(Row<T, LDS> &row, const SampleRows &R, int r, T *copy) {
+    row.copy = copy;
+    row.n = (int)R.vocab;
+    row.q = LDS ? 1 : row_q(R.vocab);
+    row.segs = (row.n + row.q * NT * STEP - 1) / (row.q * NT * STEP);
+    row.run0 = 0;
+    row.bind(static_cast<const T *>(R.logits) + (size_t)r * R.stride);
+}
+
+// ---- a row over several blocks --------------------------------------------
+//
+// Few long rows leave most CUs without work in a block per row, so slices of
+// whole runs get a block each in three kernels: the slices' largest and smallest
+// logits; their histograms, added up in device memory; the elements of the bin
+// where the kept ones end (of all bins up to it, if they are few) and
+// the runs' sums of what is kept for certain.  k_sample goes on from there with a
+// block per row.  Rows with both filters and more than NT elements up to the end of
+// top-k, and a bin of more than NT, are left to its own passes.
+constexpr int MAX_SLICES = 64;
+struct SplitRow {
+    u64 hist[BINS], list[NT], runs[RUNS];
+    struct {
+        float hi, lo;
+        int id;
+    } slice[MAX_SLICES];
+    int n;
+};
+constexpr int SPLIT_ROWS = 256, SPLIT_BLOCKS = 512;  // rows of a split call; blocks to make of them (two per CU)
+struct Split {
+    SplitRow *rows;
+    int slices, runs;  // runs of a slice: a multiple of NW
+};
+
+template <class T>
+__device__ __forceinline__ Row<T, false> slice_of(const SampleRows &R, const Split &P) {
+    Row<T, false> row;
+    bind_row<T, false>(row, R, blockIdx.y, nullptr);
+    row.run0 = blockIdx.x * P.runs;
+    row.segs = P.runs / NW;
+    return row;
+}
+
+__device__ __forceinline__ void join_slices(const SplitRow &W, const Split &P, float &hi, float &lo, int &id) {
+    const int lane = threadIdx.x & 63;
+    const bool is = lane < P.slices;
+    const float h = is ? W.slice[lane].hi : -INFINITY;
+    hi = wave_max(h);
+    lo = -wave_max(is ? -W.slice[lane].lo : -INFINITY);
+    const u64 m = __ballot(is && h == hi);  // the first slice of these
+    id = m ? W.slice[__builtin_ctzll(m)].id : -1;
+}
+
+template <class T>
+__global__ __launch_bounds__(NT, 8) void k_sample_extremes(SampleRows R, Split P) {
+    __shared__ float red[2 * NW];
+    __shared__ int first;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    SplitRow &W = P.rows[blockIdx.y];
+    for (int i = blockIdx.x * NT + tid; i < BINS; i += P.slices * NT) W.hist[i] = 0;
+    if (blockIdx.x == 0 && tid == 0) W.n = 0;
+    float hi, lo;
+    int id;
+    extremes<true>(slice_of<T>(R, P), hi, lo, id);
+    const float own = hi;
     hi = wave_max(hi);
     lo = -wave_max(-lo);
     if (lane == 0) {
-        sh.red[wave] = hi;
-        sh.red[NW + wave] = lo;
+        red[wave] = hi;
+        red[NW + wave] = lo;
     }
-    if (tid == 0) sh.at = ~0ull;
+    if (tid == 0) first = INT_MAX;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; w++) {
-        hi = fmaxf(hi, sh.red[w]);
-        lo = fminf(lo, sh.red[NW + w]);
+        hi = fmaxf(hi, red[w]);
+        lo = fminf(lo, red[NW + w]);
+    }
+    if (own == hi && hi > -INFINITY) atomicMin(&first, id);
+    __syncthreads();
+    if (tid == 0) {
+        W.slice[blockIdx.x].hi = hi;
+        W.slice[blockIdx.x].lo = lo;
+        W.slice[blockIdx.x].id = first;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(NT, 8) void k_sample_bins(SampleRows R, Split P, int S) {
+    __shared__ Shared sh;
+    const int tid = threadIdx.x;
+    SplitRow &W = P.rows[blockIdx.y];
+    Filters f;
+    f.read(R, blockIdx.y);
+    float hi, lo;
+    int id_hi;
+    join_slices(W, P, hi, lo, id_hi);
+    if (hi == -INFINITY || f.greedy() || !(f.by_count || f.by_weight)) return;
+    f.range(hi, lo, S);
+    if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
+#pragma unroll
+    for (int i = 0; i < PER; i++) sh.hist[i * NT + tid] = 0;
+    __syncthreads();
+    slice_of<T>(R, P).each([&](int, const float(&l)[STEP]) {
+#pragma unroll
+        for (int e = 0; e < STEP; e++)
+            if (l[e] > -INFINITY) atomicAdd(&sh.hist[f.bins.of(l[e])], f.by_count ? 1ull : f.W(sh, l[e]));
+    });
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int b = i * NT + tid;
+        if (sh.hist[b]) atomicAdd(&W.hist[b], sh.hist[b]);
+    }
+}
+
+// How a split row goes on, from its histogram (of counts, without top-k of weights); the same in every block.
+struct Plan {
+    enum { EVERY, LIST, BIN, SLOW } mode;  // no cut; the list of the bins 0 .. bin, or of `bin` alone; k_sample's own passes
+    int bin;
+    u64 before;
+    double want;
+};
+__device__ __forceinline__ Plan plan(Shared &sh, const SplitRow &W, const Filters &f) {
+    if (!(f.by_count || f.by_weight)) return {Plan::EVERY, BINS, 0, 0.0};
+    const int tid = threadIdx.x;
+    u64 h[PER], mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; i++) mine += h[i] = W.hist[PER * tid + i];
+    if (tid == 0) sh.bin = -1;
+    u64 run = block_scan(sh, mine, total);
+    const double want = f.by_count ? (double)f.top_k : (double)f.top_p * (double)total;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if ((double)run < want && (double)(run + h[i]) >= want) {
+            sh.bin = PER * tid + i;
+            sh.before = run;
+            sh.at = run + h[i];
+        }
+        run += h[i];
+    }
+    __syncthreads();
+    const bool cut = sh.bin >= 0 && !(f.limited && sh.bin == BINS - 1);
+    if (f.by_count && cut && sh.at <= (u64)NT) return {Plan::LIST, sh.bin, 0, 0.0};
+    if (f.by_count && f.by_weight) return {Plan::SLOW, BINS, 0, 0.0};
+    if (!cut) return {Plan::EVERY, BINS, 0, 0.0};
+    return {Plan::BIN, sh.bin, sh.before, want};
+}
+
+template <class T>
+__global__ __launch_bounds__(NT, 8) void k_sample_gather(SampleRows R, Split P, int S) {
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, lane = tid & 63;
+    SplitRow &W = P.rows[blockIdx.y];
+    Filters f;
+    f.read(R, blockIdx.y);
+    float hi, lo;
+    int id_hi;
+    join_slices(W, P, hi, lo, id_hi);
+    if (hi == -INFINITY || f.greedy()) return;
+    f.range(hi, lo, S);
+    if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
+    const Plan p = plan(sh, W, f);
+    if (p.mode == Plan::SLOW) return;
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    const Row<T, false> row = slice_of<T>(R, P);
+    const float low = f.bins.floor(p.bin);
+    const bool sums = p.mode != Plan::LIST;
+    u64 sum = 0;
+    int at = -1;
+    row.each(
+        [&](int id, const float(&l)[STEP]) {
+            if (!__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= low)) return;
+#pragma unroll
+            for (int e = 0; e < STEP; e++) {
+                const int b = l[e] > -INFINITY ? f.bins.of(l[e]) : BINS;
+                const bool take = sums ? b == p.bin && b < BINS : b <= p.bin;
+                const u64 m = __ballot(take);
+                if (m) {
+                    int to = 0;
+                    if (lane == 0) to = atomicAdd(&sh.n, (int)__popcll(m));
+                    to = __builtin_amdgcn_readfirstlane(to);
+                    to += __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+                    if (take && to < NT) sh.list[to] = place(l[e], id + e);
+                }
+                if (sums && b < p.bin) {
+                    const double w = f.W.value(sh, l[e]);
+                    sum += w >= f.least ? Weight::whole(w) : 0;
+                }
+            }
+        },
+        [&](int run) {
+            if (sums && at >= 0) {
+                sum = wave_sum64(sum);
+                if (lane == 0 && at < RUNS) W.runs[at] = sum;
+            }
+            sum = 0;
+            at = run;
+        });
+    __syncthreads();
+    const int n = sh.n;
+    if (!n) return;
+    if (tid == 0) sh.bin = atomicAdd(&W.n, n);
+    __syncthreads();
+    const int to = sh.bin + tid;
+    if (tid < min(n, NT) && to < NT) W.list[to] = sh.list[tid];
+}
+
+// ---- a block per row ------------------------------------------------------
+
+// SPLIT: after the kernels above.
+template <class T, bool LDS, bool SPLIT>
+__global__ __launch_bounds__(NT, LDS ? 8 : 4) void k_sample(SampleRows R, Split P, int S) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    Shared &sh = *reinterpret_cast<Shared *>(lds);
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Row<T, LDS> row;
+    bind_row(row, R, r, reinterpret_cast<T *>(lds + sizeof(Shared)));
+    Filters f;
+    f.read(R, r);
+    const float u = R.u[r];
+    float hi, lo, hi_t = 0.0f;  // the row's; this thread's
+    int id_hi;
+    if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
+    if constexpr (SPLIT) {
+        join_slices(P.rows[r], P, hi, lo, id_hi);
+        __syncthreads();
+    } else {
+        extremes<false>(row, hi, lo, id_hi);
+        hi_t = hi;
+        hi = wave_max(hi);
+        lo = -wave_max(-lo);
+        if (lane == 0) {
+            sh.red[wave] = hi;
+            sh.red[NW + wave] = lo;
+        }
+        if (tid == 0) sh.at = ~0ull;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            hi = fmaxf(hi, sh.red[w]);
+            lo = fminf(lo, sh.red[NW + w]);
+        }
     }
     auto put = [&](int id, float prob) {
         R.ids[r] = id;
@@ -506,44 +774,73 @@ __global__ __launch_bounds__(NT, LDS ? 8 : 4) void k_sample(SampleRows R, int S)
         if (tid == 0) put(-1, 0.0f);
         return;
     }
-    if (!(temp > 0.0f) || min_p > 1.0f || top_p <= 0.0f || top_k == 1) {  // the most likely token
-        u64 at = ~0ull;
-        row.each([&](int id, const float(&l)[STEP]) {
+    if (f.greedy()) {
+        if constexpr (SPLIT) {
+            if (tid == 0) put(id_hi, 1.0f);
+        } else {
+            u64 at = ~0ull;
+            row.each([&](int id, const float(&l)[STEP]) {
 #pragma unroll
-            for (int e = STEP - 1; e >= 0; e--) at = l[e] == hi && (u64)id < at ? (u64)(id + e) : at;
-        });
-        if (at != ~0ull) atomicMin(&sh.at, at);
-        __syncthreads();
-        if (tid == 0) put((int)sh.at, 1.0f);
+                for (int e = STEP - 1; e >= 0; e--) at = l[e] == hi && (u64)id < at ? (u64)(id + e) : at;
+            });
+            if (at != ~0ull) atomicMin(&sh.at, at);
+            __syncthreads();
+            if (tid == 0) put((int)sh.at, 1.0f);
+        }
         return;
     }
-    Weight W;
-    W.max = hi;
-    W.c = 1.4426950408889634 / (double)temp;
-    W.S = S;
-    W.low = -(double)(S + 2);
-    // Bins over the logits that have weight, or all of them if those span less.
-    const double span = (double)(S + 3) / W.c, range = (double)hi - (double)lo;
-    const bool limited = !(range < span);
-    const Bins bins{hi, (float)fmin(fmax((double)BINS / (limited ? span : range), 0x1p-118), 0x1p100)};
-    const double least = min_p > 0.0f ? __builtin_ldexp((double)min_p, S) : 0.0;
+    f.range(hi, lo, S);
+    const Weight &W = f.W;
+    const Bins &bins = f.bins;
+    const double least = f.least;
+    const float top_p = f.top_p;
+    const int top_k = f.top_k;
+    const bool by_weight = f.by_weight, limited = f.limited;
 
     Kept K{{-INFINITY, -1}, -1, 0.0};  // everything finite
-    const bool by_count = top_k > 0 && top_k < row.n, by_weight = top_p < 1.0f;
-    if (by_count && top_k <= NT) {
-        // At least top_k logits are as large as the top_k-th largest of the threads'
-        // own maxima, and not many more where the ids' order is no order of l.
-        const int bin = nth_bin(sh, bins.of(hi_t), hi_t > -INFINITY, top_k);
-        if (bin >= 0 && !(limited && bin == BINS - 1)) {
-            const int n = collect(sh, row, bins, K.keep, bin, true);
-            if (n <= NT) K.n = n;
+    int most = NT;         // a list of more than top_k elements so far: top_k
+    bool summed = false;   // the runs' sums are known but for the places in sh.list
+    bool by_count = f.by_count, left = by_count || by_weight;  // left: filters that are still to be applied
+    u64 last = ~0ull;      // thread tid's place of that list
+    if constexpr (SPLIT) {
+        const SplitRow &X = P.rows[r];
+        const Plan p = plan(sh, X, f);
+        if (p.mode == Plan::EVERY) {
+            left = false;
+            summed = true;
+        } else if (p.mode != Plan::SLOW && X.n <= NT) {
+            __syncthreads();
+            const u64 v = tid < X.n ? X.list[tid] : ~0ull;
+            left = false;
+            if (p.mode == Plan::LIST) {
+                sh.list[tid] = v;
+                K.n = X.n;
+                most = top_k;
+                __syncthreads();
+            } else {
+                last = block_sort(sh, v, X.n);
+                K.keep = by_weight ? end_of<true>(sh, W, last, X.n, p.before, p.want)
+                                   : end_of<false>(sh, W, last, X.n, p.before, p.want);
+                summed = true;
+            }
         }
     }
-    if (by_count && K.n < 0) cut<false, true>(sh, row, bins, W, K, (u64)top_k, 0.0, limited);
-    const int most = K.n >= 0 ? top_k : NT;  // a list of more than top_k elements so far
-    if (by_weight && K.n < 0) {
-        if (by_count) cut<true, false>(sh, row, bins, W, K, 0, (double)top_p, limited);
-        else cut<true, true>(sh, row, bins, W, K, 0, (double)top_p, limited);
+    if (left) {
+        if (!SPLIT && by_count && top_k <= NT) {
+            // At least top_k logits are as large as the top_k-th largest of the threads'
+            // own maxima, and not many more where the ids' order is no order of l.
+            const int bin = nth_bin(sh, bins.of(hi_t), hi_t > -INFINITY, top_k);
+            if (bin >= 0 && !(limited && bin == BINS - 1)) {
+                const int n = collect(sh, row, bins, K.keep, bin, true);
+                if (n <= NT) K.n = n;
+            }
+        }
+        if (by_count && K.n < 0) cut<false, true>(sh, row, bins, W, K, (u64)top_k, 0.0, limited);
+        if (K.n >= 0) most = top_k;
+        if (by_weight && K.n < 0) {
+            if (by_count) cut<true, false>(sh, row, bins, W, K, 0, (double)top_p, limited);
+            else cut<true, true>(sh, row, bins, W, K, 0, (double)top_p, limited);
+        }
     }
 
     if (K.n >= 0 && K.n <= 64) {  // a list of one wave: ranks and sums by comparing all pairs
@@ -617,25 +914,35 @@ __global__ __launch_bounds__(NT, LDS ? 8 : 4) void k_sample(SampleRows R, int S)
         return (keep.has(l, id) & int(w >= least)) ? Weight::whole(w) : 0;
     };
     __syncthreads();
-    sh.sums[tid] = 0;
-    __syncthreads();
-    u64 sum = 0;
-    int at = -1;
-    row.each(
-        [&](int id, const float(&l)[STEP]) {
-            if (!__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= keep.l)) return;
+    if (SPLIT && summed) {
+        sh.sums[tid] = tid < P.slices * P.runs ? P.rows[r].runs[tid] : 0;
+        __syncthreads();
+        if (last != ~0ull) {
+            const int id = (int)(uint32_t)last;
+            const u64 w = kept(id, logit_of(last));
+            if (w) atomicAdd(&sh.sums[id / (row.q * 64 * STEP)], w);
+        }
+    } else {
+        sh.sums[tid] = 0;
+        __syncthreads();
+        u64 sum = 0;
+        int at = -1;
+        row.each(
+            [&](int id, const float(&l)[STEP]) {
+                if (!__ballot(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= keep.l)) return;
 #pragma unroll
-            for (int e = 0; e < STEP; e++)
-                if (__ballot(keep.has(l[e], id + e))) sum += kept(id + e, l[e]);
-        },
-        [&](int run) {
-            if (__ballot(sum != 0)) {
-                sum = wave_sum64(sum);
-                if (lane == 0) sh.sums[at] = sum;
-            }
-            sum = 0;
-            at = run;
-        });
+                for (int e = 0; e < STEP; e++)
+                    if (__ballot(keep.has(l[e], id + e))) sum += kept(id + e, l[e]);
+            },
+            [&](int run) {
+                if (__ballot(sum != 0)) {
+                    sum = wave_sum64(sum);
+                    if (lane == 0) sh.sums[at] = sum;
+                }
+                sum = 0;
+                at = run;
+            });
+    }
     __syncthreads();
     static_assert(RUNS == NT, "a thread per run");
     const u64 mine = sh.sums[tid];
@@ -680,13 +987,15 @@ size_t row_lds(size_t vocab) {
 }  // namespace
 
 hipError_t sample_prepare_lds() {
-    for (const void *fn : {(const void *)k_sample<float, true>, (const void *)k_sample<_Float16, true>,
-                           (const void *)k_sample<bf16_bits, true>}) {
+    for (const void *fn : {(const void *)k_sample<float, true, false>, (const void *)k_sample<_Float16, true, false>,
+                           (const void *)k_sample<bf16_bits, true, false>}) {
         const hipError_t e = ensure_lds_limit(fn, ROW_BYTES + (int)sizeof(Shared));
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
+
+size_t sample_split_bytes() { return SPLIT_ROWS * sizeof(SplitRow); }
 
 hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
     if (!r.n_rows) return hipSuccess;
@@ -695,10 +1004,24 @@ hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
     const int S = 62 - lg < 50 ? 62 - lg : 50;
     auto go = [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const size_t row = row_lds<T>(r.vocab);
-        if (row <= ROW_BYTES)
-            hipLaunchKernelGGL((k_sample<T, true>), dim3((unsigned)r.n_rows), dim3(NT), sizeof(Shared) + row, s, r, S);
-        else hipLaunchKernelGGL((k_sample<T, false>), dim3((unsigned)r.n_rows), dim3(NT), sizeof(Shared), s, r, S);
+        const size_t lds = row_lds<T>(r.vocab);
+        const dim3 rows((unsigned)r.n_rows);
+        Split p{static_cast<SplitRow *>(r.split), 0, 0};
+        if (lds <= ROW_BYTES) {
+            hipLaunchKernelGGL((k_sample<T, true, false>), rows, dim3(NT), sizeof(Shared) + lds, s, r, p, S);
+        } else if (r.n_rows > SPLIT_ROWS) {
+            hipLaunchKernelGGL((k_sample<T, false, false>), rows, dim3(NT), sizeof(Shared), s, r, p, S);
+        } else {
+            const int runs = (int)((r.vocab + (size_t)row_q(r.vocab) * 64 * STEP - 1) / ((size_t)row_q(r.vocab) * 64 * STEP));
+            const int want = std::min(MAX_SLICES, std::max(1, SPLIT_BLOCKS / (int)r.n_rows));
+            p.runs = ((runs + want - 1) / want + NW - 1) / NW * NW;
+            p.slices = (runs + p.runs - 1) / p.runs;
+            const dim3 grid((unsigned)p.slices, (unsigned)r.n_rows);
+            hipLaunchKernelGGL((k_sample_extremes<T>), grid, dim3(NT), 0, s, r, p);
+            hipLaunchKernelGGL((k_sample_bins<T>), grid, dim3(NT), 0, s, r, p, S);
+            hipLaunchKernelGGL((k_sample_gather<T>), grid, dim3(NT), 0, s, r, p, S);
+            hipLaunchKernelGGL((k_sample<T, false, true>), rows, dim3(NT), sizeof(Shared), s, r, p, S);
+        }
     };
     if (r.dtype == T_F32) go((float *)nullptr);
     else if (r.dtype == T_F16) go((_Float16 *)nullptr);

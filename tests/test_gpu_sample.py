@@ -93,6 +93,40 @@ def test_types_rows_of_own_settings_and_strides(ctx, dtype, v, n):
     Call(ctx, x, dtype, u, **par).check()
 
 
+@pytest.mark.parametrize("n", [1, 3, 40, 257])
+def test_long_rows(ctx, n):
+    """Rows that several blocks share (a block each where they are many): nothing cut, cut
+    within a few elements, within many, both filters with many left, as flat and as peaked
+    rows have it."""
+    print(f"sample long rows n={n}", flush=True)
+    v = 40009 if n > 40 else 133337
+    x, u = rows(n, n, v)
+    x[::3] *= F32(0.15)
+    rng = np.random.default_rng(n)
+    for par in ({}, {"top_p": 0.9}, {"top_k": 3000}, {"top_k": 40}, {"top_k": 20000, "top_p": 0.8}, {"min_p": 0.3, "top_p": 0.95},
+                {"top_k": v - 1, "temperature": 0.05}, {"temperature": 0.0}, {"top_p": 1e-6}):
+        Call(ctx, x, G.F32, u, **par).check()
+        if n > 3:
+            break
+    par = {"temperature": rng.choice([0.0, 0.2, 1.0, 1.7], n), "top_k": rng.choice([0, 1, 20, 1500, v], n),
+           "top_p": rng.choice([0.1, 0.5, 0.95, 1.0], n), "min_p": rng.choice([0.0, 0.01, 0.2], n)}
+    Call(ctx, x, G.F32, u, **par).check()
+
+
+@pytest.mark.parametrize("par", [{}, {"top_k": 2000}, {"top_p": 0.37}, {"top_p": 0.6, "top_k": 50000}, {"min_p": 1.0}], ids=str)
+def test_long_rows_of_equal_and_missing_logits(ctx, par):
+    x, u = rows(11, 6, 70001)
+    x[0] = 1.5
+    x[1] = -np.inf
+    x[2, :] = np.nan
+    x[2, 70000] = -3
+    x[3, ::7] = x[3].max()
+    x[4, 60000:] = -np.inf
+    x[4, 13] = np.inf
+    x[5, 5:69000] = -3.4e38
+    Call(ctx, x, G.F32, u, **par).check()
+
+
 def test_ties(ctx):
     """Equal logits: the lower ids are kept, sums of equal weights are exact."""
     x = np.zeros((8, 1000), F32)
