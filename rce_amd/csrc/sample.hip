@@ -21,7 +21,10 @@
 //
 // What bounds it: one CU per row, so the instructions of the row's passes over
 // LDS (rows above 128 KB: over L2): the first one, the histogram and the collection
-// where a list follows, and two more where none does.
+// where a list follows, and two more where none does.  A top_k up to NT takes its
+// first cut from the threads' own maxima instead of a histogram of all logits.
+// 1 x 32000 f32 with top-k 40: 11 us; 500 x 32003 bf16, settings mixed: 65 us (two
+// blocks per CU).  Few rows above 128 KB are spread over several CUs, see below.
 #include "kv_cache.h"
 #include "lds_limit.h"
 
@@ -470,6 +473,7 @@ struct Filters {
         by_count = top_k > 0 && (size_t)top_k < R.vocab;
         by_weight = top_p < 1.0f;
     }
+    __device__ __forceinline__ bool few() const { return by_count && top_k <= NT; }
     // the most likely token
     __device__ __forceinline__ bool greedy() const { return !(temp > 0.0f) || min_p > 1.0f || top_p <= 0.0f || top_k == 1; }
     __device__ __forceinline__ void range(float hi, float lo, int S) {
@@ -537,8 +541,19 @@ __device__ __forceinline__ void bind_row(Row<T, LDS> &row, const SampleRows &R, 
 // logits; their histograms, added up in device memory; the elements of the bin
 // where the kept ones end (of all bins up to it, if they are few) and
 // the runs' sums of what is kept for certain.  k_sample goes on from there with a
-// block per row.  Rows with both filters and more than NT elements up to the end of
-// top-k, and a bin of more than NT, are left to its own passes.
+// block per row.  Rows with top-p and a top_k above NT, and lists of
+// more than NT elements, are left to its own passes.
+//
+// 64 x 128000 f32 with top-p: 8 + 17 + 22 + 15 us, the middle two bound by the f64
+// exponentials (14 f64 instructions per logit); a block per row took 138.  Whole calls, a
+// block per row against this (us):
+//                      top-p 0.9  none       top-k 40, top-p  top-k 5000, top-p
+//   64 x 128000 f32     133   62   61   33    27   35          174  180
+//   128                 140   87   64   52    32   43          180  187
+//   200                 147  130   71   82    38   53          186  195
+//   1 x 30000 (in LDS)   34   25   17   15    12   20           49   61
+// The filters' values are not known on the host: rows that fit LDS and more than 128
+// of them stay with a block per row.
 constexpr int MAX_SLICES = 64;
 struct SplitRow {
     u64 hist[BINS], list[NT], runs[RUNS];
@@ -548,10 +563,12 @@ struct SplitRow {
     } slice[MAX_SLICES];
     int n;
 };
-constexpr int SPLIT_ROWS = 256, SPLIT_BLOCKS = 512;  // rows of a split call; blocks to make of them (two per CU)
+constexpr int SPLIT_ROWS = 128, SPLIT_BLOCKS = 512;  // rows of a split call; blocks to make of them (two per CU)
 struct Split {
     SplitRow *rows;
+    float *tops;       // [rows][slices][NT]: the largest logits of the slices' threads
     int slices, runs;  // runs of a slice: a multiple of NW
+    __device__ float &top() const { return tops[((size_t)blockIdx.y * slices + blockIdx.x) * NT + threadIdx.x]; }
 };
 
 template <class T>
@@ -585,6 +602,7 @@ __global__ __launch_bounds__(NT, 8) void k_sample_extremes(SampleRows R, Split P
     int id;
     extremes<true>(slice_of<T>(R, P), hi, lo, id);
     const float own = hi;
+    P.top() = own;
     hi = wave_max(hi);
     lo = -wave_max(-lo);
     if (lane == 0) {
@@ -607,6 +625,8 @@ __global__ __launch_bounds__(NT, 8) void k_sample_extremes(SampleRows R, Split P
     }
 }
 
+__device__ __forceinline__ bool split_slow(const Filters &f) { return f.by_count && f.by_weight && f.top_k > NT; }
+
 template <class T>
 __global__ __launch_bounds__(NT, 8) void k_sample_bins(SampleRows R, Split P, int S) {
     __shared__ Shared sh;
@@ -617,13 +637,16 @@ __global__ __launch_bounds__(NT, 8) void k_sample_bins(SampleRows R, Split P, in
     float hi, lo;
     int id_hi;
     join_slices(W, P, hi, lo, id_hi);
-    if (hi == -INFINITY || f.greedy() || !(f.by_count || f.by_weight)) return;
+    if (hi == -INFINITY || f.greedy() || !(f.by_count || f.by_weight) || split_slow(f)) return;
     f.range(hi, lo, S);
     if (tid < 128) sh.exp2_[tid] = exp2((double)tid / 128);
 #pragma unroll
     for (int i = 0; i < PER; i++) sh.hist[i * NT + tid] = 0;
     __syncthreads();
-    slice_of<T>(R, P).each([&](int, const float(&l)[STEP]) {
+    if (f.few()) {
+        const float l = P.top();
+        if (l > -INFINITY) atomicAdd(&sh.hist[f.bins.of(l)], 1ull);
+    } else slice_of<T>(R, P).each([&](int, const float(&l)[STEP]) {
 #pragma unroll
         for (int e = 0; e < STEP; e++)
             if (l[e] > -INFINITY) atomicAdd(&sh.hist[f.bins.of(l[e])], f.by_count ? 1ull : f.W(sh, l[e]));
@@ -636,7 +659,10 @@ __global__ __launch_bounds__(NT, 8) void k_sample_bins(SampleRows R, Split P, in
     }
 }
 
-// How a split row goes on, from its histogram (of counts, without top-k of weights); the same in every block.
+// How a split row goes on, from its histogram; the same in every block.  It holds
+// the weights, or with top-k the counts; for a small top_k those of the threads'
+// largest logits alone: at least top_k logits are as large as the top_k-th of these, and
+// not many more where the ids' order is no order of l.
 struct Plan {
     enum { EVERY, LIST, BIN, SLOW } mode;  // no cut; the list of the bins 0 .. bin, or of `bin` alone; k_sample's own passes
     int bin;
@@ -645,6 +671,7 @@ struct Plan {
 };
 __device__ __forceinline__ Plan plan(Shared &sh, const SplitRow &W, const Filters &f) {
     if (!(f.by_count || f.by_weight)) return {Plan::EVERY, BINS, 0, 0.0};
+    if (split_slow(f)) return {Plan::SLOW, BINS, 0, 0.0};
     const int tid = threadIdx.x;
     u64 h[PER], mine = 0, total;
 #pragma unroll
@@ -663,8 +690,7 @@ __device__ __forceinline__ Plan plan(Shared &sh, const SplitRow &W, const Filter
     }
     __syncthreads();
     const bool cut = sh.bin >= 0 && !(f.limited && sh.bin == BINS - 1);
-    if (f.by_count && cut && sh.at <= (u64)NT) return {Plan::LIST, sh.bin, 0, 0.0};
-    if (f.by_count && f.by_weight) return {Plan::SLOW, BINS, 0, 0.0};
+    if (f.few()) return {cut ? Plan::LIST : Plan::SLOW, cut ? sh.bin : BINS, 0, 0.0};
     if (!cut) return {Plan::EVERY, BINS, 0, 0.0};
     return {Plan::BIN, sh.bin, sh.before, want};
 }
@@ -995,7 +1021,7 @@ hipError_t sample_prepare_lds() {
     return hipSuccess;
 }
 
-size_t sample_split_bytes() { return SPLIT_ROWS * sizeof(SplitRow); }
+size_t sample_split_bytes() { return SPLIT_ROWS * sizeof(SplitRow) + (size_t)SPLIT_BLOCKS * NT * sizeof(float); }
 
 hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
     if (!r.n_rows) return hipSuccess;
@@ -1006,7 +1032,7 @@ hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
         using T = std::remove_pointer_t<decltype(t)>;
         const size_t lds = row_lds<T>(r.vocab);
         const dim3 rows((unsigned)r.n_rows);
-        Split p{static_cast<SplitRow *>(r.split), 0, 0};
+        Split p{static_cast<SplitRow *>(r.split), nullptr, 0, 0};
         if (lds <= ROW_BYTES) {
             hipLaunchKernelGGL((k_sample<T, true, false>), rows, dim3(NT), sizeof(Shared) + lds, s, r, p, S);
         } else if (r.n_rows > SPLIT_ROWS) {
@@ -1016,6 +1042,7 @@ hipError_t launch_sample(const SampleRows &r, hipStream_t s) {
             const int want = std::min(MAX_SLICES, std::max(1, SPLIT_BLOCKS / (int)r.n_rows));
             p.runs = ((runs + want - 1) / want + NW - 1) / NW * NW;
             p.slices = (runs + p.runs - 1) / p.runs;
+            p.tops = reinterpret_cast<float *>(p.rows + SPLIT_ROWS);
             const dim3 grid((unsigned)p.slices, (unsigned)r.n_rows);
             hipLaunchKernelGGL((k_sample_extremes<T>), grid, dim3(NT), 0, s, r, p);
             hipLaunchKernelGGL((k_sample_bins<T>), grid, dim3(NT), 0, s, r, p, S);

@@ -93,7 +93,7 @@ def test_types_rows_of_own_settings_and_strides(ctx, dtype, v, n):
     Call(ctx, x, dtype, u, **par).check()
 
 
-@pytest.mark.parametrize("n", [1, 3, 40, 257])
+@pytest.mark.parametrize("n", [1, 3, 40, 129])
 def test_long_rows(ctx, n):
     """Rows that several blocks share (a block each where they are many): nothing cut, cut
     within a few elements, within many, both filters with many left, as flat and as peaked
