@@ -32,7 +32,6 @@
 
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <type_traits>
 
 #include "mfma_util.h"
@@ -45,10 +44,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int ROWS = 16;    // query rows of a unit
 constexpr int WAVES = 4;    // of a block
 constexpr int TILE = 64;    // positions of a wave's step
-static int envi(const char*n,int d){const char*e=getenv(n);return e?atoi(e):d;}
-#define TARGET envi("KT",512)
-#define P_TARGET envi("PT",512)
+constexpr int TARGET = 512;   // blocks that a part's tiles are spread over: two per CU
 constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
+constexpr int LINE_CHUNK = 24;  // tiles per block from which a block may serve several units
+constexpr int PAD = 4;          // a unit's prologue and epilogue, in the time of a tile
 constexpr int FEW = 32;       // query rows per kv head up to which a sequence is served in units of ROWS
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -77,17 +76,30 @@ __device__ __forceinline__ Span span_of(const Args &A, const KvSeq &q) {
     s.tiles = q.hi(A.B) > q.lo() ? (q.hi(A.B) + TILE - 1) / TILE - s.t0 : 0;
     return s;
 }
+// The cells of a unit in the line (below): its prologue's, then one per tile, one if it has none.
+__device__ __forceinline__ int line_cells(const Span &p) { return PAD + max(1, p.tiles); }
 
-// Tiles per range, the same in every block of the call.
-__device__ __forceinline__ int chunk_of(const Args &A) {
+// How a part is cut, the same in every block: tiles per range, or in a line cells per block.
+struct Cut {
+    int chunk;
+    bool line;
+};
+template <bool LINE>
+__device__ __forceinline__ Cut cut_of(const Args &A) {
     const int lane = threadIdx.x & 63;
-    float total = 0.0f;  // only a size: its rounding moves no result
+    float tiles = 0.0f, units = 0.0f;  // only sizes: their rounding moves no result
     for (int s = lane; s < A.B.n_seqs; s += 64) {
         const Span p = span_of(A, kv_seq(A.B, s));
-        total += (float)p.units * (float)p.tiles;
+        tiles += (float)p.units * (float)p.tiles;
+        if (LINE) units += (float)line_cells(p) * (float)p.units;
     }
-    total = wave_sum(total) * (float)A.P.heads;
-    return max(MIN_CHUNK, (int)fminf(ceilf(total / (float)A.target), 1e9f));
+    auto chunk = [&](float total) { return (int)fminf(ceilf(wave_sum(total) * (float)A.P.heads / (float)A.target), 1e9f); };
+    const int c = chunk(tiles);
+    if (LINE && c >= LINE_CHUNK) {
+        const int l = chunk(units);
+        if (l < 1 << 20) return {l, true};  // the line's length fits 31 bits
+    }
+    return {max(MIN_CHUNK, c), false};
 }
 
 __device__ __forceinline__ int ranges(int tiles, int chunk) { return tiles ? (tiles + chunk - 1) / chunk : 1; }
@@ -98,7 +110,10 @@ __device__ __forceinline__ int range_tiles(int tiles, int n) { return (tiles + n
 struct Work {
     KvSeq q;
     Span sp;
-    int seq, unit, range, n_ranges, step, slot;  // step: tiles of a range; slot of the unit's range 0, before the head
+    int seq, unit;
+    int t_lo, t_hi;  // tiles of the range, of the sequence
+    int slot;        // of the range, before the head
+    bool whole;      // the range is all of the unit's
 };
 
 // Range `item` of the list (sequence, unit, range).
@@ -122,16 +137,61 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
             w.seq = base + l;
             w.q = kv_seq(A.B, w.seq);
             w.sp = span_of(A, w.q);
-            w.n_ranges = ranges(w.sp.tiles, chunk);
-            w.step = range_tiles(w.sp.tiles, w.n_ranges);
-            const int u = at / w.n_ranges;
+            const int n = ranges(w.sp.tiles, chunk), step = range_tiles(w.sp.tiles, n);
+            const int u = at / n, range = at - u * n;
             w.unit = w.sp.units - 1 - u;  // the units with the most keys first
-            w.range = at - u * w.n_ranges;
-            w.slot = srun + __builtin_amdgcn_readlane(sincl - sc, l) + w.unit * w.n_ranges;
+            w.t_lo = w.sp.t0 + range * step;
+            w.t_hi = w.t_lo + step;
+            w.slot = srun + __builtin_amdgcn_readlane(sincl - sc, l) + w.unit * n + range;
+            w.whole = n == 1;
             return true;
         }
         run += total;
         srun += __builtin_amdgcn_readlane(sincl, 63);
+    }
+    return false;
+}
+
+// ---- the units as one line ------------------------------------------------
+//
+// Ranges of whole units leave lengths from chunk / 2 to chunk: the CUs that have got
+// the short ones wait.  Where a block has LINE_CHUNK tiles or more to do, all units stand in one
+// line, PAD cells for the prologue and one per tile each, and block i takes the cells i * chunk ..
+// (i + 1) * chunk - 1, of two or more units often.  What it leaves of a unit that it shares goes to
+// slot 2 i + 1 if it has the unit's first tile, else 2 i (its first unit).
+// 64 sequences of up to 4096: 100 -> 85 us.
+
+// The work at cell `pos` of the line, up to cell `end`; false: none is left.  n: the cells up to the next unit.
+__device__ __forceinline__ bool find_in_line(const Args &A, int item, int pos, int end, Work &w, int &n) {
+    const int lane = threadIdx.x & 63;
+    int run = 0;
+    for (int base = 0; base < A.B.n_seqs; base += 64) {
+        const int s = base + lane;
+        int c = 0;
+        if (s < A.B.n_seqs) {
+            const Span p = span_of(A, kv_seq(A.B, s));
+            c = p.units * line_cells(p);
+        }
+        const int incl = wave_scan(c), total = __builtin_amdgcn_readlane(incl, 63);
+        if (pos < run + total) {
+            const int l = __builtin_ctzll(__ballot(pos < run + incl));
+            const int at = pos - run - __builtin_amdgcn_readlane(incl - c, l);
+            w.seq = base + l;
+            w.q = kv_seq(A.B, w.seq);
+            w.sp = span_of(A, w.q);
+            const int cells = line_cells(w.sp);
+            w.unit = at / cells;
+            const int from = at - w.unit * cells, to = min(cells, from + end - pos);
+            n = to - from;
+            if (to <= PAD) return false;  // the unit's tiles are the next block's
+            const int t = max(from, PAD) - PAD;
+            w.t_lo = w.sp.t0 + t;
+            w.t_hi = w.sp.t0 + min(w.sp.tiles, to - PAD);
+            w.slot = 2 * item + (t == 0);
+            w.whole = t == 0 && to == cells;
+            return true;
+        }
+        run += total;
     }
     return false;
 }
@@ -215,18 +275,26 @@ struct Shared {
     float m[WAVES][ROWS], l[WAVES][ROWS];
 };
 
-template <int D, bool HILO>
-__global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
+template <int D, bool HILO, bool LINE>
+__global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 192 ? 2 : 1) void k_kv_attention(Args A) {
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
     constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
     __shared__ Shared<D> sh;
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    int block = blockIdx.x;
+    const Cut cut = cut_of<LINE>(A);
+    int line_at = cut.line ? block / A.P.heads * cut.chunk : 0;
+    const int line_end = line_at + cut.chunk;
+  for (;;) {
+    // opaque: what follows from them is not kept in registers from one unit to the next
+    int tid = threadIdx.x;
+    if constexpr (LINE) asm volatile("" : "+v"(tid), "+s"(block));
+    const int lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % A.P.heads;
-    const int chunk = chunk_of(A);
+    const int item = block / A.P.heads, h = block % A.P.heads;
     Work w;
-    if (!find_work(A, blockIdx.x / A.P.heads, chunk, w)) return;
+    int n_cells = 0;
+    if (LINE && cut.line ? !find_in_line(A, item, line_at, line_end, w, n_cells) : !find_work(A, item, cut.chunk, w)) return;
     const KvSeq &q = w.q;
     const int G = A.G, first = q.first();
     const int x0 = w.unit * ROWS, n_x = min(ROWS, (q.r1 - q.r0) * G - x0);  // rows of the unit
@@ -295,8 +363,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
     const int u_hi = min(A.B.cap - 1, first + u_tok1), u_first = first + u_tok0;
     const int all_lo = max(0, max(0, u_hi) - (A.a.window - 1)), all_hi = u_first;  // seen by every row (if all have positions)
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-    t_lo = max(t_lo, w.sp.t0 + w.range * w.step);
-    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * w.step);
+    t_lo = max(t_lo, w.t_lo);
+    t_hi = min(t_hi, w.t_hi);
     const bool placed = u_first >= 0 && first + u_tok1 < A.B.cap;  // every row has a position
     const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1;
@@ -413,8 +481,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
         sh.m[wave][n] = m;
         sh.l[wave][n] = l;
     }
-    const bool whole = w.n_ranges == 1;
-    float *part = A.a.parts + ((size_t)(w.slot + w.range) * A.P.heads + h) * (ROWS * (D + 2));
+    const bool whole = w.whole;
+    float *part = A.a.parts + ((size_t)w.slot * A.P.heads + h) * (ROWS * (D + 2));
     constexpr int PART = Shared<D>::PART;
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += PART) {
@@ -449,6 +517,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(Args A) {
             }
         }
     }
+    line_at += n_cells;
+    if (!LINE || !cut.line || line_at >= line_end) return;
+    __syncthreads();  // sh.o is read; sh.q may be written
+  }
 }
 
 // ---- many query rows ------------------------------------------------------
@@ -559,9 +631,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.P.heads;
-    const int chunk = chunk_of(A);
     Work w;
-    if (!find_work(A, blockIdx.x / A.P.heads, chunk, w)) return;
+    if (!find_work(A, blockIdx.x / A.P.heads, cut_of<false>(A).chunk, w)) return;
     const KvSeq &q = w.q;
     const int G = A.G, first = q.first();
     const int x0 = w.unit * P_ROWS, n_x = min(P_ROWS, (q.r1 - q.r0) * G - x0);
@@ -650,8 +721,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     // the block's tiles
     const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-    t_lo = max(t_lo, w.sp.t0 + w.range * w.step);
-    t_hi = min(t_hi, w.sp.t0 + (w.range + 1) * w.step);
+    t_lo = max(t_lo, w.t_lo);
+    t_hi = min(t_hi, w.t_hi);
     const int32_t *__restrict__ pages = page_table + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
 
@@ -858,12 +929,12 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     l = swap_sum(l);
     if (xr >= n_x) return;
     const float unit = ref * (1.0f / UP);
-    if (w.n_ranges == 1) {
+    if (w.whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l * unit;
         const size_t at = (size_t)(q.r0 + tok) * A.a.out_stride + (size_t)(h * G + (x0 + xr) % G) * D + 4 * g;
         store_row<NT>(A.a.out, A.a.out_dtype, at, A.vec & 4, acc, inv, l == 0.0f);
     } else {
-        float *part = A.a.parts + ((size_t)(w.slot + w.range) * A.P.heads + h) * (P_ROWS * (D + 2));
+        float *part = A.a.parts + ((size_t)w.slot * A.P.heads + h) * (P_ROWS * (D + 2));
         store_row<NT>(part, T_F32, (size_t)xr * D + 4 * g, (D + 2) * P_ROWS % 4 == 0, acc, unit, false);
         if (g == 0) {
             part[P_ROWS * D + xr] = m;
@@ -873,53 +944,87 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
 }
 
 // The split units' ranges, in range order: a wave per (unit, head, row), every
-// wave of the grid the next one.
+// wave of the grid the next one.  64 ranges at a time: their factors first, one per
+// lane, then their rows, whose loads depend on nothing.
 constexpr int JOIN_BLOCKS = 512;
-template <int D>
+template <int D, bool LINE>
 __global__ __launch_bounds__(256) void k_kv_join(Args A) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int chunk = chunk_of(A);
+    const Cut cut = cut_of<LINE>(A);
+    const int chunk = cut.chunk;
+    const bool line = LINE && cut.line;
     const int rows = A.rows;
     for (int task = blockIdx.x * 4 + wave;; task += gridDim.x * 4) {
         const int h = task % A.P.heads;
         int seq, x;  // query row x of the sequence
         if (!kv_find(A.B, task / A.P.heads, [&](const KvSeq &q) {
                 const Span p = span_of(A, q);
-                return p.units && ranges(p.tiles, chunk) > 1 ? (q.r1 - q.r0) * A.G : 0;
+                return p.units && (line || ranges(p.tiles, chunk) > 1) ? (q.r1 - q.r0) * A.G : 0;
             }, seq, x))
             return;
-        // the ranges before this unit's
-        int slot = 0;
+        // what stands in front of the sequence: cells of the line, or split ranges
+        int before = 0;
         for (int s = lane; s < seq; s += 64) {
             const Span p = span_of(A, kv_seq(A.B, s));
             const int n = ranges(p.tiles, chunk);
-            slot += n > 1 ? p.units * n : 0;
+            before += line ? p.units * line_cells(p) : n > 1 ? p.units * n : 0;
         }
-        slot = __builtin_amdgcn_readlane(wave_scan(slot), 63);
+        before = __builtin_amdgcn_readlane(wave_scan(before), 63);
         const KvSeq q = kv_seq(A.B, seq);
-        const int nr = ranges(span_of(A, q).tiles, chunk), r = x % rows;
-        slot += x / rows * nr;
-        const size_t step = (size_t)A.P.heads * (rows * (D + 2));
-        const float *part = A.a.parts + ((size_t)slot * A.P.heads + h) * (rows * (D + 2));
+        const Span sp = span_of(A, q);
+        const int r = x % rows;
+        int slot, nr;  // the first range's; their number
+        if (line) {
+            const int cells = line_cells(sp), t0 = before + x / rows * cells;
+            const int b0 = (t0 + PAD) / chunk, b1 = (t0 + cells - 1) / chunk;
+            if (b0 == b1) continue;
+            slot = 2 * b0 + 1;  // the next 2 (b0 + 1), every other slot from there
+            nr = b1 - b0 + 1;
+        } else {
+            nr = ranges(sp.tiles, chunk);
+            slot = before + x / rows * nr;
+        }
+        const size_t step = (size_t)A.P.heads * (rows * (D + 2)) * (line ? 2 : 1);
+        const size_t head = (size_t)h * (rows * (D + 2));
+        const float *part = A.a.parts + (size_t)(slot + 1) * A.P.heads * (rows * (D + 2)) + head;  // of range 1
+        const float *part0 = A.a.parts + (size_t)slot * A.P.heads * (rows * (D + 2)) + head;
+        auto at = [&](int k) { return k ? part + (size_t)(k - 1) * step : part0; };
         float top = -INFINITY;
-        for (int k = lane; k < nr; k += 64) top = fmaxf(top, part[k * step + rows * D + r]);
+        for (int k = lane; k < nr; k += 64) top = fmaxf(top, at(k)[rows * D + r]);
         top = wave_max(top);
         const float base = top == -INFINITY ? 0.0f : top;
         float o[D / 64], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 64; i++) o[i] = 0.0f;
-#pragma unroll 4
-        for (int k = 0; k < nr; k++) {
-            const float *p = part + k * step;
-            const float f = exp2_(p[rows * D + r] - base);
-            sum = __builtin_fmaf(f, p[rows * D + rows + r], sum);
+        for (int k0 = 0; k0 < nr; k0 += 64) {
+            const int n = min(64, nr - k0);
+            float f = 0.0f, l = 0.0f;
+            if (lane < n) {
+                const float *p = at(k0 + lane) + rows * D + r;
+                f = exp2_(p[0] - base);
+                l = f * p[rows];
+            }
+            sum += wave_sum(l);
+            for (int k = 0; k < n; k += 8) {
+                float v[8][D / 64];
 #pragma unroll
-            for (int i = 0; i < D / 64; i++) o[i] = __builtin_fmaf(f, p[r * D + lane + 64 * i], o[i]);
+                for (int e = 0; e < 8; e++) {
+                    const float *p = at(k0 + min(k + e, n - 1)) + r * D + lane;
+#pragma unroll
+                    for (int i = 0; i < D / 64; i++) v[e][i] = p[64 * i];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k + e));
+#pragma unroll
+                    for (int i = 0; i < D / 64; i++) o[i] = k + e < n ? __builtin_fmaf(fk, v[e][i], o[i]) : o[i];
+                }
+            }
         }
-        const size_t at = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D;
+        const size_t to = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D;
 #pragma unroll
         for (int i = 0; i < D / 64; i++)
-            store_any(A.a.out, A.a.out_dtype, at + lane + 64 * i, sum == 0.0f ? 0.0f : o[i] / sum);
+            store_any(A.a.out, A.a.out_dtype, to + lane + 64 * i, sum == 0.0f ? 0.0f : o[i] / sum);
     }
 }
 
@@ -927,8 +1032,9 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
 
 // A part's split units have at least two ranges, all but the last of `chunk` tiles, so that
 // there are at most twice `target` of them (heads included); a rounding of the total
-// adds less than one in 2^10 (n_seqs is at most 2^20).
-constexpr int slots(int target) { return 2 * target + target / 16; }
+// adds less than one in 2^10 (n_seqs is at most 2^20).  In a line the blocks have two slots each, and
+// there is at most one block more per head: heads are at most target / 20 there.
+constexpr int slots(int target) { return 2 * target + target / 8; }
 constexpr size_t PARTS = (size_t)34 << 20;
 size_t kv_attention_parts_bytes() { return PARTS; }
 
@@ -941,24 +1047,33 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         auto part = [&](bool many, int lo, int hi) {
             Args A{pool, rows, a, G, many ? P_ROWS : ROWS, lo, hi, 0, 0};
             const size_t fit = PARTS / ((size_t)A.rows * (D + 2) * sizeof(float));  // slots
-            A.target = std::min(many ? P_TARGET : TARGET, (int)(fit * 16 / 33));
-            if (many) {
-                const int size = a.q_dtype == T_F32 ? 4 : 2;
-                if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
-                if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
-                if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride * (a.out_dtype == T_F32 ? 4 : 2) % 16 == 0) A.vec |= 4;
-            }
+            A.target = std::min(TARGET, (int)(fit * 16 / 34));
             // units of the part at most
             size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
             if (hi != INT_MAX) u = std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
-            const bool split = rows.cap > MIN_CHUNK * TILE;
+            const bool split = rows.cap > MIN_CHUNK * TILE, f32 = a.out_dtype == T_F32;
             const dim3 grid((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
-            const bool f32 = a.out_dtype == T_F32;
-            if (many && f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
-            else if (many) hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
-            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, true>), grid, dim3(64 * WAVES), 0, s, A);
-            else hipLaunchKernelGGL((k_kv_attention<D, false>), grid, dim3(64 * WAVES), 0, s, A);
-            if (split) hipLaunchKernelGGL((k_kv_join<D>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
+            // can its tiles come to a line at all?
+            const bool line = !many && split && pool.heads * 20 <= A.target &&
+                              (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
+            auto few = [&](auto l) {
+                constexpr bool LINE = decltype(l)::value;
+                if (f32) hipLaunchKernelGGL((k_kv_attention<D, true, LINE>), grid, dim3(64 * WAVES), 0, s, A);
+                else hipLaunchKernelGGL((k_kv_attention<D, false, LINE>), grid, dim3(64 * WAVES), 0, s, A);
+                if (split) hipLaunchKernelGGL((k_kv_join<D, LINE>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
+            };
+            if (!many) {
+                if (line) few(std::true_type{});
+                else few(std::false_type{});
+                return;
+            }
+            const int size = a.q_dtype == T_F32 ? 4 : 2;
+            if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
+            if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
+            if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride * (f32 ? 4 : 2) % 16 == 0) A.vec |= 4;
+            if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
+            else hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
+            if (split) hipLaunchKernelGGL((k_kv_join<D, false>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
         };
         if (x > (size_t)FEW * rows.n_seqs) {
             part(true, FEW + 1, INT_MAX);

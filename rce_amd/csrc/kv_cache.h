@@ -83,15 +83,39 @@ __device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int s) {
     return q;
 }
 
-// Inclusive prefix sum over the wave's lanes.
+// v of the lane CTRL names (0 where there is none, or for rows outside ROWS).
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int dpp32(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ unsigned long long dpp64(unsigned long long v) {
+    const uint32_t lo = (uint32_t)dpp32<CTRL, ROWS>((int)(uint32_t)v), hi = (uint32_t)dpp32<CTRL, ROWS>((int)(uint32_t)(v >> 32));
+    return (unsigned long long)hi << 32 | lo;
+}
+// Inclusive prefix sum over the wave's lanes: within rows of 16 (shifts by 1, 2, 4, 8), then
+// lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(v, o);
-        if (lane >= o) v += y;
-    }
+    v += dpp32<0x111>(v);
+    v += dpp32<0x112>(v);
+    v += dpp32<0x114>(v);
+    v += dpp32<0x118>(v);
+    v += dpp32<0x142, 0xA>(v);
+    v += dpp32<0x143, 0xC>(v);
     return v;
+}
+__device__ __forceinline__ unsigned long long wave_scan64(unsigned long long v) {
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xA>(v);
+    v += dpp64<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ unsigned long long lane64(unsigned long long v, int l) {
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
 }
 
 // Item `item` of the list that has count(seq) consecutive items for every

@@ -80,28 +80,6 @@ __device__ __forceinline__ void narrow(float x, float &t) { t = x; }
 __device__ __forceinline__ void narrow(float x, _Float16 &t) { t = (_Float16)x; }
 __device__ __forceinline__ void narrow(float x, bf16_bits &t) { t.u = (uint16_t)(__float_as_uint(x) >> 16); }
 
-// v of the lane CTRL names (0 where there is none, or for rows outside ROWS).
-template <int CTRL, int ROWS = 0xF>
-__device__ __forceinline__ u64 dpp64(u64 v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
-    return (u64)hi << 32 | lo;
-}
-// Inclusive prefix sum over the lanes: within rows of 16 (shifts by 1, 2, 4, 8), then
-// lane 15 of rows 0 and 2 into rows 1 and 3, then lane 31 into rows 2 and 3.
-__device__ __forceinline__ u64 wave_scan64(u64 v) {
-    v += dpp64<0x111>(v);
-    v += dpp64<0x112>(v);
-    v += dpp64<0x114>(v);
-    v += dpp64<0x118>(v);
-    v += dpp64<0x142, 0xA>(v);
-    v += dpp64<0x143, 0xC>(v);
-    return v;
-}
-__device__ __forceinline__ u64 lane64(u64 v, int l) {
-    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
-}
 __device__ __forceinline__ u64 wave_sum64(u64 v) { return lane64(wave_scan64(v), 63); }
 
 // Exclusive prefix sum over the block's threads; total in every thread.
