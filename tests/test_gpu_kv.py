@@ -282,6 +282,21 @@ def test_attention_long_sequences_split(ctx, page, out_dtype):
     check_attention(ctx, 256, 1, 1, page, [1500], [1], G.F16, out_dtype, window=900)
 
 
+@pytest.mark.parametrize("out_dtype,window", [(G.F32, 0), (G.F16, 0), (G.F16, 30001)])
+def test_attention_long_ragged_sequences_in_line(ctx, out_dtype, window):
+    """Blocks that serve the end of one sequence and the beginning of the next."""
+    check_attention(ctx, 64, 8, 2, 64, [60000, 100, 40000, 0, 33333, 64, 31000], [1, 1, 2, 0, 1, 1, 9], G.F32, out_dtype,
+                    rope=64, window=window)
+
+
+def test_attention_in_line_of_many_units(ctx):
+    """More sequences than a wave has lanes, several of them in a block."""
+    rng = np.random.default_rng(8)
+    lens = [int(n) for n in rng.integers(0, 30000, 70)]
+    lens[5] = lens[66] = 0
+    check_attention(ctx, 64, 1, 1, 256, lens, [min(n, 1) for n in lens], G.F16, G.F16)
+
+
 def test_attention_many_sequences(ctx):
     """More sequences than a wave has lanes, empty ones among them."""
     rng = np.random.default_rng(11)
@@ -298,6 +313,52 @@ def test_attention_many_sequences(ctx):
 def test_attention_prompts(ctx, news, out_dtype):
     check_attention(ctx, 128, 2, 4, 64, news, news, out_dtype, out_dtype, rope=128)
     check_attention(ctx, 64, 1, 3, 16, [n + 100 for n in news], news, out_dtype, out_dtype, window=77)
+
+
+@pytest.mark.parametrize("d,rope", [(64, 34), (64, 64), (128, 6), (128, 64), (192, 192), (192, 0), (256, 128), (256, 256)])
+@pytest.mark.parametrize("q_dtype,out_dtype", [(G.F32, G.F32), (G.F16, G.F16), (G.BF16, G.BF16), (G.BF16, G.F32)])
+def test_attention_prompts_of_every_head_size(ctx, d, rope, q_dtype, out_dtype):
+    """Units of 128 query rows: one short of full, full, one more; single rows beside them."""
+    check_attention(ctx, d, 2, 3, 32, [43, 128, 170, 90], [43, 33, 1, 90], q_dtype, out_dtype, rope=rope)
+
+
+@pytest.mark.parametrize("page", [16, 64, 1024])
+@pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
+def test_attention_prompts_after_long_contexts(ctx, page, out_dtype):
+    """Split key ranges of 128-row units, beside single tokens whose ranges are split too."""
+    check_attention(ctx, 128, 1, 4, page, [3000, 700, 2500], [40, 1, 70], G.F16, out_dtype, rope=128)
+    check_attention(ctx, 64, 2, 2, page, [5000, 0, 900], [50, 0, 100], G.F32, out_dtype, window=2000)
+    check_attention(ctx, 256, 1, 1, page, [2000], [129], G.F16, out_dtype, rope=256)
+
+
+@pytest.mark.parametrize("window", [1, 15, 64, 65, 200])
+@pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
+def test_attention_prompts_with_windows(ctx, window, out_dtype):
+    check_attention(ctx, 64, 1, 5, 16, [300, 64, 130], [300, 64, 7], G.F32, out_dtype, rope=64, window=window)
+    check_attention(ctx, 192, 1, 2, 128, [150, 280], [70, 140], G.F16, out_dtype, window=window)
+
+
+@pytest.mark.parametrize("gap", [1, 2, 8])
+def test_attention_prompts_of_odd_strides_and_row_counts(ctx, gap):
+    for t in (G.F32, G.F16, G.BF16):
+        check_attention(ctx, 64, 2, 3, 16, [70, 9, 33], [70, 3, 33], t, t, gap=gap, rope=64, n_rows=120)
+
+
+@pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
+@pytest.mark.parametrize("d", [64, 256])
+def test_attention_prompts_of_growing_scores(ctx, out_dtype, d):
+    """Each block's scores pass the earlier ones' by much, or its values' scale does:
+    the running maximum and the running scale move at every tile; and the reverse."""
+    for name in ("k", "v"):
+        for flip in (False, True):
+            def edit(pool, b):
+                for s in range(len(b.lens)):
+                    n = max(1, (b.lens[s] + 15) // 16)
+                    for blk in range(n):
+                        f = 10.0 ** (4.0 * (n - 1 - blk if flip else blk) / n - 2)
+                        page = b.pages[s, blk * 16 // pool.page]
+                        getattr(pool, name + "_scale")[page, :, blk % pool.b] *= F32(f)
+            check_attention(ctx, d, 1, 2, 32, [400, 90], [200, 90], G.F32, out_dtype, edit=edit)
 
 
 def test_attention_rows_left_out(ctx):
