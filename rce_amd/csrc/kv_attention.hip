@@ -46,6 +46,7 @@ constexpr int WAVES = 4;    // of a block
 constexpr int TILE = 64;    // positions of a wave's step
 constexpr int TARGET = 512;   // blocks that a part's tiles are spread over: two per CU
 constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
+constexpr int P_MIN_CHUNK = 4;  // of units of P_ROWS rows
 constexpr int LINE_CHUNK = 24;  // tiles per block from which a block may serve several units
 constexpr int PAD = 4;          // a unit's prologue and epilogue, in the time of a tile
 constexpr int FEW = 32;       // query rows per kv head up to which a sequence is served in units of ROWS
@@ -60,6 +61,8 @@ struct Args {
     int rows;       // query rows of a unit
     int lo_x, hi_x; // the call's part: sequences of lo_x .. hi_x query rows per kv head
     int target;     // blocks that the part's tiles are spread over
+    int min_chunk;  // tiles of the shortest range
+    int line;       // 1: the units may be cut as one line
     int vec;        // query rows (1) and rotation table (2) can be read, output rows (4) written 16 bytes at a time
 };
 
@@ -95,11 +98,11 @@ __device__ __forceinline__ Cut cut_of(const Args &A) {
     }
     auto chunk = [&](float total) { return (int)fminf(ceilf(wave_sum(total) * (float)A.P.heads / (float)A.target), 1e9f); };
     const int c = chunk(tiles);
-    if (LINE && c >= LINE_CHUNK) {
+    if (LINE && A.line && c >= LINE_CHUNK) {
         const int l = chunk(units);
         if (l < 1 << 20) return {l, true};  // the line's length fits 31 bits
     }
-    return {max(MIN_CHUNK, c), false};
+    return {max(A.min_chunk, c), false};
 }
 
 __device__ __forceinline__ int ranges(int tiles, int chunk) { return tiles ? (tiles + chunk - 1) / chunk : 1; }
@@ -943,12 +946,15 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     }
 }
 
-// The split units' ranges, in range order: a wave per (unit, head, row), every
-// wave of the grid the next one.  64 ranges at a time: their factors first, one per
-// lane, then their rows, whose loads depend on nothing.
-constexpr int JOIN_BLOCKS = 512;
+// The split units' ranges, in range order: a wave takes 256 / D consecutive rows of a (unit,
+// head), four values per lane, every wave of the grid the next ones; U ranges
+// at a time, whose loads depend on nothing.
+constexpr int JOIN_BLOCKS = 1024;  // at most: four waves per SIMD
 template <int D, bool LINE>
-__global__ __launch_bounds__(256) void k_kv_join(Args A) {
+__global__ __launch_bounds__(256) void k_kv_join(Args A0, Args A1) {
+    constexpr int LPR = D / 4, RPW = 64 / LPR;  // lanes of a row, rows of a wave
+    constexpr int U = LINE ? 16 : 8;  // a line's units are the long ones
+    const Args &A = blockIdx.y ? A1 : A0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Cut cut = cut_of<LINE>(A);
     const int chunk = cut.chunk;
@@ -956,11 +962,11 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
     const int rows = A.rows;
     for (int task = blockIdx.x * 4 + wave;; task += gridDim.x * 4) {
         const int h = task % A.P.heads;
-        int seq, x;  // query row x of the sequence
+        int seq, group;
         if (!kv_find(A.B, task / A.P.heads, [&](const KvSeq &q) {
                 const Span p = span_of(A, q);
-                return p.units && (line || ranges(p.tiles, chunk) > 1) ? (q.r1 - q.r0) * A.G : 0;
-            }, seq, x))
+                return p.units && (line || ranges(p.tiles, chunk) > 1) ? ((q.r1 - q.r0) * A.G + RPW - 1) / RPW : 0;
+            }, seq, group))
             return;
         // what stands in front of the sequence: cells of the line, or split ranges
         int before = 0;
@@ -972,59 +978,58 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
         before = __builtin_amdgcn_readlane(wave_scan(before), 63);
         const KvSeq q = kv_seq(A.B, seq);
         const Span sp = span_of(A, q);
-        const int r = x % rows;
+        const int x0 = group * RPW, unit = x0 / rows;
         int slot, nr;  // the first range's; their number
         if (line) {
-            const int cells = line_cells(sp), t0 = before + x / rows * cells;
+            const int cells = line_cells(sp), t0 = before + unit * cells;
             const int b0 = (t0 + PAD) / chunk, b1 = (t0 + cells - 1) / chunk;
             if (b0 == b1) continue;
             slot = 2 * b0 + 1;  // the next 2 (b0 + 1), every other slot from there
             nr = b1 - b0 + 1;
         } else {
             nr = ranges(sp.tiles, chunk);
-            slot = before + x / rows * nr;
+            slot = before + unit * nr;
         }
-        const size_t step = (size_t)A.P.heads * (rows * (D + 2)) * (line ? 2 : 1);
-        const size_t head = (size_t)h * (rows * (D + 2));
-        const float *part = A.a.parts + (size_t)(slot + 1) * A.P.heads * (rows * (D + 2)) + head;  // of range 1
-        const float *part0 = A.a.parts + (size_t)slot * A.P.heads * (rows * (D + 2)) + head;
-        auto at = [&](int k) { return k ? part + (size_t)(k - 1) * step : part0; };
-        float top = -INFINITY;
-        for (int k = lane; k < nr; k += 64) top = fmaxf(top, at(k)[rows * D + r]);
-        top = wave_max(top);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float o[D / 64], sum = 0.0f;
+        const int sub = lane / LPR, x = x0 + sub, r = x % rows, d = lane % LPR * 4;
+        if (sub < RPW && x < (q.r1 - q.r0) * A.G) {
+            const size_t unit_size = (size_t)rows * (D + 2), step = (size_t)A.P.heads * unit_size * (line ? 2 : 1);
+            const float *part0 = A.a.parts + ((size_t)slot * A.P.heads + h) * unit_size;
+            const float *part1 = part0 + (size_t)A.P.heads * unit_size;  // of range 1
+            float top = -INFINITY, sum = 0.0f;
+            f32x4 o[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+            for (int k0 = 0; k0 < nr; k0 += U) {
+                float m[U], l[U];
+                f32x4 v[U];
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) o[i] = 0.0f;
-        for (int k0 = 0; k0 < nr; k0 += 64) {
-            const int n = min(64, nr - k0);
-            float f = 0.0f, l = 0.0f;
-            if (lane < n) {
-                const float *p = at(k0 + lane) + rows * D + r;
-                f = exp2_(p[0] - base);
-                l = f * p[rows];
-            }
-            sum += wave_sum(l);
-            for (int k = 0; k < n; k += 8) {
-                float v[8][D / 64];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float *p = at(k0 + min(k + e, n - 1)) + r * D + lane;
-#pragma unroll
-                    for (int i = 0; i < D / 64; i++) v[e][i] = p[64 * i];
+                for (int e = 0; e < U; e++) {
+                    const int k = min(k0 + e, nr - 1);
+                    const float *p = k ? part1 + (size_t)(k - 1) * step : part0;
+                    m[e] = p[rows * D + r];
+                    l[e] = p[rows * D + rows + r];
+                    v[e] = *reinterpret_cast<const f32x4 *>(p + r * D + d);
                 }
+                float to = top;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k + e));
+                for (int e = 0; e < U; e++) to = fmaxf(to, m[e]);  // the last one again: no change
+                const float base = to == -INFINITY ? 0.0f : to, back = exp2_(top - base);
+                top = to;
+                sum *= back;
 #pragma unroll
-                    for (int i = 0; i < D / 64; i++) o[i] = k + e < n ? __builtin_fmaf(fk, v[e][i], o[i]) : o[i];
+                for (int i = 0; i < 4; i++) o[0][i] *= back;
+#pragma unroll
+                for (int e = 0; e < U; e++) {
+                    const bool in = k0 + e < nr;  // (a select: past the end may be a NaN times 0)
+                    const float f = exp2_(m[e] - base);
+                    sum = in ? __builtin_fmaf(f, l[e], sum) : sum;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[0][i] = in ? __builtin_fmaf(f, v[e][i], o[0][i]) : o[0][i];
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[0][i] /= sum;
+            const size_t at = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D + d;
+            store_row<1>(A.a.out, A.a.out_dtype, at, A.vec & 4, o, 1.0f, sum == 0.0f);
         }
-        const size_t to = (size_t)(q.r0 + x / A.G) * A.a.out_stride + (size_t)(h * A.G + x % A.G) * D;
-#pragma unroll
-        for (int i = 0; i < D / 64; i++)
-            store_any(A.a.out, A.a.out_dtype, to + lane + 64 * i, sum == 0.0f ? 0.0f : o[i] / sum);
     }
 }
 
@@ -1035,8 +1040,10 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A) {
 // adds less than one in 2^10 (n_seqs is at most 2^20).  In a line the blocks have two slots each, and
 // there is at most one block more per head: heads are at most target / 20 there.
 constexpr int slots(int target) { return 2 * target + target / 8; }
-constexpr size_t PARTS = (size_t)34 << 20;
-size_t kv_attention_parts_bytes() { return PARTS; }
+// Partial results of units of ROWS and of P_ROWS rows.  Room for TARGET blocks of few rows at every
+// head size, for 127 (256 dimensions) to 500 of many.
+constexpr size_t FEW_PARTS = (size_t)18 << 20, MANY_PARTS = (size_t)34 << 20;
+size_t kv_attention_parts_bytes() { return FEW_PARTS + MANY_PARTS; }
 
 hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_head, const KvAttention &a, hipStream_t s) {
     if (!rows.n_rows) return hipSuccess;
@@ -1044,43 +1051,56 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
     const size_t x = (size_t)rows.n_rows * G;
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        auto part = [&](bool many, int lo, int hi) {
-            Args A{pool, rows, a, G, many ? P_ROWS : ROWS, lo, hi, 0, 0};
-            const size_t fit = PARTS / ((size_t)A.rows * (D + 2) * sizeof(float));  // slots
-            A.target = std::min(TARGET, (int)(fit * 16 / 34));
-            // units of the part at most
-            size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
-            if (hi != INT_MAX) u = std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
-            const bool split = rows.cap > MIN_CHUNK * TILE, f32 = a.out_dtype == T_F32;
-            const dim3 grid((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
+        const bool f32 = a.out_dtype == T_F32;
+        int vec = 0;
+        if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * (a.q_dtype == T_F32 ? 4 : 2) % 16 == 0) vec |= 1;
+        if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) vec |= 2;
+        if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride * (f32 ? 4 : 2) % 16 == 0) vec |= 4;
+        Args join[2];
+        int joins = 0;
+        bool in_line = false;
+        // units of the part at most, and its grid
+        auto units = [&](const Args &A, int hi) {
+            const size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
+            return hi == INT_MAX ? u : std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
+        };
+        auto grid = [&](Args &A, size_t u) {
+            const bool split = rows.cap > A.min_chunk * TILE;
+            if (split) join[joins++] = A;
+            return dim3((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
+        };
+        auto target = [](size_t room, int unit) { return std::min(TARGET, (int)(room / ((size_t)unit * (D + 2) * sizeof(float)) * 16 / 34)); };
+        auto few = [&](int hi) {
+            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), MIN_CHUNK, 0, vec};
+            const size_t u = units(A, hi);
             // can its tiles come to a line at all?
-            const bool line = !many && split && pool.heads * 20 <= A.target &&
-                              (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
-            auto few = [&](auto l) {
-                constexpr bool LINE = decltype(l)::value;
-                if (f32) hipLaunchKernelGGL((k_kv_attention<D, true, LINE>), grid, dim3(64 * WAVES), 0, s, A);
-                else hipLaunchKernelGGL((k_kv_attention<D, false, LINE>), grid, dim3(64 * WAVES), 0, s, A);
-                if (split) hipLaunchKernelGGL((k_kv_join<D, LINE>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
-            };
-            if (!many) {
-                if (line) few(std::true_type{});
-                else few(std::false_type{});
-                return;
-            }
-            const int size = a.q_dtype == T_F32 ? 4 : 2;
-            if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * size % 16 == 0) A.vec |= 1;
-            if (reinterpret_cast<uintptr_t>(a.rope.cs) % 16 == 0) A.vec |= 2;
-            if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride * (f32 ? 4 : 2) % 16 == 0) A.vec |= 4;
-            if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
-            else hipLaunchKernelGGL((k_kv_prompt<D, false>), grid, dim3(64 * P_WAVES), 0, s, A, rows.pages);
-            if (split) hipLaunchKernelGGL((k_kv_join<D, false>), dim3(JOIN_BLOCKS), dim3(256), 0, s, A);
+            A.line = rows.cap > MIN_CHUNK * TILE && pool.heads * 20 <= A.target &&
+                     (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
+            in_line = A.line;
+            const dim3 g = grid(A, u), b(64 * WAVES);
+            if (A.line && f32) hipLaunchKernelGGL((k_kv_attention<D, true, true>), g, b, 0, s, A);
+            else if (A.line) hipLaunchKernelGGL((k_kv_attention<D, false, true>), g, b, 0, s, A);
+            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, true, false>), g, b, 0, s, A);
+            else hipLaunchKernelGGL((k_kv_attention<D, false, false>), g, b, 0, s, A);
+        };
+        auto many = [&](int lo) {
+            Args A{pool, rows, a, G, P_ROWS, lo, INT_MAX, target(MANY_PARTS, P_ROWS), P_MIN_CHUNK, 0, vec};
+            A.a.parts += FEW_PARTS / sizeof(float);
+            const dim3 g = grid(A, units(A, INT_MAX)), b(64 * P_WAVES);
+            if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), g, b, 0, s, A, rows.pages);
+            else hipLaunchKernelGGL((k_kv_prompt<D, false>), g, b, 0, s, A, rows.pages);
         };
         if (x > (size_t)FEW * rows.n_seqs) {
-            part(true, FEW + 1, INT_MAX);
-            part(false, 0, FEW);
+            many(FEW + 1);
+            few(FEW);
         } else {
-            part(false, 0, INT_MAX);
+            few(INT_MAX);
         }
+        if (!joins) return;
+        constexpr int RPB = 4 * (256 / D);  // rows of a block
+        const dim3 g((unsigned)std::min((size_t)JOIN_BLOCKS, (x * pool.heads + RPB - 1) / RPB), (unsigned)joins), b(256);
+        if (in_line) hipLaunchKernelGGL((k_kv_join<D, true>), g, b, 0, s, join[0], join[joins - 1]);
+        else hipLaunchKernelGGL((k_kv_join<D, false>), g, b, 0, s, join[0], join[joins - 1]);
     };
     switch (d_head) {
     case 64: go(std::integral_constant<int, 64>{}); break;
