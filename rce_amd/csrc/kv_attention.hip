@@ -46,6 +46,10 @@ constexpr int WAVES = 4;    // of a block
 constexpr int TILE = 64;    // positions of a wave's step
 constexpr int TARGET = 512;   // blocks that a part's tiles are spread over: two per CU
 constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
+// Tables of up to so many tiles are not split: one sequence of 1000 in one range 16 us, in two 13 and the join 5;
+// of 4000 in ranges of 8 tiles 12.5 + 5, in ranges of 24 19 + 5.
+constexpr int SPLIT_FROM = 16;
+constexpr int WHOLE = 1 << 24;  // tiles of a range where there is no split
 constexpr int P_MIN_CHUNK = 4;  // of units of P_ROWS rows
 constexpr int LINE_CHUNK = 24;  // tiles per block from which a block may serve several units
 constexpr int PAD = 4;          // a unit's prologue and epilogue, in the time of a tile
@@ -266,15 +270,123 @@ __device__ __forceinline__ void limbs_of(const float (&x)[16], float id, i32x4 (
     }
 }
 
-// LDS: the query rows in f32 before the loop, the waves' results after it (at
-// most 128 dimensions at a time: 34 KB).
+// N pieces of 16 values from the value indexes i: at multiples of 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_pieces(const void *p, uint32_t t, const size_t (&i)[N], float (&x)[N][16]) {
+    if (t == T_F32) {
+        float4 v[N][4];
+#pragma unroll
+        for (int s = 0; s < N; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[s][k] = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i[s])[k];
+#pragma unroll
+        for (int s = 0; s < N; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[s][4 * k] = v[s][k].x;
+                x[s][4 * k + 1] = v[s][k].y;
+                x[s][4 * k + 2] = v[s][k].z;
+                x[s][4 * k + 3] = v[s][k].w;
+            }
+        return;
+    }
+    u32x4 v[N][2];
+#pragma unroll
+    for (int s = 0; s < N; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) v[s][k] = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i[s])[k];
+    const bool f16 = t == T_F16;
+#pragma unroll
+    for (int s = 0; s < N; s++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const uint32_t w = v[s][k >> 2][k & 3];
+            const half2v e = as_h2(w);
+            x[s][2 * k] = f16 ? (float)e.x : __uint_as_float(w << 16);
+            x[s][2 * k + 1] = f16 ? (float)e.y : __uint_as_float(w & 0xFFFF0000u);
+        }
+}
+
+// Row x_row of the sequence and kv head h, rotated to position pos, as codes: the 16 dimensions
+// 64 s + 16 g .. of this lane in qf[s], the factor of its base-2 scores in qs.  is: the row has a position.
+template <int D, int LIMBS>
+__device__ __forceinline__ void query_codes(const Args &A, const KvSeq &q, int h, int x_row, int pos, bool is, int g,
+                                            i32x4 (&qf)[D / 64][LIMBS], float &qs) {
+    constexpr int NQ = D / 64;
+    constexpr float QMAX = LIMBS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
+    float x[NQ][16];
+    const int half = A.a.rope.cs ? A.a.rope.half : 0;
+    // A row without a position reads row 0 of the call and of the table, and is zeroed after:
+    // no load stands under a condition of its lane, all are in flight together.
+    const size_t at = is ? (size_t)(q.r0 + x_row / A.G) * A.a.q_stride + (size_t)(h * A.G + x_row % A.G) * D : 0;
+    const float *cs = A.a.rope.cs + (size_t)(is ? pos : 0) * half * 2;
+    if ((A.vec & 3) == 3 && half % 16 == 0) {  // the pieces' partners are whole pieces too
+        size_t own[NQ], other[NQ];
+#pragma unroll
+        for (int s = 0; s < NQ; s++) {
+            const int d = 64 * s + 16 * g;
+            own[s] = at + d;
+            other[s] = at + (d < half ? d + half : d < 2 * half ? d - half : d);
+        }
+        load_pieces<NQ>(A.a.q, A.a.q_dtype, own, x);
+        if (half) {
+            float y[NQ][16];
+            load_pieces<NQ>(A.a.q, A.a.q_dtype, other, y);
+#pragma unroll
+            for (int s = 0; s < NQ; s++) {
+                const int d = 64 * s + 16 * g;
+                const bool lo = d < half, turns = d < 2 * half;
+                const float4 *c = reinterpret_cast<const float4 *>(cs + 2 * (lo ? d : turns ? d - half : 0));
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 v = c[j];
+                    const float ac = x[s][2 * j] * v.x, as = y[s][2 * j] * v.y;
+                    const float bc = x[s][2 * j + 1] * v.z, bs = y[s][2 * j + 1] * v.w;
+                    const float a = lo ? ac - as : as + ac, b = lo ? bc - bs : bs + bc;
+                    x[s][2 * j] = turns ? a : x[s][2 * j];
+                    x[s][2 * j + 1] = turns ? b : x[s][2 * j + 1];
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < NQ; s++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int d = 64 * s + 16 * g + j;
+                x[s][j] = load_any(A.a.q, A.a.q_dtype, at + d);
+                if (d < 2 * half) {
+                    const bool lo = d < half;
+                    const int k = lo ? d : d - half;
+                    const float p = load_any(A.a.q, A.a.q_dtype, at + (lo ? d + half : k));
+                    const float xc = x[s][j] * cs[2 * k], ys = p * cs[2 * k + 1];
+                    x[s][j] = lo ? xc - ys : ys + xc;
+                }
+            }
+    }
+    float amax = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int s = 0; s < NQ; s++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            x[s][j] = is ? x[s][j] : 0.0f;
+            amax = fmaxf(amax, fabsf(x[s][j]));
+            bad |= !(fabsf(x[s][j]) < __builtin_inff());
+        }
+    amax = swap_max(amax);
+    bad = swap_max(bad ? 1.0f : 0.0f) != 0.0f;
+    const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
+    qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
+#pragma unroll
+    for (int s = 0; s < NQ; s++) limbs_of<LIMBS>(x[s], id, qf[s]);
+}
+
+// LDS: the waves' results (at most 128 dimensions at a time: 34 KB).
 template <int D>
 struct Shared {
     static constexpr int PART = D <= 128 ? D : D / 2;
-    union {
-        alignas(16) float q[ROWS][D + 4];
-        alignas(16) float o[WAVES][ROWS][PART + 4];
-    };
+    alignas(16) float o[WAVES][ROWS][PART + 4];
     float m[WAVES][ROWS], l[WAVES][ROWS];
 };
 
@@ -282,7 +394,6 @@ template <int D, bool HILO, bool LINE>
 __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 192 ? 2 : 1) void k_kv_attention(Args A) {
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
-    constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
     __shared__ Shared<D> sh;
     int block = blockIdx.x;
     const Cut cut = cut_of<LINE>(A);
@@ -302,64 +413,13 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
     const int G = A.G, first = q.first();
     const int x0 = w.unit * ROWS, n_x = min(ROWS, (q.r1 - q.r0) * G - x0);  // rows of the unit
 
-    // the query rows, rotated, to LDS; rows past the unit's or without a position: zeros
-    for (int i = tid; i < ROWS * D; i += 64 * WAVES) {
-        const int r = i / D, d = i % D;
-        float x = 0.0f;
-        const int tok = (x0 + r) / G, pos = first + tok;
-        if (r < n_x && pos >= 0 && pos < A.B.cap) {
-            const size_t at = (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + r) % G) * D;
-            x = load_any(A.a.q, A.a.q_dtype, at + d);
-            const int half = A.a.rope.half;
-            if (A.a.rope.cs && d < 2 * half) {
-                const bool lo = d < half;
-                const int k = lo ? d : d - half;
-                const float y = load_any(A.a.q, A.a.q_dtype, at + (lo ? d + half : k));
-                const float *cs = A.a.rope.cs + ((size_t)pos * half + k) * 2;
-                const float xc = x * cs[0], ys = y * cs[1];
-                x = lo ? xc - ys : ys + xc;
-            }
-        }
-        sh.q[r][d] = x;
-    }
-    __syncthreads();
-
     // this lane's query row: positions it sees, codes and scale
-    int p_hi = -1, p_lo = 0;  // keys p_lo .. p_hi
-    if (n < n_x) {
-        const int pos = first + (x0 + n) / G;
-        if (pos >= 0 && pos < A.B.cap) {
-            p_hi = pos;
-            p_lo = max(0, pos - (A.a.window - 1));
-        }
-    }
+    const int pos = first + (x0 + n) / G;
+    const bool is = n < n_x && pos >= 0 && pos < A.B.cap;
+    const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;  // keys p_lo .. p_hi
     i32x4 qf[NQ][LIMBS];
     float qs;
-    {
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int s = 0; s < NQ; s++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float x = fabsf(sh.q[n][64 * s + 16 * g + j]);
-                amax = fmaxf(amax, x);
-                bad |= !(x < __builtin_inff());
-            }
-        amax = swap_max(amax);
-        bad = swap_max(bad ? 1.0f : 0.0f) != 0.0f;
-        // below 2^-100 a row's scores vanish beside any scale in use
-        const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
-        qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
-#pragma unroll
-        for (int s = 0; s < NQ; s++) {
-            float x[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = sh.q[n][64 * s + 16 * g + j];
-            limbs_of<LIMBS>(x, id, qf[s]);
-        }
-    }
-    __syncthreads();  // sh.q is read; sh.o may be written
+    query_codes<D, LIMBS>(A, q, h, x0 + n, pos, is, g, qf, qs);
 
     // tiles of this unit and range; keys that every row sees need no mask
     const int u_tok0 = x0 / G, u_tok1 = (x0 + n_x - 1) / G;
@@ -522,7 +582,7 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
     }
     line_at += n_cells;
     if (!LINE || !cut.line || line_at >= line_end) return;
-    __syncthreads();  // sh.o is read; sh.q may be written
+    __syncthreads();  // sh is read
   }
 }
 
@@ -542,43 +602,6 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
 // the LDS reads per product).
 constexpr int P_ROWS = 128, P_WAVES = 8;
 constexpr float LAG = 6.0f, UP = 512.0f;  // UP = 2^9
-
-// N pieces of 16 values from the value indexes i: at multiples of 16 bytes.
-template <int N>
-__device__ __forceinline__ void load_pieces(const void *p, uint32_t t, const size_t (&i)[N], float (&x)[N][16]) {
-    if (t == T_F32) {
-        float4 v[N][4];
-#pragma unroll
-        for (int s = 0; s < N; s++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[s][k] = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i[s])[k];
-#pragma unroll
-        for (int s = 0; s < N; s++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                x[s][4 * k] = v[s][k].x;
-                x[s][4 * k + 1] = v[s][k].y;
-                x[s][4 * k + 2] = v[s][k].z;
-                x[s][4 * k + 3] = v[s][k].w;
-            }
-        return;
-    }
-    u32x4 v[N][2];
-#pragma unroll
-    for (int s = 0; s < N; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) v[s][k] = reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i[s])[k];
-    const bool f16 = t == T_F16;
-#pragma unroll
-    for (int s = 0; s < N; s++)
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const uint32_t w = v[s][k >> 2][k & 3];
-            const half2v e = as_h2(w);
-            x[s][2 * k] = f16 ? (float)e.x : __uint_as_float(w << 16);
-            x[s][2 * k + 1] = f16 ? (float)e.y : __uint_as_float(w & 0xFFFF0000u);
-        }
-}
 
 // A lane's accumulators times f: four consecutive values every 16 from value index i; vec:
 // at multiples of their size.
@@ -627,7 +650,6 @@ template <int D, bool HILO>
 __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k_kv_prompt(Args A, const int32_t *__restrict__ page_table) {
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
-    constexpr float QMAX = HILO ? 127.0f * 65536.0f : 127.0f * 256.0f;
     constexpr int NK = (TILE * D + 16 * 64 * P_WAVES - 1) / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
     constexpr int BUFS = D <= 128 ? 2 : 1;  // two where they fit 64 KB
     __shared__ PShared<D> buf[BUFS];
@@ -645,74 +667,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
 
     i32x4 qf[NQ][LIMBS];
     float qs;
-    {
-        float x[NQ][16];
-        const int half = A.a.rope.cs ? A.a.rope.half : 0;
-        // A row without a position reads row 0 of the call and of the table, and is zeroed after:
-        // no load stands under a condition of its lane, all are in flight together.
-        const size_t at = is ? (size_t)(q.r0 + tok) * A.a.q_stride + (size_t)(h * G + (x0 + xr) % G) * D : 0;
-        const float *cs = A.a.rope.cs + (size_t)(is ? pos : 0) * half * 2;
-        if ((A.vec & 3) == 3 && half % 16 == 0) {  // the pieces' partners are whole pieces too
-            size_t own[NQ], other[NQ];
-#pragma unroll
-            for (int s = 0; s < NQ; s++) {
-                const int d = 64 * s + 16 * g;
-                own[s] = at + d;
-                other[s] = at + (d < half ? d + half : d < 2 * half ? d - half : d);
-            }
-            load_pieces<NQ>(A.a.q, A.a.q_dtype, own, x);
-            if (half) {
-                float y[NQ][16];
-                load_pieces<NQ>(A.a.q, A.a.q_dtype, other, y);
-#pragma unroll
-                for (int s = 0; s < NQ; s++) {
-                    const int d = 64 * s + 16 * g;
-                    const bool lo = d < half, turns = d < 2 * half;
-                    const float4 *c = reinterpret_cast<const float4 *>(cs + 2 * (lo ? d : turns ? d - half : 0));
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float4 v = c[j];
-                        const float ac = x[s][2 * j] * v.x, as = y[s][2 * j] * v.y;
-                        const float bc = x[s][2 * j + 1] * v.z, bs = y[s][2 * j + 1] * v.w;
-                        const float a = lo ? ac - as : as + ac, b = lo ? bc - bs : bs + bc;
-                        x[s][2 * j] = turns ? a : x[s][2 * j];
-                        x[s][2 * j + 1] = turns ? b : x[s][2 * j + 1];
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < NQ; s++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int d = 64 * s + 16 * g + j;
-                    x[s][j] = load_any(A.a.q, A.a.q_dtype, at + d);
-                    if (d < 2 * half) {
-                        const bool lo = d < half;
-                        const int k = lo ? d : d - half;
-                        const float p = load_any(A.a.q, A.a.q_dtype, at + (lo ? d + half : k));
-                        const float xc = x[s][j] * cs[2 * k], ys = p * cs[2 * k + 1];
-                        x[s][j] = lo ? xc - ys : ys + xc;
-                    }
-                }
-        }
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int s = 0; s < NQ; s++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                x[s][j] = is ? x[s][j] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[s][j]));
-                bad |= !(fabsf(x[s][j]) < __builtin_inff());
-            }
-        amax = swap_max(amax);
-        bad = swap_max(bad ? 1.0f : 0.0f) != 0.0f;
-        const float id = bad || amax < 0x1p-100f ? 0.0f : QMAX / amax;
-        qs = bad ? __builtin_nanf("") : id == 0.0f ? 0.0f : amax / QMAX * A.a.scale * LOG2E;
-#pragma unroll
-        for (int s = 0; s < NQ; s++) limbs_of<LIMBS>(x[s], id, qf[s]);
-    }
+    query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
 
     const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;
     // the wave's rows: positions that all of them see, or that any of them sees
@@ -1065,16 +1020,16 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
             return hi == INT_MAX ? u : std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
         };
         auto grid = [&](Args &A, size_t u) {
-            const bool split = rows.cap > A.min_chunk * TILE;
+            const bool split = rows.cap > (int64_t)A.min_chunk * TILE;
             if (split) join[joins++] = A;
             return dim3((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
         };
         auto target = [](size_t room, int unit) { return std::min(TARGET, (int)(room / ((size_t)unit * (D + 2) * sizeof(float)) * 16 / 34)); };
         auto few = [&](int hi) {
-            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), MIN_CHUNK, 0, vec};
+            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), rows.cap > SPLIT_FROM * TILE ? MIN_CHUNK : WHOLE, 0, vec};
             const size_t u = units(A, hi);
             // can its tiles come to a line at all?
-            A.line = rows.cap > MIN_CHUNK * TILE && pool.heads * 20 <= A.target &&
+            A.line = rows.cap > SPLIT_FROM * TILE && pool.heads * 20 <= A.target &&
                      (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
             in_line = A.line;
             const dim3 g = grid(A, u), b(64 * WAVES);
