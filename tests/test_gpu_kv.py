@@ -297,6 +297,29 @@ def test_attention_in_line_of_many_units(ctx):
     check_attention(ctx, 64, 1, 1, 256, lens, [min(n, 1) for n in lens], G.F16, G.F16)
 
 
+def test_attention_of_sequences_that_share_their_pages(ctx):
+    """16384 sequences of the same pages: block number times a block's cells passes 31 bits.
+    Four queries in turn, so that every row has its expected value."""
+    rng = np.random.default_rng(14)
+    n, length, page, heads, d = 16384, 33000, 1024, 8, 64
+    one, n_pages = kc.make_batch(rng, [length], [4], page)
+    pool = kc.Pool(n_pages, page, heads, d, rng)
+    four = kc.Batch([length] * 4, [1] * 4, np.repeat(one.pages, 4, 0), page)
+    batch = kc.Batch([length] * n, [1] * n, np.repeat(one.pages, n, 0), page)
+    q = kc.to_bits(rng.standard_normal((4, heads * d)).astype(F32), G.F16)
+    dev = kc.Device(ctx, pool, batch)
+    x = rce_amd.DeviceBuffer.from_numpy(ctx, np.tile(q, (n // 4, 1)))
+    out = rce_amd.DeviceBuffer(ctx, n * heads * d * 2)
+    rce_amd.kv_attention_dev(ctx, dev.cache, dev.b, x.ptr, G.F16, heads * d, heads, out.ptr, G.F16, 0.125)
+    ctx.synchronize()
+    got = out.download(np.float16, n * heads * d).reshape(n // 4, 4, heads, d).astype(np.float64)
+    want, bound = kc.attention(pool, four, q.astype(F32).reshape(4, heads, d), None, 0.125, 0, False)
+    assert np.all(np.abs(got - want) <= bound + kc.out_eps(G.F16) * (np.abs(want) + bound) + 2.0 ** -25)
+    for b in (x, out):
+        b.free()
+    dev.free()
+
+
 def test_attention_many_sequences(ctx):
     """More sequences than a wave has lanes, empty ones among them."""
     rng = np.random.default_rng(11)
