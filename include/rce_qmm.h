@@ -445,7 +445,9 @@ rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache 
  * on the matrix cores; softmax in f32; its weights rounded to binary16 (out_dtype
  * F32: two binary16 terms) against the value codes, f32 sums.  Fixed order for
  * a batch: run-to-run bit-identical; a row's last bits depend on the batch.
- * Calls that split long sequences use a buffer allocated with the context. */
+ * Calls that split long sequences use a buffer allocated with the context
+ * (as rce_qmm_sample_dev does for long rows): a recorded call stays valid, and
+ * calls or graphs that may run at the same time need a context each. */
 rce_qmm_status rce_qmm_kv_attention_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
                                         const rce_qmm_kv_batch *batch, const void *q_dev, uint32_t q_dtype,
                                         size_t q_stride, size_t n_q_heads, const rce_qmm_rope *rope, float scale,
@@ -474,7 +476,8 @@ typedef struct rce_qmm_sampling {
  * probability 0.  vocab at most 2^24.
  * Weights are exponentials to 2^-46 as whole numbers, the largest 2^S, S = min(50,
  * 62 - ceil(log2 vocab)), so every sum is exact in any order: run-to-run
- * identical. */
+ * identical, whatever the other rows.  Rows of more than 128 KB in calls of at
+ * most 128 rows use the context's buffer (see rce_qmm_kv_attention_dev). */
 rce_qmm_status rce_qmm_sample_dev(rce_qmm_context *ctx, const void *logits_dev, uint32_t dtype, size_t n_rows,
                                   size_t vocab, size_t row_stride, const rce_qmm_sampling *sampling, int32_t *ids_dev,
                                   float *probs_dev, void *stream);

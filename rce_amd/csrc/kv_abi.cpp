@@ -241,7 +241,7 @@ rce_qmm_status rce_qmm_kv_attention_dev(rce_qmm_context *ctx, const rce_qmm_kv_c
             return st;
         if (!r.cap) return fail(RCE_QMM_BAD_SHAPE, "max_pages must be at least 1");
         const size_t rows = (size_t)r.n_rows * n_q_heads;
-        if (rows > (size_t)INT_MAX / 2 || (rows / 16 + ((size_t)r.n_seqs + 2) * p.heads + 4096) * 4 > MAX_WAVES)
+        if (rows > (size_t)INT_MAX / 2 || (rows / 12 + ((size_t)r.n_seqs + 2) * p.heads + 4096) * 4 > MAX_WAVES)
             return fail(RCE_QMM_BAD_SHAPE, "too many rows and heads for one launch");
         a.q = q_dev;
         a.q_dtype = q_dtype;

@@ -113,6 +113,35 @@ def test_long_rows(ctx, n):
     Call(ctx, x, G.F32, u, **par).check()
 
 
+def test_long_rows_recorded_and_replayed():
+    """The kernels of split rows share a buffer of the context's: replays between other calls of
+    both kinds equal the expected tokens every time."""
+    with rce_amd.Context(0) as c:
+        x, u = rows(21, 5, 90001)
+        a = Call(c, x, G.F32, u, top_p=0.9, temperature=0.8)
+        y, w = rows(22, 3, 50001)
+        b = Call(c, y, G.F32, w, top_k=30, top_p=0.9)
+        hip = Hip()
+        g, ex = hip.capture(c.stream, a.call)
+        for i in range(4):
+            u = np.roll(u, 1)
+            a.u = u
+            a.ub.upload(u)
+            a.ids.upload(np.full(6, -77, np.int32))
+            b.call()
+            c.synchronize()
+            hip.launch(ex, c.stream)
+            b.call()
+            c.synchronize()
+            for call in (a, b):
+                ids, probs = call.result()
+                for r, (t, p) in enumerate(call.expect()):
+                    assert ids[r] == t and abs(probs[r] - p) <= 2.0 ** -23 * p
+        hip.destroy(g, ex)
+        a.free()
+        b.free()
+
+
 @pytest.mark.parametrize("par", [{}, {"top_k": 2000}, {"top_p": 0.37}, {"top_p": 0.6, "top_k": 50000}, {"min_p": 1.0}], ids=str)
 def test_long_rows_of_equal_and_missing_logits(ctx, par):
     x, u = rows(11, 6, 70001)
