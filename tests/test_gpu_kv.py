@@ -289,6 +289,13 @@ def test_attention_long_ragged_sequences_in_line(ctx, out_dtype, window):
                     rope=64, window=window)
 
 
+@pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
+def test_attention_long_tokens_in_line_beside_prompts(ctx, out_dtype):
+    """Both parts of a call split, one of them as a line: one join for both."""
+    check_attention(ctx, 64, 8, 2, 128, [30000, 900, 28001, 33333, 64, 31000, 29999], [1, 150, 2, 1, 64, 1, 1], G.F16, out_dtype,
+                    rope=64, n_rows=225)
+
+
 def test_attention_in_line_of_many_units(ctx):
     """More sequences than a wave has lanes, several of them in a block."""
     rng = np.random.default_rng(8)
