@@ -56,6 +56,10 @@ constexpr int MIN_CHUNK = 8;  // tiles of the shortest range
 // Tables of up to so many tiles are not split: one sequence of 1000 in one range 16 us, in two 13 and the join 5;
 // of 4000 in ranges of 8 tiles 12.5 + 5, in ranges of 24 19 + 5.
 constexpr int SPLIT_FROM = 16;
+// A single sequence in a table of up to so many tiles has one part whatever its rows turn out to be: 64 rows
+// of 64 11 us against 13 with a launch for few rows too, 12 after 5000 21 : 24, 512 after 4096 82 : 87. One row in a
+// batch with room for 16: at 4096 positions 18 : 18, at 32768 38 : 32, at 131072 101 : 59.
+constexpr int ONE_TABLE = 128;
 constexpr int WHOLE = 1 << 24;  // tiles of a range where there is no split
 constexpr int P_MIN_CHUNK = 4;  // of units of P_ROWS rows: 3 x 201 f32 in ranges of 4 tiles 21 us, of 8 25, of 2 28
 constexpr int LINE_CHUNK = 24;  // tiles per block from which a block may serve several units
@@ -1059,8 +1063,9 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
             else hipLaunchKernelGGL((k_kv_prompt<D, false>), g, b, 0, s, A, rows.pages);
         };
         if (x > (size_t)FEW * rows.n_seqs) {
-            many(FEW + 1);
-            few(FEW);
+            const bool one = rows.n_seqs == 1 && rows.cap <= ONE_TABLE * TILE;
+            many(one ? 0 : FEW + 1);
+            if (!one) few(FEW);
         } else {
             few(INT_MAX);
         }

@@ -352,6 +352,12 @@ def test_attention_prompts_of_every_head_size(ctx, d, rope, q_dtype, out_dtype):
     check_attention(ctx, d, 2, 3, 32, [43, 128, 170, 90], [43, 33, 1, 90], q_dtype, out_dtype, rope=rope)
 
 
+@pytest.mark.parametrize("length,new", [(0, 0), (1, 1), (700, 1), (700, 5), (300, 300), (7000, 20), (20000, 1), (20000, 90)])
+def test_attention_of_one_sequence_in_a_padded_batch(ctx, length, new):
+    for t in (G.F32, G.F16):
+        check_attention(ctx, 64, 2, 2, 64, [length], [new], t, t, rope=64, n_rows=new + 40)
+
+
 @pytest.mark.parametrize("page", [16, 64, 1024])
 @pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
 def test_attention_prompts_after_long_contexts(ctx, page, out_dtype):
