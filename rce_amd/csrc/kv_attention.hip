@@ -691,8 +691,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int w0 = wave * 16, w_n = min(16, n_x - w0);  // rows (none: w_n <= 0)
     const int f0 = first + (x0 + w0) / G, f1 = first + (x0 + w0 + max(w_n, 1) - 1) / G;
     const bool placed = w_n > 0 && f0 >= 0 && f1 < A.B.cap;
-    const int w_lo = max(0, f0 - (A.a.window - 1)), w_hi = w_n > 0 ? min(f1, A.B.cap - 1) : -1;
-    const int all_lo = max(0, f1 - (A.a.window - 1)), all_hi = f0;
+    const int w_lo = max(0, max(0, f0) - (A.a.window - 1)), w_hi = w_n > 0 ? min(f1, A.B.cap - 1) : -1;
+    const int all_lo = max(0, max(0, f1) - (A.a.window - 1)), all_hi = f0;
     // the block's tiles
     const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
     int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;

@@ -416,6 +416,14 @@ def test_attention_rows_left_out(ctx):
     check_attention(ctx, 128, 1, 1, 16, [100, 40, 32], [100, 20, 1], G.F16, G.F16, edit=short)
 
 
+@pytest.mark.parametrize("window", [0, 1, 40])
+@pytest.mark.parametrize("per", [1, 3])
+def test_attention_prompts_with_rows_before_the_first_position(ctx, per, window):
+    """A unit's 16 rows begin at negative positions and end at valid ones."""
+    check_attention(ctx, 64, 1, per, 16, [100, 3, 64], [130, 150, 70], G.F32, G.F32, rope=64, window=window)
+    check_attention(ctx, 128, 1, per, 16, [100, 3, 64], [130, 150, 70], G.F16, G.F16, window=window)
+
+
 @pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_attention_non_finite_blocks(ctx, bad, out_dtype):
