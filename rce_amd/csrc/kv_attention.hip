@@ -767,7 +767,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     f32x4 acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f, ref = 0.0f, inv_ref = 0.0f;
+    // (ref from 2^-110 on: UP / ref stays finite, and smaller scales keep 2^-18 of the largest weight)
+    float m = -INFINITY, l = 0.0f, ref = 0x1p-110f, inv_ref = UP * 0x1p110f;
     // This lane's operands in LDS: key position 16 (n / 4) + n % 4 + 4 i, piece 4 s + g, and value
     // row n + 16 i, piece 2 g + u.
     const int k_pos = 16 * (n >> 2) + (n & 3);
@@ -848,7 +849,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                     for (int e = 0; e < 4; e++) acc[i][e] *= back;
                 m = m_new;
                 ref = ref_new;
-                inv_ref = ref > 0.0f ? UP / ref : 0.0f;
+                inv_ref = UP / ref;
             }
             const float base = m == -INFINITY ? 0.0f : m;
             // what the values' scale makes of the weights; an infinite or NaN one makes NaN of the

@@ -459,6 +459,21 @@ def test_attention_values_far_apart(ctx, out_dtype):
     check_attention(ctx, 64, 2, 2, 32, [64, 40, 200], [64, 3, 60], G.F32, out_dtype, scale=2.0)
 
 
+@pytest.mark.parametrize("lens,news", [([400, 90], [200, 90]), ([1500, 90], [1, 2])])
+@pytest.mark.parametrize("exp", [-126, -118, -100])
+def test_attention_of_tiny_values(ctx, exp, lens, news):
+    """Value scales down to 2^-126: as the same call with scales near 1, to a power of two (weights
+    are rounded to 2^-11, or 2^-18 of the largest where the scales are at their least)."""
+    def edit(to):
+        def f(pool, b):
+            r = np.random.default_rng(6)
+            pool.v_scale[:] = (r.uniform(1.0, 1.9, pool.v_scale.shape) * 2.0 ** to).astype(F32)
+        return f
+    got, want = (check_attention(ctx, 64, 1, 2, 32, lens, news, G.F32, G.F32, edit=edit(e)).astype(np.float64) * 2.0 ** -e
+                 for e in (exp, 0))
+    assert np.isfinite(got).all() and np.abs(got - want).max() <= 2.0 ** -10 * np.abs(want).max()
+
+
 def test_attention_strides_and_unwritten_pages(ctx):
     check_attention(ctx, 64, 2, 2, 16, [70, 9], [1, 3], gap=5)
     check_attention(ctx, 128, 2, 1, 16, [70, 9], [1, 3], G.F16, G.F16, gap=1)
