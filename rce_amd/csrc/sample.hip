@@ -522,8 +522,10 @@ __device__ __forceinline__ void bind_row(Row<T, LDS> &row, const SampleRows &R, 
 // block per row.  Rows with top-p and a top_k above NT, and lists of
 // more than NT elements, are left to its own passes.
 //
-// 64 x 128000 f32 with top-p: 8 + 17 + 22 + 15 us, the middle two bound by the f64
-// exponentials (14 f64 instructions per logit); a block per row took 138.  Whole calls, a
+// 64 x 128000 f32 with top-p: 8 + 20 + 22 + 16 us, the gathering bound by VALU issue (10 M
+// instructions, 60 % of its cycles; 16 logits per lane, a third of the instructions in front of
+// them) and by its chain of dependent loads: 4 f64 operations fewer per logit, or half the
+// blocks, leave its time as it is.  A block per row took 138.  Whole calls, a
 // block per row against this (us):
 //                      top-p 0.9  none       top-k 40, top-p  top-k 5000, top-p
 //   64 x 128000 f32     133   62   61   33    27   35          174  180
