@@ -27,7 +27,7 @@
 //                 (k slot 8 g + j of MFMA u is position 16 g + 8 u + j), V^T the
 //                 value codes as stored, 16 positions of a dimension in a
 //                 word.  P carries its block's value scale relative to the
-//                 tile's largest, times 2^14 (so that small weights stay
+//                 largest that its row sees in the tile, times 2^14 (so that small weights stay
 //                 normal in binary16); HILO adds a second binary16 term.
 //
 // What bounds it: the codes' way from HBM, where there are enough of them.  2 x 131072 ragged, 8
@@ -502,9 +502,9 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
                     x[j] = see ? x[j] * f : -INFINITY;
                 }
                 if (!__ballot(any)) continue;
-                // a block that no row sees may hold anything
-                const unsigned long long b = __ballot(any);
-                if (!((b >> (16 * g)) & 0xFFFFull)) sv = 0.0f;
+                // a block that this lane's row does not see may hold anything, values far larger than
+                // all that it does see among it
+                if (!any) sv = 0.0f;
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; j++) x[j] = x[j] * f;
@@ -516,8 +516,8 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
             const float base = m_new == -INFINITY ? 0.0f : m_new;
             const float alpha = exp2_(m - base);
             m = m_new;
-            // The tile's largest (finite) scale gets weights up to 2^14; an infinite
-            // or NaN one makes NaN of the rows that see its block, no others.
+            // The largest (finite) scale that the row sees in the tile gets weights up to 2^14; an
+            // infinite or NaN one makes NaN of the rows that see its block, no others.
             const float sv_max = swap_max(sv < __builtin_inff() ? sv : 0.0f);
             const float pw = sv_max > 0.0f ? sv / sv_max * 16384.0f : sv < __builtin_inff() ? 0.0f : sv;
             float sum = 0.0f;
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
 // with their 16-byte pieces in another order per row (else reads of one piece of
 // 16 rows would fall on the same banks).  The next tile's codes travel to registers meanwhile.
 // O stays in the MFMAs' accumulators, in units of `ref`, the largest value
-// scale so far, and of the row's m.  m moves, and O and l are rescaled, only when a
+// scale that the row has seen, and of the row's m.  m moves, and O and l are rescaled, only when a
 // score passes it by more than LAG (base 2): weights are then at most 2^LAG,
 // times UP in binary16 at most 2^15.
 // 3 prompts of 4096, 32 query and 8 kv heads of 128, f16: 355 GFLOP in 544 us, 30 % of the time of
@@ -788,8 +788,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
             const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
             const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
             // opaque: what is formed from them would be kept over the loop, in registers that spill
-            int k_row = k_row0, v_row = v_row0, my = lane;
-            asm volatile("" : "+v"(k_row), "+v"(v_row), "+v"(my));
+            int k_row = k_row0, v_row = v_row0;
+            asm volatile("" : "+v"(k_row), "+v"(v_row));
             int xi[16];  // scores as whole numbers (HILO: without the highest limb, which is xh)
             float xh[HILO ? 16 : 1];
 #pragma unroll
@@ -820,10 +820,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                 if (masked) {
                     const int p = TILE * t + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
                     seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
-                    // a block that no row of the wave sees may hold anything
-                    const unsigned long long b = __ballot(seen != 0);
-                    const uint32_t half = my < 32 ? (uint32_t)b : (uint32_t)(b >> 32);
-                    if (!(half >> (my & 16) & 0xFFFFu)) sv = 0.0f;
+                    if (!seen) sv = 0.0f;  // as in k_kv_attention
                 }
                 asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
 #pragma unroll
@@ -835,7 +832,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                 top = (float)x * f;
             }
             top = swap_max(top);
-            // `top` above m + LAG, or a larger value scale: rescale
+            // `top` above m + LAG, or a larger value scale that the row sees: rescale (lanes alone for the
+            // scale: a ballot over both costs registers that spill)
             const bool fin = sv < __builtin_inff();
             const float scale = swap_max(fin ? sv : 0.0f);
             if (__ballot(top > m + LAG) || scale > ref) {

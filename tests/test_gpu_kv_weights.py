@@ -1,5 +1,6 @@
-"""Attention's softmax weights where they are small: weights far below the
-largest count in their sum."""
+"""Attention's softmax weights where they are small or meet values of very
+different size: weights far below the largest count in their sum, and what a
+row does not see has no part in its precision."""
 import numpy as np
 import pytest
 
@@ -7,7 +8,7 @@ import kv_case as kc
 import rce_amd
 from kv_case import F32
 from rce_amd import GgufDtype as G
-from test_gpu_kv import Attn
+from test_gpu_kv import Attn, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,21 @@ def test_many_small_weights_count_in_the_sum(ctx, new, n, out_dtype):
     off = np.abs(got / want - 1).max()
     a.free()
     assert off <= allowed, (off, allowed)
+
+
+@pytest.mark.parametrize("out_dtype", [G.F32, G.BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 9])
+def test_values_of_unseen_blocks_cost_no_precision(ctx, d, window, out_dtype):
+    """Each block's values are 2^30 times the last one's, or (rows that see at most 9 positions) the
+    next one's: rows of one unit see values of very different size, and every row is as exact as what
+    it sees allows."""
+    for flip in (False, True)[:2 if window else 1]:
+        def edit(pool, b):
+            for s, length in enumerate(b.lens):
+                for blk in range(-(-length // 16)):
+                    page = b.pages[s, blk * 16 // pool.page]
+                    pool.v_scale[page, :, blk % pool.b] *= F32(2.0 ** (30 * ((3 - blk) if flip else blk)))
+        check_attention(ctx, d, 1, 1, 32, [60, 37], [20, 5], G.F32, out_dtype, edit=edit, window=window)
+        check_attention(ctx, d, 2, 1, 32, [64], [64], G.F32, out_dtype, edit=edit, window=window)
+        check_attention(ctx, d, 1, 4, 16, [50, 64], [50, 40], G.F32, out_dtype, edit=edit, window=window)
