@@ -442,8 +442,11 @@ rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache 
  * scale >= 0 and finite.
  * Numerics: q' as whole numbers of 15 bits (out_dtype F32: 22 bits) of its
  * head's largest value against the 8-bit key codes in exact int32 products
- * on the matrix cores; softmax in f32; its weights rounded to binary16 (out_dtype
- * F32: two binary16 terms) against the value codes, f32 sums.  Fixed order for
+ * on the matrix cores; softmax in f32, its weights' sum in f32; the weights against
+ * the value codes as two binary16 terms, for many rows (calls of more than 32 query
+ * rows per kv head) to F16 and BF16 also as one, rounded by up to 2^-11; f32 sums.  A
+ * weight is held to 2^-34 of its row's largest, times the largest value scale that
+ * the row sees over its own block's.  Fixed order for
  * a batch: run-to-run bit-identical; a row's last bits depend on the batch.
  * Calls that split long sequences use a buffer allocated with the context
  * (as rce_qmm_sample_dev does for long rows): a recorded call stays valid, and

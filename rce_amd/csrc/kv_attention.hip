@@ -28,7 +28,9 @@
 //                 value codes as stored, 16 positions of a dimension in a
 //                 word.  P carries its block's value scale relative to the
 //                 largest that its row sees in the tile, times 2^14 (so that small weights stay
-//                 normal in binary16); HILO adds a second binary16 term.
+//                 normal in binary16), as two binary16 terms: one would round the
+//                 weights by up to 2^-11, as much as a binary16 result is rounded
+//                 itself, and saves 1 to 2 % (64 x 4096 ragged 81.5 : 79.9 us, 5 rows x 16 x 2000 19.5 : 18.8).
 //
 // What bounds it: the codes' way from HBM, where there are enough of them.  2 x 131072 ragged, 8
 // kv heads of 128, bf16: 340 MB in 70 us (4.9 TB/s, what a copy reaches) and 10 us
@@ -401,10 +403,9 @@ struct Shared {
     float m[WAVES][ROWS], l[WAVES][ROWS];
 };
 
-template <int D, bool HILO, bool LINE>
-__global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 192 ? 2 : 1) void k_kv_attention(Args A) {
+template <int D, int LIMBS, bool LINE>
+__global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1) void k_kv_attention(Args A) {
     constexpr int NQ = D / 64, NT = D / 16;
-    constexpr int LIMBS = HILO ? 3 : 2;
     __shared__ Shared<D> sh;
     int block = blockIdx.x;
     const Cut cut = cut_of<LINE>(A);
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
                 for (int e = 0; e < 4; e++) {
                     // |sum of a limb| <= 256 * 128 * 127: the two lower limbs join in int32
                     const float lo = (float)(c[LIMBS - 2][e] * 256 + c[LIMBS - 1][e]);
-                    if constexpr (HILO) x[4 * i + e] = (float)c[0][e] * 65536.0f + lo;
+                    if constexpr (LIMBS == 3) x[4 * i + e] = (float)c[0][e] * 65536.0f + lo;
                     else x[4 * i + e] = lo;
                 }
             }
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
                 const float p = masked && x[j] == -INFINITY ? 0.0f : e * pw;
                 const _Float16 hi = (_Float16)p;
                 ph[j >> 3][j & 7] = hi;
-                if constexpr (HILO) pl[j >> 3][j & 7] = (_Float16)(p - (float)hi);
+                pl[j >> 3][j & 7] = (_Float16)(p - (float)hi);
             }
             l = l * alpha + sum;
             const float back = sv_max * 0x1p-14f;
@@ -543,10 +544,8 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
                 f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], o, 0, 0, 0);
                 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], o, 0, 0, 0);
-                if constexpr (HILO) {
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], o, 0, 0, 0);
-                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], o, 0, 0, 0);
-                }
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], o, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[i][e] = __builtin_fmaf(acc[i][e], alpha, o[e] * back);
             }
@@ -610,6 +609,9 @@ __global__ __launch_bounds__(64 * WAVES, D * (HILO ? 3 : 2) <= 256 ? 3 : D <= 19
 // scale that the row has seen, and of the row's m.  m moves, and O and l are rescaled, only when a
 // score passes it by more than LAG (base 2): weights are then at most 2^LAG,
 // times UP in binary16 at most 2^15.
+// Results in 16 bits take one binary16 term per weight (HILO: two).  Its rounding, 2^-11 at most, adds
+// a third to the error of a binary16 result (normwise against 64 bits 2.7e-4, 2.1e-4 for the
+// result's own rounding; below 1 % for BF16); a second term costs a third of the time (3 x 4096 f16 565 : 770 us).
 // 3 prompts of 4096, 32 query and 8 kv heads of 128, f16: 355 GFLOP in 544 us, 30 % of the time of
 // the MFMAs, 0.65 PFLOP/s.  What bounds it: the vector unit (16 exponentials, their conversions and
 // the scores' of a lane per tile and row) and the reads of LDS, a quarter of them in conflict.
@@ -1048,10 +1050,10 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
                      (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
             in_line = A.line;
             const dim3 g = grid(A, u), b(64 * WAVES);
-            if (A.line && f32) hipLaunchKernelGGL((k_kv_attention<D, true, true>), g, b, 0, s, A);
-            else if (A.line) hipLaunchKernelGGL((k_kv_attention<D, false, true>), g, b, 0, s, A);
-            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, true, false>), g, b, 0, s, A);
-            else hipLaunchKernelGGL((k_kv_attention<D, false, false>), g, b, 0, s, A);
+            if (A.line && f32) hipLaunchKernelGGL((k_kv_attention<D, 3, true>), g, b, 0, s, A);
+            else if (A.line) hipLaunchKernelGGL((k_kv_attention<D, 2, true>), g, b, 0, s, A);
+            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, 3, false>), g, b, 0, s, A);
+            else hipLaunchKernelGGL((k_kv_attention<D, 2, false>), g, b, 0, s, A);
         };
         auto many = [&](int lo) {
             Args A{pool, rows, a, G, P_ROWS, lo, INT_MAX, target(MANY_PARTS, P_ROWS), P_MIN_CHUNK, 0, vec};

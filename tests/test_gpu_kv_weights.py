@@ -71,3 +71,26 @@ def test_values_of_unseen_blocks_cost_no_precision(ctx, d, window, out_dtype):
         check_attention(ctx, d, 1, 1, 32, [60, 37], [20, 5], G.F32, out_dtype, edit=edit, window=window)
         check_attention(ctx, d, 2, 1, 32, [64], [64], G.F32, out_dtype, edit=edit, window=window)
         check_attention(ctx, d, 1, 4, 16, [50, 64], [50, 40], G.F32, out_dtype, edit=edit, window=window)
+
+
+@pytest.mark.parametrize("out_dtype", [G.F16, G.BF16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+def test_single_tokens_to_16_bits_have_two_terms_per_weight(ctx, d, out_dtype):
+    """Queries that are exact in 15 bits and small scores, so that the bound of F32 results holds;
+    results near 0 (many of those over all dimensions) tell a weight's rounding to 2^-11 from one to 2^-21."""
+    rng = np.random.default_rng(d)
+    batch, n_pages = kc.make_batch(rng, [20, 17, 2500, 40], [1, 2, 1, 3], 32)
+    pool = kc.Pool(n_pages, 32, 2, d, rng)
+
+    def q_edit(x):
+        x[:] = np.rint(x * 30).clip(-127, 127)
+        x[:, ::d] = 127
+    a = Attn(ctx, pool, batch, 6, G.F16, out_dtype, scale=2.0 ** -10, q_edit=q_edit)
+    a.call()
+    ctx.synchronize()
+    rows = batch.n_rows
+    got = kc.widen(a.bits(), out_dtype).reshape(rows, 6, d).astype(np.float64)
+    want, bound = kc.attention(pool, batch, a.q, None, a.scale, 0, True)
+    a.free()
+    far = np.abs(got - want) - (bound + kc.out_eps(out_dtype) * (np.abs(want) + bound) + 2.0 ** -25)
+    assert far.max() <= 0, (far.max(), bound.max())
