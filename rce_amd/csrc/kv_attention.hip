@@ -67,6 +67,15 @@ constexpr int P_MIN_CHUNK = 4;  // of units of P_ROWS rows: 3 x 201 f32 in range
 constexpr int LINE_CHUNK = 24;  // tiles per block from which a block may serve several units
 constexpr int PAD = 4;          // a unit's prologue and epilogue, in the time of a tile
 constexpr int FEW = 32;       // query rows per kv head up to which a sequence is served in units of ROWS
+// A call of more than FEW rows per sequence on average has a part in units of P_ROWS.  So has one of LONG rows
+// or more besides a token per sequence, which may be one prompt's, where that prompt in units of ROWS could
+// come to LONG_TILES tiles for each of TARGET blocks by the table's span.  All in units of ROWS : with the
+// part (us, f16, heads of 128), single tokens beside a prompt of that many rows, and those tiles:
+//   1020 rows after 1744, 32: 82 : 88;  1196 new, 5 (heads of 64): 12 : 25;  1996 new, 31: 68 : 94;  3992 new, 8: 30 : 53;
+//   1899 new, 59: 171 : 176;  1999 new, 62: 139 : 137;  1996 after 1500, 62: 129 : 119;  1792 after 3647, 112: 159 : 137;
+//   1996 after 7692, 250: 287 : 194;  3992 after 3000, 500: 350 : 206;  6999 new, 751: 811 : 285.
+// LONG: 16 sequences of 5 drafts in long tables are spared the launch (4 us of 27).
+constexpr int LONG = 1536, LONG_TILES = 48;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -1033,7 +1042,8 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         bool in_line = false;
         // units of the part at most, and its grid
         auto units = [&](const Args &A, int hi) {
-            const size_t u = std::min(x, x / A.rows + (size_t)rows.n_seqs);
+            const size_t n = std::min((size_t)rows.n_seqs, x / std::max(A.lo_x, 1));  // sequences of the part
+            const size_t u = std::min(x, x / A.rows + n);
             return hi == INT_MAX ? u : std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
         };
         auto grid = [&](Args &A, size_t u) {
@@ -1062,7 +1072,10 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
             if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), g, b, 0, s, A, rows.pages);
             else hipLaunchKernelGGL((k_kv_prompt<D, false>), g, b, 0, s, A, rows.pages);
         };
-        if (x > (size_t)FEW * rows.n_seqs) {
+        const size_t tokens = (size_t)G * rows.n_seqs, more = x > tokens ? x - tokens : 0;
+        const bool prompt = more >= (size_t)LONG &&
+                            (double)more / ROWS * (rows.cap / TILE) * pool.heads >= (double)LONG_TILES * TARGET;
+        if (x > (size_t)FEW * rows.n_seqs || prompt) {
             const bool one = rows.n_seqs == 1 && rows.cap <= ONE_TABLE * TILE;
             many(one ? 0 : FEW + 1);
             if (!one) few(FEW);

@@ -1,6 +1,6 @@
 """Attention where blocks serve the ends and beginnings of several sequences, at
-every head size; pools whose
-codes pass 32-bit offsets."""
+every head size; pools whose codes pass 32-bit offsets; batches of single
+tokens beside a long prompt."""
 import numpy as np
 import pytest
 
@@ -8,7 +8,7 @@ import kv_case as kc
 import rce_amd
 from kv_case import F32
 from rce_amd import GgufDtype as G
-from test_gpu_kv import Attn, fused
+from test_gpu_kv import Attn, check_attention, fused
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,17 @@ def test_codes_past_32_bit_offsets(ctx):
     for z in (x, pages, table, *keep, *out):
         z.free()
     cache.free()
+
+
+@pytest.mark.parametrize("out_dtype", [G.F32, G.F16])
+@pytest.mark.parametrize("per,new,page", [(1, 1600, 4096), (4, 449, 64), (4, 449, 2048), (2, 900, 4096)])
+def test_single_tokens_beside_a_long_prompt(ctx, per, new, page, out_dtype):
+    """The prompt among so many single tokens that a sequence has few rows on average, in tables of
+    a page each, short and long; empty sequences and rows behind the last one."""
+    n, heads = 90, 8
+    rng = np.random.default_rng(new)
+    lens = [int(x) for x in rng.integers(1, 300, n)]
+    news = [1] * n
+    lens[n // 2], news[n // 2] = new + 60, new
+    lens[5] = news[5] = news[9] = 0
+    check_attention(ctx, 64, heads, per, page, lens, news, G.F16, out_dtype, rope=64, window=200, n_rows=sum(news) + 7)
