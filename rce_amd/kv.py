@@ -62,6 +62,10 @@ class KvCache:
         return b.value, n.value
 
     def free(self) -> None:
+        """Free a pool that ``allocate`` made: later calls with it are refused
+        (a null cache buffer)."""
+        if self.buffers:
+            self.raw = _pack(_CACHE, 0, 0, 0, 0, *_CACHE.unpack(self.raw)[4:])
         for b in self.buffers:
             b.free()
         self.buffers = ()
