@@ -152,7 +152,7 @@ rce_qmm_status rce_qmm_rope_table(float freq_base, size_t dim, size_t n_pos, flo
         if (!cs && dim && n_pos) return fail(RCE_QMM_NULL_ARGUMENT, "null table");
         if (dim % 2 || dim > 65536 || n_pos > (size_t)INT_MAX)
             return fail(RCE_QMM_BAD_SHAPE, "dim must be even and at most 65536, n_pos below 2^31");
-        if (!(freq_base > 0.0f)) return fail(RCE_QMM_BAD_SHAPE, "freq_base must be positive");
+        if (!(freq_base > 0.0f) || !std::isfinite(freq_base)) return fail(RCE_QMM_BAD_SHAPE, "freq_base must be positive and finite");
         fill_rope_table(freq_base, dim, n_pos, cs);
         return RCE_QMM_OK;
     });

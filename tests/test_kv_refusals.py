@@ -1,8 +1,9 @@
-"""More of what the kv entry points refuse, on the host: a pool that was freed."""
+"""More of what the kv entry points refuse, on the host: a pool that was freed,
+rotation bases without angles."""
 import pytest
 
 import rce_amd
-from test_kv_args import NULL, append, attend, batch, cache, read, refused
+from test_kv_args import BAD, NULL, append, attend, batch, cache, read, refused
 
 
 class Buffer:
@@ -28,3 +29,8 @@ def test_the_callers_own_pool_stays_its_own():
     raw = c.raw
     c.free()
     assert c.raw == raw
+
+
+def test_rotation_bases_without_angles():
+    for base in (float("inf"), float("nan"), 0.0, -1.0):
+        refused(BAD, rce_amd.Rope.table, base, 8, 5)
