@@ -369,7 +369,7 @@ rce_qmm_status rce_qmm_llama_check(rce_qmm_llama *m);
  *   v code of dimension d  v[(((p * n_kv_heads + h) * B + b) * d_head + d) * 16 + i]
  *   scales                 k_scale, v_scale[(p * n_kv_heads + h) * B + b]
  * d_head: 64, 128, 192 or 256; fewer than 2^32 blocks.  k and v 16-byte
- * aligned, the scales 4. */
+ * aligned, the scales 4.  Scales are not negative (an append writes none that is). */
 typedef struct rce_qmm_kv_cache {
     int8_t *k, *v;
     float *k_scale, *v_scale;
@@ -416,8 +416,12 @@ rce_qmm_status rce_qmm_rope_table(float freq_base, size_t dim, size_t n_pos, flo
  * grew, the codes of its earlier slots become rint(q * (old scale / scale)).
  * Slots behind the new rows keep their bytes.  A block that gets an infinite
  * or NaN value has that scale and codes 0 and reads as NaN until its first
- * slot is written again.  No block may be written for two sequences in one
- * call.  n_rows at most 2^27. */
+ * slot is written again.  A scale never falls before that either: rows that a
+ * program takes back (rejected drafts) and writes again later leave the rows in
+ * front of them in their block at the scale, and the codes at the rounding, that the
+ * taken-back values made; to be rid of it the block's rows are appended again from its
+ * first slot.  No block may be written twice in one call, for two sequences or
+ * through a page that a table names twice.  n_rows at most 2^27. */
 rce_qmm_status rce_qmm_kv_append_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
                                      const rce_qmm_kv_batch *batch, const void *k_dev, size_t k_stride,
                                      const void *v_dev, size_t v_stride, uint32_t dtype, const rce_qmm_rope *rope,
@@ -438,19 +442,20 @@ rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache 
  * (window 0: from 0), q' the rotated q (rope NULL: q).  A row that sees no
  * key, or is left out, gives zeros; rows behind row_offsets[n_seqs] keep their
  * bytes.  q_dev [n_rows][n_q_heads * d_head] with q_stride values from row to
- * row, q_dtype F32, F16 or BF16; out_dev likewise with out_stride, out_dtype.
- * scale >= 0 and finite.
+ * row, q_dtype F32, F16 or BF16; out_dev likewise with out_stride, out_dtype,
+ * apart from q_dev.  scale >= 0 and finite; max_pages at least 1.
  * Numerics: q' as whole numbers of 15 bits (out_dtype F32: 22 bits) of its
- * head's largest value against the 8-bit key codes in exact int32 products
+ * head's largest value (0 where that is below 2^-100) against the 8-bit key codes in exact int32 products
  * on the matrix cores; softmax in f32, its weights' sum in f32; the weights against
  * the value codes as two binary16 terms, for many rows (calls of more than 32 query
  * rows per kv head) to F16 and BF16 also as one, rounded by up to 2^-11; f32 sums.  A
  * weight is held to 2^-34 of its row's largest, times the largest value scale that
- * the row sees over its own block's.  Fixed order for
- * a batch: run-to-run bit-identical; a row's last bits depend on the batch.
- * Calls that split long sequences use a buffer allocated with the context
- * (as rce_qmm_sample_dev does for long rows): a recorded call stays valid, and
- * calls or graphs that may run at the same time need a context each. */
+ * the row sees (at least 2^-110) over its own block's.  Scores have to fit binary32.
+ * Fixed order for a batch: run-to-run bit-identical; a row's last bits depend on the
+ * batch.  Calls that split long sequences use a buffer of 52 MiB that every context
+ * holds from its creation (as rce_qmm_sample_dev does for long rows): a recorded
+ * call stays valid, and calls or graphs that may run at the same time need a
+ * context each. */
 rce_qmm_status rce_qmm_kv_attention_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
                                         const rce_qmm_kv_batch *batch, const void *q_dev, uint32_t q_dtype,
                                         size_t q_stride, size_t n_q_heads, const rce_qmm_rope *rope, float scale,

@@ -30,13 +30,13 @@
 //                 largest that its row sees in the tile, times 2^14 (so that small weights stay
 //                 normal in binary16), as two binary16 terms: one would round the
 //                 weights by up to 2^-11, as much as a binary16 result is rounded
-//                 itself, and saves 1 to 2 % (64 x 4096 ragged 81.5 : 79.9 us, 5 rows x 16 x 2000 19.5 : 18.8).
+//                 itself, and saves 1 to 3 % (64 x 4096 ragged 81.5 : 79.9 us, 5 rows x 16 x 2000 19.5 : 18.8).
 //
 // What bounds it: the codes' way from HBM, where there are enough of them.  2 x 131072 ragged, 8
-// kv heads of 128, bf16: 340 MB in 70 us (4.9 TB/s, what a copy reaches) and 10 us
-// of the join; 64 x 4096 ragged: 348 MB in 81 + 6 us.  Below some 50 MB a block's own
+// kv heads of 128, bf16: 340 MB in 70 us (4.9 TB/s, what a copy reaches) and 11 us
+// of the join; 64 x 4096 ragged: 348 MB in 82 + 6 us.  Below some 50 MB a block's own
 // way from its arguments to its result: 5 rows x 16 x 2000, 41 MB in 19 + 5 us, one
-// row x 700 in 11 us.
+// row x 700 in 11 us (a table of more than SPLIT_FROM tiles: in two ranges and a join, whole calls 10 : 13).
 #include "kv_cache.h"
 
 #include <algorithm>
@@ -621,10 +621,11 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
 // Results in 16 bits take one binary16 term per weight (HILO: two).  Its rounding, 2^-11 at most, adds
 // a third to the error of a binary16 result (normwise against 64 bits 2.7e-4, 2.1e-4 for the
 // result's own rounding; below 1 % for BF16); a second term costs a third of the time (3 x 4096 f16 565 : 770 us).
-// 3 prompts of 4096, 32 query and 8 kv heads of 128, f16: 355 GFLOP in 544 us, 30 % of the time of
-// the MFMAs, 0.65 PFLOP/s.  What bounds it: the vector unit (16 exponentials, their conversions and
+// 3 prompts of 4096, 32 query and 8 kv heads of 128, f16: 355 GFLOP in 500 us for the whole call, 0.71
+// PFLOP/s, the MFMAs busy 30 % of the time.  What bounds it: the vector unit (16 exponentials, their conversions and
 // the scores' of a lane per tile and row) and the reads of LDS, a quarter of them in conflict.
-// 3 x 201 rows f32, 16 kv heads of 64, a window of 512: 21 us and 8 of the join.
+// 3 x 201 rows f32, 16 kv heads of 64, a window of 512: 21 us and 8 of the join; no unit is busy there
+// (VALU a third of the time, MFMAs and LDS 3 %): a block's chain of loads and barriers.
 // 16 rows and not 32 per wave: MFMAs, exponentials and the vector unit overlap only across
 // waves, and 16 rows fit 128 registers (four waves per SIMD; at the price of twice
 // the LDS reads per product).
@@ -1022,7 +1023,7 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A0, Args A1) {
 // there is at most one block more per head: heads are at most target / 20 there.
 constexpr int slots(int target) { return 2 * target + target / 8; }
 // Partial results of units of ROWS and of P_ROWS rows.  Room for TARGET blocks of few rows at every
-// head size, for 127 (256 dimensions) to 500 of many.
+// head size, for 126 (256 dimensions) to 496 of many.
 constexpr size_t FEW_PARTS = (size_t)18 << 20, MANY_PARTS = (size_t)34 << 20;
 size_t kv_attention_parts_bytes() { return FEW_PARTS + MANY_PARTS; }
 

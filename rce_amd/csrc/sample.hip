@@ -532,8 +532,9 @@ __device__ __forceinline__ void bind_row(Row<T, LDS> &row, const SampleRows &R, 
 //   128                 140   87   64   52    32   43          180  187
 //   200                 147  130   71   82    38   53          186  195
 //   1 x 30000 (in LDS)   34   25   17   15    12   20           49   61
-// The filters' values are not known on the host: rows that fit LDS and more than 128
-// of them stay with a block per row.
+// The filters' values are not known on the host, so rows that fit LDS and more than 128 of
+// them stay with a block per row, also in the calls without a top_k array (which the
+// host does see) that the table has faster over several blocks.
 constexpr int MAX_SLICES = 64;
 struct SplitRow {
     u64 hist[BINS], list[NT], runs[RUNS];
