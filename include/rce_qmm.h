@@ -445,12 +445,13 @@ rce_qmm_status rce_qmm_kv_read_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache 
  * row, q_dtype F32, F16 or BF16; out_dev likewise with out_stride, out_dtype,
  * apart from q_dev.  scale >= 0 and finite; max_pages at least 1.
  * Numerics: q' as whole numbers of 15 bits (out_dtype F32: 22 bits) of its
- * head's largest value (0 where that is below 2^-100) against the 8-bit key codes in exact int32 products
- * on the matrix cores; softmax in f32, its weights' sum in f32; the weights against
- * the value codes as two binary16 terms, for many rows (calls of more than 32 query
- * rows per kv head) to F16 and BF16 also as one, rounded by up to 2^-11; f32 sums.  A
- * weight is held to 2^-34 of its row's largest, times the largest value scale that
- * the row sees (at least 2^-110) over its own block's.  Scores have to fit binary32.
+ * head's largest value (0 where that is below 2^-100) against the 8-bit key codes
+ * in exact int32 products on the matrix cores; scores, which have to fit binary32,
+ * softmax and the sum of its weights in f32; the weights against the value codes as
+ * two binary16 terms, for many rows (calls of more than 32 query rows per kv head)
+ * to F16 and BF16 also as one, rounded by up to 2^-11; f32 sums.  A weight is held
+ * to 2^-34 of its row's largest, times the largest value scale that the row sees
+ * (at least 2^-110) over its own block's.
  * Fixed order for a batch: run-to-run bit-identical; a row's last bits depend on the
  * batch.  Calls that split long sequences use a buffer of 52 MiB that every context
  * holds from its creation (as rce_qmm_sample_dev does for long rows): a recorded
