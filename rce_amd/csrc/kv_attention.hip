@@ -71,7 +71,8 @@ constexpr int FEW = 32;       // query rows per kv head up to which a sequence i
 // or more besides a token per sequence, which may be one prompt's, where that prompt in units of ROWS could
 // come to LONG_TILES tiles for each of TARGET blocks by the table's span.  All in units of ROWS : with the
 // part (us, f16, heads of 128), single tokens beside a prompt of that many rows, and those tiles:
-//   1020 rows after 1744, 32: 82 : 88;  1196 new, 5 (heads of 64): 12 : 25;  1996 new, 31: 68 : 94;  3992 new, 8: 30 : 53;
+//   1020 rows after 1744, 32: 82 : 88;  1196 new, 36: 86 : 78, 5 (heads of 64): 12 : 25;  1996 new, 31: 68 : 94;
+//   3992 new, 8: 30 : 53;
 //   1899 new, 59: 171 : 176;  1999 new, 62: 139 : 137;  1996 after 1500, 62: 129 : 119;  1792 after 3647, 112: 159 : 137;
 //   1996 after 7692, 250: 287 : 194;  3992 after 3000, 500: 350 : 206;  6999 new, 751: 811 : 285.
 // LONG: 16 sequences of 5 drafts in long tables are spared the launch (4 us of 27).
