@@ -251,6 +251,32 @@ rce_qmm_status rce_qmm_mm_batched_dev_noalloc(rce_qmm_context *ctx, const void *
 rce_qmm_status rce_qmm_moe_router(const float *logits, size_t n_tokens, size_t n_expert,
                                   size_t top_k, int normalize, int32_t *ids, float *weights);
 
+/* Scores of rce_qmm_moe_route_dev. */
+enum { RCE_QMM_SCORES_SOFTMAX = 0, RCE_QMM_SCORES_SIGMOID = 1 };
+
+typedef struct rce_qmm_moe_routing {
+    int scoring;         /* RCE_QMM_SCORES_* of a token's logits */
+    const float *bias;   /* device, n_expert values that move the choice, not the weights; NULL: none */
+    size_t top_k;        /* experts of a token, at most 64 */
+    size_t n_group;      /* groups of n_expert / n_group consecutive experts, at most 64; 0, 1: none */
+    size_t topk_group;   /* groups of a token that experts are chosen from */
+    size_t group_top;    /* a group counts by the sum of so many of its highest scores (bias included): 1 or 2 */
+    int normalize;       /* weights divided by their sum */
+    float scale;         /* and times this */
+} rce_qmm_moe_routing;
+
+/* rce_qmm_moe_router on the device, the ids and weights that rce_qmm_moe_ffn_dev and rce_qmm_moe_swiglu_dev
+ * take, without a host round trip: logits_dev [n_tokens][n_expert] (row_stride values from row to row; F32,
+ * F16 or BF16) -> ids_dev, weights_dev [n_tokens][top_k], the highest score + bias first, the lower id first
+ * among equals (of groups too).  Scores softmax(l) over all experts, or 1 / (1 + e^-l); weight scale * score, or with
+ * `normalize` scale * score / (sum of the chosen ones' scores).  An expert whose logit is NaN or -inf, or whose bias is NaN or
+ * -inf, is chosen only where its groups have no other left, the lower id first, with weight 0: ids are always experts.
+ * Without a bias experts are compared by their logits, with one by scores in 64 bits; weights are formed
+ * in 64 bits and rounded once.  n_expert at most 1024, n_tokens 2^24. */
+rce_qmm_status rce_qmm_moe_route_dev(rce_qmm_context *ctx, const void *logits_dev, uint32_t dtype, size_t n_tokens,
+                                     size_t n_expert, size_t row_stride, const rce_qmm_moe_routing *how,
+                                     int32_t *ids_dev, float *weights_dev, void *stream);
+
 /* Grouped-expert FFN on device buffers: for every token t and decision j,
  * e = ids[t, j]: h = silu(W1[e] x_t), y_j = W2[e] h, and
  * out_t = sum_j weights[t, j] * y_j in decision order from +0.0
@@ -406,6 +432,27 @@ typedef struct rce_qmm_rope {
  * library's logf / expf / cosf / sinf in the reference's order. */
 rce_qmm_status rce_qmm_rope_table(float freq_base, size_t dim, size_t n_pos, float *cs);
 
+/* How a table is scaled for contexts longer than the model was trained on.
+ * Pair i turns by f_i = freq_base^(-2 i / dim) / divisors[i] per position
+ * (divisors: host, dim / 2 values, NULL: none; a file's rope_freqs), divided
+ * by `factor` (1: not scaled).  With orig_context not 0 the fast pairs keep f_i:
+ * with pair(t) = dim ln(orig_context / (2 pi t)) / (2 ln freq_base), the pair that turns t
+ * times over the original context, low = max(0, floor(pair(beta_fast))), high = min(dim - 1,
+ * ceil(pair(beta_slow))) and r = clamp((i - low) / max(0.001, high - low), 0, 1), pair i turns by
+ * f_i (1 - r) + f_i / factor r.  Every (cos, sin) is times `magnitude` (1: not
+ * scaled). */
+typedef struct rce_qmm_rope_scaling {
+    float factor, magnitude;
+    const float *divisors;
+    size_t orig_context;
+    float beta_fast, beta_slow;
+} rce_qmm_rope_scaling;
+
+/* A rotation table on the host with such a scaling: angles, cosines and sines
+ * in 64 bits, rounded once. */
+rce_qmm_status rce_qmm_rope_table_scaled(float freq_base, size_t dim, size_t n_pos, const rce_qmm_rope_scaling *how,
+                                         float *cs);
+
 /* Append n_rows rows of keys and values to their sequences' pages; the keys
  * are rotated on the way (rope NULL: as they are).  k_dev [n_rows][n_kv_heads *
  * d_head] with k_stride values from row to row (v likewise; slices of one
@@ -462,6 +509,101 @@ rce_qmm_status rce_qmm_kv_attention_dev(rce_qmm_context *ctx, const rce_qmm_kv_c
                                         size_t q_stride, size_t n_q_heads, const rce_qmm_rope *rope, float scale,
                                         size_t window, void *out_dev, uint32_t out_dtype, size_t out_stride,
                                         void *stream);
+
+/* rce_qmm_kv_attention_dev with a sliding window and `sinks` first positions
+ * that every row sees whatever the window: the keys of a row at position p are
+ * j = 0 .. min(sinks, p + 1) - 1 and max(0, p - window + 1) .. p, each once.
+ * sinks 0, and window 0, are rce_qmm_kv_attention_dev, bit for bit.  Pages that lie
+ * wholly between may be freed (rce_qmm_kv_release_dev); what their entries name
+ * changes nothing.  Keys and queries are rotated by their positions in the
+ * sequence. */
+rce_qmm_status rce_qmm_kv_attention_sinks_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                              const rce_qmm_kv_batch *batch, const void *q_dev, uint32_t q_dtype,
+                                              size_t q_stride, size_t n_q_heads, const rce_qmm_rope *rope,
+                                              float scale, size_t window, size_t sinks, void *out_dev,
+                                              uint32_t out_dtype, size_t out_stride, void *stream);
+
+/* Query or key heads of a call: row r's head h is the d_head values from in +
+ * r * in_stride + h * d_head (strides in values), its result likewise in out.
+ * weight: d_head f32 values (device; NULL: ones). */
+typedef struct rce_qmm_heads {
+    const void *in;
+    size_t in_stride;
+    void *out;
+    size_t out_stride;
+    const float *weight;
+    size_t n_heads;
+} rce_qmm_heads;
+
+/* Norms of query and key heads and their rotation in one pass, in front of
+ * rce_qmm_kv_append_dev and rce_qmm_kv_attention_dev without a table of their own: every
+ * head x becomes x / sqrt(mean x^2 + eps) * weight (eps below 0: no norm, no weight), its first
+ * rope->dim values then turn by the row's position (rope NULL: not), pairs (i, i + dim / 2) or,
+ * `interleaved` not 0, (2 i, 2 i + 1); f32, one rounding to out_dtype.  The sum of
+ * squares has to fit binary32.
+ * q, k: either may be NULL or have no heads; d_head even, 2 to 1024, any other
+ * alignment than that of the values; in_dtype and out_dtype F32, F16 or BF16.  out may be in
+ * (one type size, one stride); other overlaps are not allowed.  Of the batch only
+ * row_offsets, seq_lens, n_seqs and n_rows are read.  Rows of no sequence, at negative
+ * positions or (with a table) at positions from rope->n_pos on are left as they were. */
+rce_qmm_status rce_qmm_qk_norm_rope_dev(rce_qmm_context *ctx, const rce_qmm_kv_batch *batch, const rce_qmm_heads *q,
+                                        const rce_qmm_heads *k, size_t d_head, uint32_t in_dtype, uint32_t out_dtype,
+                                        float eps, const rce_qmm_rope *rope, int interleaved, void *stream);
+
+/* ---- pages of the KV cache ------------------------------------------------- */
+
+/* Sequences' page tables (device; the `pages` of a batch) for the calls that
+ * change them.  Entries outside the pool name no page; these calls write -1 for that.  They
+ * keep refs[n_pages] (device, int32, zero at first): refs[p] is the number of entries, in all
+ * of the program's tables, that name page p; 0 where it is free.  Entries behind a
+ * sequence's last page must name none.  All are asynchronous and read nothing back. */
+typedef struct rce_qmm_kv_table {
+    int32_t *pages;
+    size_t n_seqs, max_pages;
+} rce_qmm_kv_table;
+
+/* Pages src_dev[i] of `from` to pages dst_dev[i] of `to` (codes and scales), i < n: two pools of one
+ * page shape, or one pool and itself.  A pair with an id outside its pool is left out.  No page may be the
+ * destination of two pairs, or of one and the source of another. */
+rce_qmm_status rce_qmm_kv_copy_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *from, const rce_qmm_kv_cache *to,
+                                   const int32_t *src_dev, const int32_t *dst_dev, size_t n, void *stream);
+
+/* Fork: sequence i of `to` gets the table of sequence parents_dev[i] of `from` (parents of `to`'s n_seqs; where
+ * `to` has more entries they are -1, where fewer the rest is dropped), and the pages' counts grow.
+ * parents outside `from` leave their sequence as it was.  What `to`'s entries named before is not
+ * released by this.  to may be from, for sequences none of whose parents is written. */
+rce_qmm_status rce_qmm_kv_fork_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache, const rce_qmm_kv_table *from,
+                                   const rce_qmm_kv_table *to, const int32_t *parents_dev, int32_t *refs_dev,
+                                   void *stream);
+
+/* Release: the pages that lie wholly in positions from_dev[s] .. to_dev[s] - 1 of their sequence (NULL: from
+ * 0, to the table's end) lose a count, their entries become -1.  What ends: all of a sequence; what a window
+ * has left behind: (sinks, length - window + 1); rejected drafts: (length, NULL). */
+rce_qmm_status rce_qmm_kv_release_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                      const rce_qmm_kv_table *table, const int32_t *from_dev, const int32_t *to_dev,
+                                      int32_t *refs_dev, void *stream);
+
+/* Reserve, in front of an append of the same batch (whose `pages` this writes): every page that the batch's rows
+ * touch becomes one of their sequence's own.  A position without a page gets a free one, the lowest first,
+ * in the order of sequences and positions.  A page that other entries name too (count above 1) is left for a
+ * free one, into which the blocks of 16 positions are copied that start in front of the sequence's first row of the
+ * batch; where all that name a page would leave it, the first of them keeps it.  missing_dev[s]
+ * (n_seqs counts; may be NULL): pages that the pool had none left for.  Their entries become -1: their rows are
+ * left out of the calls that follow, and where a shared page was to be left the
+ * sequence has lost what stood there. */
+rce_qmm_status rce_qmm_kv_reserve_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                      const rce_qmm_kv_batch *batch, int32_t *refs_dev, int32_t *missing_dev,
+                                      void *stream);
+
+/* Compact: of the n used pages (count not 0) those behind page n - 1 move, in order, to the free pages below
+ * n; table and counts follow.  new_ids_dev[p] (n_pages values): where page p is now, -1 where it was free: for the program's
+ * other tables.  n_used_dev (may be NULL): n.  n_pages at most 2^23.  This and
+ * rce_qmm_kv_reserve_dev plan in the context's buffer (see rce_qmm_kv_attention_dev). */
+rce_qmm_status rce_qmm_kv_compact_dev(rce_qmm_context *ctx, const rce_qmm_kv_cache *cache,
+                                      const rce_qmm_kv_table *table, int32_t *refs_dev, int32_t *new_ids_dev,
+                                      int32_t *n_used_dev, void *stream);
+
+/* ---- sampling ------------------------------------------------------------------ */
 
 /* How the rows of rce_qmm_sample_dev are sampled: device arrays of one value
  * per row; NULL turns a filter off (temperature: 1). */

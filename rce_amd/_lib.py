@@ -35,6 +35,7 @@ SIGNATURES = {
     "rce_qmm_mm_batched_dev": (STATUS, [P, P, U32, S, P, P, I, P]),
     "rce_qmm_mm_batched_dev_noalloc": (STATUS, [P, P, U32, S, P, P, I, P]),
     "rce_qmm_moe_router": (STATUS, [P, S, S, S, I, P, P]),
+    "rce_qmm_moe_route_dev": (STATUS, [P, P, U32, S, S, S, P, P, P, P]),
     "rce_qmm_moe_ffn_dev": (STATUS, [P, P, P, S, P, S, P, P, S, P, I, P]),
     "rce_qmm_moe_swiglu_dev": (STATUS, [P, P, P, P, S, P, S, P, P, S, P, I, P]),
     "rce_qmm_llama_create": (STATUS, [P, P, P, P, P, P, I, P]),
@@ -57,9 +58,17 @@ SIGNATURES = {
     "rce_qmm_gguf_read_f32": (STATUS, [P, ctypes.c_char_p, P, S]),
     "rce_qmm_kv_sizes": (STATUS, [P, P, P]),
     "rce_qmm_rope_table": (STATUS, [F, S, S, P]),
+    "rce_qmm_rope_table_scaled": (STATUS, [F, S, S, P, P]),
     "rce_qmm_kv_append_dev": (STATUS, [P, P, P, P, S, P, S, U32, P, P]),
     "rce_qmm_kv_read_dev": (STATUS, [P, P, P, P, P, U32, P]),
     "rce_qmm_kv_attention_dev": (STATUS, [P, P, P, P, U32, S, S, P, F, S, P, U32, S, P]),
+    "rce_qmm_kv_attention_sinks_dev": (STATUS, [P, P, P, P, U32, S, S, P, F, S, S, P, U32, S, P]),
+    "rce_qmm_qk_norm_rope_dev": (STATUS, [P, P, P, P, S, U32, U32, F, P, I, P]),
+    "rce_qmm_kv_copy_dev": (STATUS, [P, P, P, P, P, S, P]),
+    "rce_qmm_kv_fork_dev": (STATUS, [P, P, P, P, P, P, P]),
+    "rce_qmm_kv_release_dev": (STATUS, [P, P, P, P, P, P, P]),
+    "rce_qmm_kv_reserve_dev": (STATUS, [P, P, P, P, P, P]),
+    "rce_qmm_kv_compact_dev": (STATUS, [P, P, P, P, P, P, P]),
     "rce_qmm_sample_dev": (STATUS, [P, P, U32, S, S, S, P, P, P, P]),
     "rce_qmm_dtype_for_qmm_id": (U32, [S]),
     "rce_qmm_hip_cost_prior": (None, [P, P, P]),

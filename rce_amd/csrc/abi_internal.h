@@ -71,9 +71,9 @@ struct rce_qmm_context {
     // needs, allocated with the context and never moved, so a call recorded
     // into a graph stays valid whatever calls follow it.
     rce_qmm_abi::Scratch parts;
-    // Partial results of attention's split key ranges, and of rows that sampling splits: the larger of
-    // kv_attention_parts_bytes() and sample_split_bytes(), allocated
-    // as parts.
+    // Partial results of attention's split key ranges, rows that sampling splits, and what reserving and
+    // compacting pages plan: the largest of kv_attention_parts_bytes(), sample_split_bytes() and kv_pages_bytes(),
+    // allocated as parts.
     rce_qmm_abi::Scratch kv_parts;
     rce_qmm_abi::Scratch act_q;  // several tokens' Q8 activations, quantized once per launch
     // grouped experts: grouping metadata, expert tables, stage buffers

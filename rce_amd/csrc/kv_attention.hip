@@ -93,19 +93,55 @@ struct Args {
     int vec;        // query rows (1) and rotation table (2) can be read, output rows (4) written 16 bytes at a time
 };
 
-// The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one.
+// The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one,
+// numbers t0 .. t0 + tiles - 1.
+//
+// Sinks: the tiles of the first positions stand in front of the window's.  Tile number t from `own` on is the tile of
+// positions 64 t .., a number below it is a tile from the sequence's beginning (0 for t0), as many as the
+// sinks reach into and the window does not.
 struct Span {
-    int units, t0, tiles;
+    int units, t0, tiles, own;
 };
+template <bool SINKS>
 __device__ __forceinline__ Span span_of(const Args &A, const KvSeq &q) {
     Span s;
     const int x = (q.r1 - q.r0) * A.G;
     s.units = x >= A.lo_x && x <= A.hi_x ? (x + A.rows - 1) / A.rows : 0;
     const int lo = max(0, q.lo() - (A.a.window - 1));
-    s.t0 = lo / TILE;
+    s.own = lo / TILE;
+    s.t0 = SINKS ? s.own - min(s.own, (A.a.sinks + TILE - 1) / TILE) : s.own;
     s.tiles = q.hi(A.B) > q.lo() ? (q.hi(A.B) + TILE - 1) / TILE - s.t0 : 0;
     return s;
 }
+
+// The tiles that a unit visits of its range [w_lo, w_hi) of tile numbers: those that sinks reach into, then the window's, numbers
+// `lo` .. `hi` - 1.  Without sinks the numbers are the tiles.
+template <bool SINKS>
+struct Visits {
+    int lo, hi;
+    int n_front, front, back, own, t0;  // SINKS: visit i < n_front is number front + i, the others back + i
+    __device__ Visits(const Args &A, const Span &p, int w_lo, int w_hi, int u_lo, int u_hi) {
+        if constexpr (SINKS) {
+            own = p.own;
+            t0 = p.t0;
+            const int end = min(w_hi, u_hi), reach = min(end, max(own, (A.a.sinks + TILE - 1) / TILE));
+            front = w_lo;
+            n_front = max(0, reach - w_lo);
+            const int from = max(max(w_lo, reach), u_lo);
+            back = from - n_front;
+            lo = 0;
+            hi = n_front + max(0, end - from);
+        } else {
+            lo = max(u_lo, w_lo);
+            hi = min(u_hi, w_hi);
+        }
+    }
+    __device__ __forceinline__ int tile(int i) const {
+        if constexpr (!SINKS) return i;
+        const int t = i + (i < n_front ? front : back);
+        return t < own ? t - t0 : t;
+    }
+};
 // The cells of a unit in the line (below): its prologue's, then one per tile, one if it has none.
 __device__ __forceinline__ int line_cells(const Span &p) { return PAD + max(1, p.tiles); }
 
@@ -114,12 +150,12 @@ struct Cut {
     int chunk;
     bool line;
 };
-template <bool LINE>
+template <bool LINE, bool SINKS>
 __device__ __forceinline__ Cut cut_of(const Args &A) {
     const int lane = threadIdx.x & 63;
     float tiles = 0.0f, units = 0.0f;  // only sizes: their rounding moves no result
     for (int s = lane; s < A.B.n_seqs; s += 64) {
-        const Span p = span_of(A, kv_seq(A.B, s));
+        const Span p = span_of<SINKS>(A, kv_seq(A.B, s));
         tiles += (float)p.units * (float)p.tiles;
         if (LINE) units += (float)line_cells(p) * (float)p.units;
     }
@@ -147,6 +183,7 @@ struct Work {
 };
 
 // Range `item` of the list (sequence, unit, range).
+template <bool SINKS>
 __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Work &w) {
     const int lane = threadIdx.x & 63;
     int run = 0, srun = 0;
@@ -154,7 +191,7 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
         const int s = base + lane;
         int c = 0, sc = 0;
         if (s < A.B.n_seqs) {
-            const Span p = span_of(A, kv_seq(A.B, s));
+            const Span p = span_of<SINKS>(A, kv_seq(A.B, s));
             const int n = ranges(p.tiles, chunk);
             c = p.units * n;
             sc = n > 1 ? c : 0;
@@ -166,7 +203,7 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
             const int at = item - run - __builtin_amdgcn_readlane(incl - c, l);
             w.seq = base + l;
             w.q = kv_seq(A.B, w.seq);
-            w.sp = span_of(A, w.q);
+            w.sp = span_of<SINKS>(A, w.q);
             const int n = ranges(w.sp.tiles, chunk), step = range_tiles(w.sp.tiles, n);
             const int u = at / n, range = at - u * n;
             w.unit = w.sp.units - 1 - u;  // the units with the most keys first
@@ -192,6 +229,7 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
 // 64 sequences of up to 4096: 100 -> 85 us.
 
 // The work at cell `pos` of the line, up to cell `end`; false: none is left.  n: the cells up to the next unit.
+template <bool SINKS>
 __device__ __forceinline__ bool find_in_line(const Args &A, int item, int pos, int end, Work &w, int &n) {
     const int lane = threadIdx.x & 63;
     int run = 0;
@@ -199,7 +237,7 @@ __device__ __forceinline__ bool find_in_line(const Args &A, int item, int pos, i
         const int s = base + lane;
         int c = 0;
         if (s < A.B.n_seqs) {
-            const Span p = span_of(A, kv_seq(A.B, s));
+            const Span p = span_of<SINKS>(A, kv_seq(A.B, s));
             c = p.units * line_cells(p);
         }
         const int incl = wave_scan(c), total = __builtin_amdgcn_readlane(incl, 63);
@@ -208,7 +246,7 @@ __device__ __forceinline__ bool find_in_line(const Args &A, int item, int pos, i
             const int at = pos - run - __builtin_amdgcn_readlane(incl - c, l);
             w.seq = base + l;
             w.q = kv_seq(A.B, w.seq);
-            w.sp = span_of(A, w.q);
+            w.sp = span_of<SINKS>(A, w.q);
             const int cells = line_cells(w.sp);
             w.unit = at / cells;
             const int from = at - w.unit * cells, to = min(cells, from + end - pos);
@@ -413,12 +451,12 @@ struct Shared {
     float m[WAVES][ROWS], l[WAVES][ROWS];
 };
 
-template <int D, int LIMBS, bool LINE>
+template <int D, int LIMBS, bool LINE, bool SINKS>
 __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1) void k_kv_attention(Args A) {
     constexpr int NQ = D / 64, NT = D / 16;
     __shared__ Shared<D> sh;
     int block = blockIdx.x;
-    const Cut cut = cut_of<LINE>(A);
+    const Cut cut = cut_of<LINE, SINKS>(A);
     // a line is at most `target` blocks and one more per head; past it the products below would pass 31 bits
     if (LINE && cut.line && block / A.P.heads > A.target) return;
     int line_at = cut.line ? block / A.P.heads * cut.chunk : 0;
@@ -432,7 +470,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
         const int item = block / A.P.heads, h = block % A.P.heads;
         Work w;
         int n_cells = 0;
-        if (LINE && cut.line ? !find_in_line(A, item, line_at, line_end, w, n_cells) : !find_work(A, item, cut.chunk, w)) return;
+        if (LINE && cut.line ? !find_in_line<SINKS>(A, item, line_at, line_end, w, n_cells) : !find_work<SINKS>(A, item, cut.chunk, w)) return;
         const KvSeq &q = w.q;
         const int G = A.G, first = q.first();
         const int x0 = w.unit * ROWS, n_x = min(ROWS, (q.r1 - q.r0) * G - x0);  // rows of the unit
@@ -449,9 +487,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
         const int u_tok0 = x0 / G, u_tok1 = (x0 + n_x - 1) / G;
         const int u_hi = min(A.B.cap - 1, first + u_tok1), u_first = first + u_tok0;
         const int all_lo = max(0, max(0, u_hi) - (A.a.window - 1)), all_hi = u_first;  // seen by every row (if all have positions)
-        int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-        t_lo = max(t_lo, w.t_lo);
-        t_hi = min(t_hi, w.t_hi);
+        const Visits<SINKS> visit(A, w.sp, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, u_hi < 0 ? 0 : u_hi / TILE + 1);
         const bool placed = u_first >= 0 && first + u_tok1 < A.B.cap;  // every row has a position
         const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
         const int bmask = (1 << A.P.lg_b) - 1;
@@ -460,7 +496,8 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
 #pragma unroll
         for (int i = 0; i < NT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
-        for (int t = t_lo + wave; t < t_hi; t += WAVES) {
+        for (int i_t = visit.lo + wave; i_t < visit.hi; i_t += WAVES) {
+            const int t = visit.tile(i_t);
             // the K block of this lane's operand rows, the block of its scores
             const int max_block = A.B.cap / KV_BLOCK - 1;
             const int kb = min(4 * t + (n >> 2), max_block), vb = min(4 * t + g, max_block);
@@ -501,14 +538,14 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
                 }
             }
             const float f = sk * qs;
-            const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;  // the same in all lanes
+            const bool full = placed && (TILE * t >= all_lo || (SINKS && TILE * t + TILE <= A.a.sinks)) && TILE * t + TILE - 1 <= all_hi;  // the same in all lanes
             const bool masked = !full || __ballot(!v_ok) != 0;
             if (masked) {
                 bool any = false;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     const int p = TILE * t + 16 * g + j;
-                    const bool see = v_ok && p >= p_lo && p <= p_hi;
+                    const bool see = v_ok && (p >= p_lo || (SINKS && p < A.a.sinks)) && p <= p_hi;
                     any |= see;
                     x[j] = see ? x[j] * f : -INFINITY;
                 }
@@ -676,7 +713,7 @@ __device__ __forceinline__ int key_piece(int p, int c) {
     return D % 128 == 0 ? c ^ ((p & 3) | (p >> 2 & 4)) : c ^ ((p >> 1 & 1) | (p >> 3 & 2));
 }
 
-template <int D, bool HILO>
+template <int D, bool HILO, bool SINKS>
 __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k_kv_prompt(Args A, const int32_t *__restrict__ page_table) {
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
@@ -687,7 +724,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.P.heads;
     Work w;
-    if (!find_work(A, blockIdx.x / A.P.heads, cut_of<false>(A).chunk, w)) return;
+    if (!find_work<SINKS>(A, blockIdx.x / A.P.heads, cut_of<false, SINKS>(A).chunk, w)) return;
     const KvSeq &q = w.q;
     const int G = A.G, first = q.first();
     const int x0 = w.unit * P_ROWS, n_x = min(P_ROWS, (q.r1 - q.r0) * G - x0);
@@ -708,9 +745,8 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int all_lo = max(0, max(0, f1) - (A.a.window - 1)), all_hi = f0;
     // the block's tiles
     const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
-    int t_lo = max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, t_hi = u_hi < 0 ? 0 : u_hi / TILE + 1;
-    t_lo = max(t_lo, w.t_lo);
-    t_hi = min(t_hi, w.t_hi);
+    const Visits<SINKS> visit(A, w.sp, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, u_hi < 0 ? 0 : u_hi / TILE + 1);
+    const int t_lo = visit.lo, t_hi = visit.hi;
     const int32_t *__restrict__ pages = page_table + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
 
@@ -787,18 +823,19 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int k_pos = 16 * (n >> 2) + (n & 3);
     const int k_row0 = k_pos * D + key_piece<D>(k_pos, g) * 16, v_row0 = n * TILE + (2 * g ^ (n & 7)) * 8;
     if (t_lo < t_hi) {
-        look(t_lo);
-        fetch(t_lo);
-        look(t_lo + 1);
+        look(visit.tile(t_lo));
+        fetch(visit.tile(t_lo));
+        look(visit.tile(t_lo + 1));
         place(buf[0]);
-        if (t_lo + 1 < t_hi) fetch(t_lo + 1);
-        look(t_lo + 2);
+        if (t_lo + 1 < t_hi) fetch(visit.tile(t_lo + 1));
+        look(visit.tile(t_lo + 2));
     }
     __syncthreads();
-    for (int t = t_lo; t < t_hi; t++) {
-        const PShared<D> &sh = buf[(t - t_lo) & (BUFS - 1)];
-        if (TILE * t <= w_hi && TILE * t + TILE - 1 >= w_lo) {  // some row of the wave sees it (the same in all lanes)
-            const bool full = placed && TILE * t >= all_lo && TILE * t + TILE - 1 <= all_hi;
+    for (int i_t = t_lo; i_t < t_hi; i_t++) {
+        const PShared<D> &sh = buf[(i_t - t_lo) & (BUFS - 1)];
+        const int t = visit.tile(i_t);
+        if (TILE * t <= w_hi && (TILE * t + TILE - 1 >= w_lo || (SINKS && TILE * t < A.a.sinks))) {  // some row of the wave sees it (the same in all lanes)
+            const bool full = placed && (TILE * t >= all_lo || (SINKS && TILE * t + TILE <= A.a.sinks)) && TILE * t + TILE - 1 <= all_hi;
             const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
             // opaque: what is formed from them would be kept over the loop, in registers that spill
             int k_row = k_row0, v_row = v_row0;
@@ -833,6 +870,10 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                 if (masked) {
                     const int p = TILE * t + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
                     seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
+                    if constexpr (SINKS) {
+                        const int last = min(hi, A.a.sinks - 1 - p);
+                        if (sh.ok[g] && last >= 0) seen |= 0xFFFFu >> (15 - last);
+                    }
                     if (!seen) sv = 0.0f;  // as in k_kv_attention
                 }
                 asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
@@ -904,10 +945,10 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                 }
         }
         if constexpr (BUFS == 1) __syncthreads();
-        if (t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
-            place(buf[(t + 1 - t_lo) & (BUFS - 1)]);
-            if (t + 2 < t_hi) fetch(t + 2);
-            look(t + 3);
+        if (i_t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
+            place(buf[(i_t + 1 - t_lo) & (BUFS - 1)]);
+            if (i_t + 2 < t_hi) fetch(visit.tile(i_t + 2));
+            look(visit.tile(i_t + 3));
         }
         __syncthreads();
     }
@@ -933,13 +974,13 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
 // head), four values per lane, every wave of the grid the next ones; U ranges
 // at a time, whose loads depend on nothing.
 constexpr int JOIN_BLOCKS = 1024;  // at most: four waves per SIMD
-template <int D, bool LINE>
+template <int D, bool LINE, bool SINKS>
 __global__ __launch_bounds__(256) void k_kv_join(Args A0, Args A1) {
     constexpr int LPR = D / 4, RPW = 64 / LPR;  // lanes of a row, rows of a wave
     constexpr int U = LINE ? 16 : 8;  // a line's units are the long ones
     const Args &A = blockIdx.y ? A1 : A0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Cut cut = cut_of<LINE>(A);
+    const Cut cut = cut_of<LINE, SINKS>(A);
     const int chunk = cut.chunk;
     const bool line = LINE && cut.line;
     const int rows = A.rows;
@@ -947,20 +988,20 @@ __global__ __launch_bounds__(256) void k_kv_join(Args A0, Args A1) {
         const int h = task % A.P.heads;
         int seq, group;
         if (!kv_find(A.B, task / A.P.heads, [&](const KvSeq &q) {
-                const Span p = span_of(A, q);
+                const Span p = span_of<SINKS>(A, q);
                 return p.units && (line || ranges(p.tiles, chunk) > 1) ? ((q.r1 - q.r0) * A.G + RPW - 1) / RPW : 0;
             }, seq, group))
             return;
         // what stands in front of the sequence: cells of the line, or split ranges
         int before = 0;
         for (int s = lane; s < seq; s += 64) {
-            const Span p = span_of(A, kv_seq(A.B, s));
+            const Span p = span_of<SINKS>(A, kv_seq(A.B, s));
             const int n = ranges(p.tiles, chunk);
             before += line ? p.units * line_cells(p) : n > 1 ? p.units * n : 0;
         }
         before = __builtin_amdgcn_readlane(wave_scan(before), 63);
         const KvSeq q = kv_seq(A.B, seq);
-        const Span sp = span_of(A, q);
+        const Span sp = span_of<SINKS>(A, q);
         const int x0 = group * RPW, unit = x0 / rows;
         int slot, nr;  // the first range's; their number
         if (line) {
@@ -1032,8 +1073,12 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
     if (!rows.n_rows) return hipSuccess;
     const int G = a.n_q / pool.heads;
     const size_t x = (size_t)rows.n_rows * G;
-    auto go = [&](auto d) {
+    // positions that the tiles of a sequence span at most: with sinks the window's and theirs (a sequence's rows are n_rows at most)
+    const int64_t span = a.sinks ? std::min((int64_t)rows.cap, TILE * (((int64_t)a.sinks + TILE - 1) / TILE + ((int64_t)a.window + rows.n_rows) / TILE + 2))
+                                 : (int64_t)rows.cap;
+    auto go = [&](auto d, auto with_sinks) {
         constexpr int D = decltype(d)::value;
+        constexpr bool SINKS = decltype(with_sinks)::value;
         const bool f32 = a.out_dtype == T_F32;
         int vec = 0;
         if (reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride * (a.q_dtype == T_F32 ? 4 : 2) % 16 == 0) vec |= 1;
@@ -1049,36 +1094,36 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
             return hi == INT_MAX ? u : std::min(u, (size_t)rows.n_seqs * ((hi + A.rows - 1) / A.rows));
         };
         auto grid = [&](Args &A, size_t u) {
-            const bool split = rows.cap > (int64_t)A.min_chunk * TILE;
+            const bool split = span > (int64_t)A.min_chunk * TILE;
             if (split) join[joins++] = A;
             return dim3((unsigned)((u + (split ? slots(A.target) / pool.heads + 1 : 0)) * pool.heads));
         };
         auto target = [](size_t room, int unit) { return std::min(TARGET, (int)(room / ((size_t)unit * (D + 2) * sizeof(float)) * 16 / 34)); };
         auto few = [&](int hi) {
-            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), rows.cap > SPLIT_FROM * TILE ? MIN_CHUNK : WHOLE, 0, vec};
+            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), span > SPLIT_FROM * TILE ? MIN_CHUNK : WHOLE, 0, vec};
             const size_t u = units(A, hi);
             // can its tiles come to a line at all?
-            A.line = rows.cap > SPLIT_FROM * TILE && pool.heads * 20 <= A.target &&
-                     (double)u * pool.heads * (rows.cap / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
+            A.line = span > SPLIT_FROM * TILE && pool.heads * 20 <= A.target &&
+                     (double)u * pool.heads * (span / TILE + 2) >= (double)A.target * (LINE_CHUNK - 1);
             in_line = A.line;
             const dim3 g = grid(A, u), b(64 * WAVES);
-            if (A.line && f32) hipLaunchKernelGGL((k_kv_attention<D, 3, true>), g, b, 0, s, A);
-            else if (A.line) hipLaunchKernelGGL((k_kv_attention<D, 2, true>), g, b, 0, s, A);
-            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, 3, false>), g, b, 0, s, A);
-            else hipLaunchKernelGGL((k_kv_attention<D, 2, false>), g, b, 0, s, A);
+            if (A.line && f32) hipLaunchKernelGGL((k_kv_attention<D, 3, true, SINKS>), g, b, 0, s, A);
+            else if (A.line) hipLaunchKernelGGL((k_kv_attention<D, 2, true, SINKS>), g, b, 0, s, A);
+            else if (f32) hipLaunchKernelGGL((k_kv_attention<D, 3, false, SINKS>), g, b, 0, s, A);
+            else hipLaunchKernelGGL((k_kv_attention<D, 2, false, SINKS>), g, b, 0, s, A);
         };
         auto many = [&](int lo) {
             Args A{pool, rows, a, G, P_ROWS, lo, INT_MAX, target(MANY_PARTS, P_ROWS), P_MIN_CHUNK, 0, vec};
             A.a.parts += FEW_PARTS / sizeof(float);
             const dim3 g = grid(A, units(A, INT_MAX)), b(64 * P_WAVES);
-            if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true>), g, b, 0, s, A, rows.pages);
-            else hipLaunchKernelGGL((k_kv_prompt<D, false>), g, b, 0, s, A, rows.pages);
+            if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true, SINKS>), g, b, 0, s, A, rows.pages);
+            else hipLaunchKernelGGL((k_kv_prompt<D, false, SINKS>), g, b, 0, s, A, rows.pages);
         };
         const size_t tokens = (size_t)G * rows.n_seqs, more = x > tokens ? x - tokens : 0;
         const bool prompt = more >= (size_t)LONG &&
-                            (double)more / ROWS * (rows.cap / TILE) * pool.heads >= (double)LONG_TILES * TARGET;
+                            (double)more / ROWS * (span / TILE) * pool.heads >= (double)LONG_TILES * TARGET;
         if (x > (size_t)FEW * rows.n_seqs || prompt) {
-            const bool one = rows.n_seqs == 1 && rows.cap <= ONE_TABLE * TILE;
+            const bool one = rows.n_seqs == 1 && span <= ONE_TABLE * TILE;
             many(one ? 0 : FEW + 1);
             if (!one) few(FEW);
         } else {
@@ -1087,14 +1132,18 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         if (!joins) return;
         constexpr int RPB = 4 * (256 / D);  // rows of a block
         const dim3 g((unsigned)std::min((size_t)JOIN_BLOCKS, (x * pool.heads + RPB - 1) / RPB), (unsigned)joins), b(256);
-        if (in_line) hipLaunchKernelGGL((k_kv_join<D, true>), g, b, 0, s, join[0], join[joins - 1]);
-        else hipLaunchKernelGGL((k_kv_join<D, false>), g, b, 0, s, join[0], join[joins - 1]);
+        if (in_line) hipLaunchKernelGGL((k_kv_join<D, true, SINKS>), g, b, 0, s, join[0], join[joins - 1]);
+        else hipLaunchKernelGGL((k_kv_join<D, false, SINKS>), g, b, 0, s, join[0], join[joins - 1]);
+    };
+    auto pick = [&](auto d) {
+        if (a.sinks) go(d, std::true_type{});
+        else go(d, std::false_type{});
     };
     switch (d_head) {
-    case 64: go(std::integral_constant<int, 64>{}); break;
-    case 128: go(std::integral_constant<int, 128>{}); break;
-    case 192: go(std::integral_constant<int, 192>{}); break;
-    case 256: go(std::integral_constant<int, 256>{}); break;
+    case 64: pick(std::integral_constant<int, 64>{}); break;
+    case 128: pick(std::integral_constant<int, 128>{}); break;
+    case 192: pick(std::integral_constant<int, 192>{}); break;
+    case 256: pick(std::integral_constant<int, 256>{}); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

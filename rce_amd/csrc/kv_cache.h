@@ -41,6 +41,7 @@ struct KvAttention {
     uint32_t q_dtype, out_dtype;
     int n_q;
     int window;   // INT_MAX: none
+    int sinks;    // first positions that every row sees, window or not
     float scale;
     KvRope rope;
     float *parts;  // kv_attention_parts_bytes()

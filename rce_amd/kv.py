@@ -1,7 +1,8 @@
-"""The paged 8-bit KV cache, attention over it and sampling
-(``rce_qmm_kv_*``, ``rce_qmm_sample_dev`` in include/rce_qmm.h): what a
-program that steps many sequences with ``mm_batched_dev`` needs between the
-projections and after the head.  Everything works on device addresses and is
+"""The paged 8-bit KV cache, its pages, norms and rotation of heads, attention
+and sampling (``rce_qmm_kv_*``, ``rce_qmm_qk_norm_rope_dev``,
+``rce_qmm_sample_dev`` in include/rce_qmm.h): what a program that steps many
+sequences with ``mm_batched_dev`` needs between the projections and after the
+head.  Everything works on device addresses and is
 asynchronous on the given stream (None: the context's); there is no CPU path.
 """
 from __future__ import annotations
@@ -14,7 +15,9 @@ import numpy as np
 from ._lib import QmmError, check, lib
 from .qmm import Context, DeviceBuffer, _ptr
 
-__all__ = ["KvCache", "KvBatch", "Rope", "kv_append_dev", "kv_read_dev", "kv_attention_dev", "sample_dev"]
+__all__ = ["KvCache", "KvBatch", "KvTable", "Rope", "Heads", "kv_append_dev", "kv_read_dev", "kv_attention_dev",
+           "kv_attention_sinks_dev", "qk_norm_rope_dev", "kv_copy_dev", "kv_fork_dev", "kv_release_dev",
+           "kv_reserve_dev", "kv_compact_dev", "sample_dev"]
 
 
 # The header's structs as bytes: made once per object, passed as they are (a
@@ -23,6 +26,9 @@ _CACHE = struct.Struct("@PPPPNNNN")
 _BATCH = struct.Struct("@PPPNNN")
 _ROPE = struct.Struct("@PNN")
 _SAMPLING = struct.Struct("@PPPPP")
+_TABLE = struct.Struct("@PNN")
+_HEADS = struct.Struct("@PNPNPN")
+_SCALING = struct.Struct("@ffPNff")
 
 
 def _pack(fmt: struct.Struct, *values: int) -> bytes:
@@ -100,12 +106,53 @@ class Rope:
         check(lib().rce_qmm_rope_table(freq_base, dim, n_pos, _ptr(out)))
         return out
 
+    @staticmethod
+    def scaled_table(freq_base: float, dim: int, n_pos: int, factor: float = 1.0, divisors=None, orig_context: int = 0,
+                     beta_fast: float = 32.0, beta_slow: float = 1.0, magnitude: float = 1.0) -> np.ndarray:
+        """A table [n_pos, dim / 2, 2] for long contexts, by angles in 64
+        bits (rce_qmm_rope_table_scaled): frequencies divided by `divisors`
+        (one per pair) and by `factor`, with `orig_context` the slow pairs'
+        only, between beta_fast and beta_slow turns over it."""
+        if dim % 2 or dim < 0 or n_pos < 0:
+            raise QmmError(2, "dim must be even, n_pos not negative")
+        if divisors is not None:
+            divisors = np.ascontiguousarray(divisors, np.float32)
+            if divisors.shape != (dim // 2,):
+                raise QmmError(2, "divisors must be one value per pair")
+        out = np.empty((n_pos, dim // 2, 2), np.float32)
+        how = _pack(_SCALING, factor, magnitude, 0 if divisors is None else divisors.ctypes.data, orig_context, beta_fast, beta_slow)
+        check(lib().rce_qmm_rope_table_scaled(freq_base, dim, n_pos, how, _ptr(out)))
+        return out
+
     @classmethod
-    def upload(cls, ctx: Context, freq_base: float, dim: int, n_pos: int) -> "Rope":
-        b = DeviceBuffer.from_numpy(ctx, cls.table(freq_base, dim, n_pos))
+    def upload(cls, ctx: Context, freq_base: float, dim: int, n_pos: int, **scaling) -> "Rope":
+        """The decoder's table on the device, or with any of
+        ``scaled_table``'s arguments that one."""
+        make = cls.scaled_table if scaling else cls.table
+        b = DeviceBuffer.from_numpy(ctx, make(freq_base, dim, n_pos, **scaling))
         r = cls(b.ptr, dim, n_pos)
         r.buffer = b
         return r
+
+
+class KvTable:
+    """Sequences' page tables (rce_qmm_kv_table): device address of pages
+    [n_seqs][max_pages] int32, -1 where there is no page."""
+
+    __slots__ = ("raw",)
+
+    def __init__(self, pages: int, n_seqs: int, max_pages: int):
+        self.raw = _pack(_TABLE, pages, n_seqs, max_pages)
+
+
+class Heads:
+    """Query or key heads of ``qk_norm_rope_dev`` (rce_qmm_heads): device
+    addresses, strides in values from row to row; weight 0: ones."""
+
+    __slots__ = ("raw",)
+
+    def __init__(self, in_dev: int, in_stride: int, n_heads: int, out_dev: int, out_stride: int, weight: int = 0):
+        self.raw = _pack(_HEADS, in_dev, in_stride, out_dev, out_stride, weight, n_heads)
 
 
 def _raw(x) -> bytes | None:
@@ -139,6 +186,73 @@ def kv_attention_dev(ctx: Context, cache: KvCache, batch: KvBatch, q_dev: int, q
         out_stride = n_q_heads * cache.d_head
     st = lib().rce_qmm_kv_attention_dev(ctx.handle, _raw(cache), _raw(batch), q_dev, q_dtype, q_stride, n_q_heads, _raw(rope),
                                         scale, window, out_dev, out_dtype, out_stride or 0, stream)
+    if st:
+        check(st)
+
+
+def kv_attention_sinks_dev(ctx: Context, cache: KvCache, batch: KvBatch, q_dev: int, q_dtype, q_stride: int, n_q_heads: int,
+                           out_dev: int, out_dtype, scale: float, window: int, sinks: int, rope: Rope | None = None,
+                           out_stride: int | None = None, stream: int | None = None) -> None:
+    """``kv_attention_dev`` with a window and `sinks` first positions that
+    every row sees (rce_qmm_kv_attention_sinks_dev)."""
+    if out_stride is None and cache is not None:
+        out_stride = n_q_heads * cache.d_head
+    st = lib().rce_qmm_kv_attention_sinks_dev(ctx.handle, _raw(cache), _raw(batch), q_dev, q_dtype, q_stride, n_q_heads,
+                                              _raw(rope), scale, window, sinks, out_dev, out_dtype, out_stride or 0, stream)
+    if st:
+        check(st)
+
+
+def qk_norm_rope_dev(ctx: Context, batch: KvBatch, q: Heads | None, k: Heads | None, d_head: int, in_dtype, out_dtype,
+                     eps: float | None = None, rope: Rope | None = None, interleaved: bool = False,
+                     stream: int | None = None) -> None:
+    """Norms (eps None: none) and rotation of query and key heads in one
+    pass (rce_qmm_qk_norm_rope_dev)."""
+    st = lib().rce_qmm_qk_norm_rope_dev(ctx.handle, _raw(batch), _raw(q), _raw(k), d_head, in_dtype, out_dtype,
+                                        -1.0 if eps is None else eps, _raw(rope), interleaved, stream)
+    if st:
+        check(st)
+
+
+def kv_copy_dev(ctx: Context, src: KvCache, dst: KvCache, src_ids_dev: int, dst_ids_dev: int, n: int,
+                stream: int | None = None) -> None:
+    """Pages of one pool to pages of another, or of itself (rce_qmm_kv_copy_dev)."""
+    st = lib().rce_qmm_kv_copy_dev(ctx.handle, _raw(src), _raw(dst), src_ids_dev, dst_ids_dev, n, stream)
+    if st:
+        check(st)
+
+
+def kv_fork_dev(ctx: Context, cache: KvCache, src: KvTable, dst: KvTable, parents_dev: int, refs_dev: int,
+                stream: int | None = None) -> None:
+    """Every sequence of `dst` gets its parent's pages in `src`
+    (rce_qmm_kv_fork_dev)."""
+    st = lib().rce_qmm_kv_fork_dev(ctx.handle, _raw(cache), _raw(src), _raw(dst), parents_dev, refs_dev, stream)
+    if st:
+        check(st)
+
+
+def kv_release_dev(ctx: Context, cache: KvCache, table: KvTable, refs_dev: int, from_dev: int | None = None,
+                   to_dev: int | None = None, stream: int | None = None) -> None:
+    """Give up the pages wholly in positions from .. to - 1 of each sequence
+    (rce_qmm_kv_release_dev; None: all)."""
+    st = lib().rce_qmm_kv_release_dev(ctx.handle, _raw(cache), _raw(table), from_dev, to_dev, refs_dev, stream)
+    if st:
+        check(st)
+
+
+def kv_reserve_dev(ctx: Context, cache: KvCache, batch: KvBatch, refs_dev: int, missing_dev: int | None = None,
+                   stream: int | None = None) -> None:
+    """Pages of their own for the batch's rows, written into its tables
+    (rce_qmm_kv_reserve_dev)."""
+    st = lib().rce_qmm_kv_reserve_dev(ctx.handle, _raw(cache), _raw(batch), refs_dev, missing_dev, stream)
+    if st:
+        check(st)
+
+
+def kv_compact_dev(ctx: Context, cache: KvCache, table: KvTable, refs_dev: int, new_ids_dev: int,
+                   n_used_dev: int | None = None, stream: int | None = None) -> None:
+    """The used pages to the front of the pool (rce_qmm_kv_compact_dev)."""
+    st = lib().rce_qmm_kv_compact_dev(ctx.handle, _raw(cache), _raw(table), refs_dev, new_ids_dev, n_used_dev, stream)
     if st:
         check(st)
 

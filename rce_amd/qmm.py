@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import struct
 
 import numpy as np
 
@@ -22,7 +23,7 @@ from ._lib import QmmError, check, lib
 __all__ = [
     "GgufDtype", "Mode", "Context", "QuantWeight", "DeviceBuffer", "QmmError",
     "block_geometry", "row_bytes", "supports", "mm_1d", "mm_1d_serial", "mm_batched",
-    "mm_batched_dev", "moe_router", "moe_ffn_dev", "moe_swiglu_dev", "quantize",
+    "mm_batched_dev", "moe_router", "MoeRouting", "moe_route_dev", "moe_ffn_dev", "moe_swiglu_dev", "quantize",
 ]
 
 
@@ -313,6 +314,32 @@ def moe_router(logits, top_k: int, normalize: bool = True):
     wts = np.empty((n_tokens, top_k), np.float32)
     check(lib().rce_qmm_moe_router(_ptr(lg), n_tokens, n_expert, top_k, int(normalize), _ptr(ids), _ptr(wts)))
     return ids, wts
+
+
+class MoeRouting:
+    """How tokens are routed (rce_qmm_moe_routing): softmax or sigmoid scores,
+    a bias on the device that moves the choice alone, groups of which the best
+    topk_group are kept."""
+
+    __slots__ = ("raw",)
+    _FMT = struct.Struct("@iPNNNNif")
+
+    def __init__(self, top_k: int, sigmoid: bool = False, bias_dev: int = 0, n_group: int = 1, topk_group: int = 1,
+                 group_top: int = 1, normalize: bool = True, scale: float = 1.0):
+        try:
+            self.raw = self._FMT.pack(int(bool(sigmoid)), bias_dev or 0, top_k, n_group, topk_group, group_top, int(bool(normalize)), scale)
+        except struct.error as e:
+            raise QmmError(2, f"an address or a size is out of range: {e}") from None
+
+
+def moe_route_dev(ctx: Context, logits_dev: int, dtype, n_tokens: int, n_expert: int, row_stride: int, how: MoeRouting,
+                  ids_dev: int, weights_dev: int, stream: int | None = None) -> None:
+    """Experts and weights of every token from its logits, on the device
+    (rce_qmm_moe_route_dev): what moe_ffn_dev and moe_swiglu_dev take."""
+    st = lib().rce_qmm_moe_route_dev(ctx.handle, logits_dev, dtype, n_tokens, n_expert, row_stride,
+                                     None if how is None else how.raw, ids_dev, weights_dev, stream)
+    if st:
+        check(st)
 
 
 def moe_ffn_dev(ctx: Context, w1: list[QuantWeight], w2: list[QuantWeight], x_dev: int, t_rows: int,
