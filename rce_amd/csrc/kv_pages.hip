@@ -17,6 +17,14 @@ __device__ __forceinline__ int seen(const int32_t *p) {  // what other waves' at
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A barrier behind which the block's waves see each other's accesses to memory by `seen` and atomics: waves of one block share an
+// L2, so that it is enough for them to have arrived there.  (A fence for the whole GPU writes back what the L2 holds of the kernels before:
+// behind a copy of 300 MB it cost 3 us.)
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // ---- tables -----------------------------------------------------------------
 
 __global__ __launch_bounds__(256) void k_kv_fork(KvTable from, KvTable to, const int32_t *parents, KvRefs R) {
@@ -46,12 +54,19 @@ __global__ __launch_bounds__(256) void k_kv_release(KvTable t, int page_tokens, 
 
 // The pages that a call's rows touch are its items, in the order of (sequence, position): one block
 // plans them all.  An item without a page needs one; an item whose page others name too asks to leave
-// it.  Where all that name a page ask (its count falls to 0), the first of them keeps it: its number - CODE
-// is then the least that is written to the count.
+// it.  Where all that name a page ask, the first of them keeps it.  Free pages are those whose count is 0, in
+// order, looked for EACH * PLAN counts at a time.
+//
+// A call of up to PLAN items (a token of every sequence) keeps them in registers and finds who asks for the same page in a
+// table in LDS.  Others go over the items once per step, and count on the pages' own counts: an item that asks takes one off;
+// where that leaves none, the least item number - CODE that is written there keeps the page.
+//
+// What bounds it: the chain of loads (lengths, entries, counts), barriers of 16 waves.
 constexpr int PLAN = 1024;       // threads
 constexpr int CODE = 1 << 30;    // items are fewer than 2^24
-constexpr int EACH = 4;          // counts that a thread looks at for free pages
+constexpr int EACH = 4;          // counts that a thread looks at for free pages, and items of a thread's step
 constexpr int RING = 2 * EACH * PLAN;
+constexpr int SLOTS = 2 * PLAN;  // of the table in LDS
 
 struct Front {  // the first `blocks` blocks of page src to page dst, every head
     int src, dst, blocks, pad;
@@ -79,111 +94,228 @@ __device__ __forceinline__ int block_scan(int v, int *part, int &total) {
     return before + incl - v;
 }
 
+// Ranks among N * PLAN values in the order of (wave, e, lane): value e of this thread is number 64 (N wave + e) + lane.
+// of[e]: the true ones before it; the total is the same in all threads.
+template <int N>
+__device__ __forceinline__ int ranks(const bool (&is)[N], int *part, int (&of)[N]) {
+    const int wave = threadIdx.x >> 6;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        const uint64_t m = __ballot(is[e]);
+        of[e] = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        n += __popcll(m);
+    }
+    if ((threadIdx.x & 63) == 0) part[wave] = n;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN / 64; w++) {
+        const int p = part[w];
+        before += w < wave ? p : 0;
+        total += p;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; e++) of[e] += before;
+    return total;
+}
+template <int N>
+__device__ __forceinline__ int numbered(int e) { return 64 * (N * (threadIdx.x >> 6) + e) + (threadIdx.x & 63); }
+
 __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int32_t *pages, KvRefs R, int32_t *missing, Room *room) {
-    __shared__ int part[PLAN / 64], start[PLAN + 1], slot0[PLAN], ring[RING];
+    __shared__ int part[PLAN / 64], start[PLAN + 1], slot0[PLAN], front0[PLAN], lost[PLAN], ring[RING];
     __shared__ int n_fronts;
+    int *const key = ring, *const asked = ring + SLOTS, *const first_ask = ring + 2 * SLOTS;  // before the ring is used
+    static_assert(3 * SLOTS <= RING, "the table fits the ring");
     const int tid = threadIdx.x;
+    if (!B.n_rows || !B.cap) {  // no items; the batch's arrays may be null
+        if (missing)
+            for (int s = tid; s < B.n_seqs; s += PLAN) missing[s] = 0;
+        return;
+    }
+    auto entry = [&](int s, int slot) { return pages + (size_t)s * B.max_pages + slot; };
+
+    // the first counts, on their way while the items are found
+    int ahead[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) ahead[e] = R.refs[min(numbered<EACH>(e), R.n_pages - 1)];
+    int head = 0, have = 0, looked = 0;  // the ring's first free page, its free pages, counts looked at
+    auto look = [&] {
+        bool free[EACH];
+        int of[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int at = looked + numbered<EACH>(e);
+            free[e] = at < R.n_pages && (looked ? seen(R.refs + at) : ahead[e]) == 0;
+        }
+        const int more = ranks<EACH>(free, part, of);
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+            if (free[e]) ring[(head + have + of[e]) & (RING - 1)] = looked + numbered<EACH>(e);
+        have += more;
+        looked += min(EACH * PLAN, R.n_pages - looked);
+        __syncthreads();
+    };
+    // a free page for an item (rank: items of this step that need one before it), or none; its page p is left behind if it has one
+    auto give = [&](int s, int slot, int rank, int p, bool leaves) {
+        const int to = rank < have ? ring[(head + rank) & (RING - 1)] : -1;
+        *entry(s, slot) = to;
+        if (to < 0) return false;
+        R.refs[to] = 1;
+        // what stands in front of the call's rows in the page it leaves
+        const int q = s & (PLAN - 1);
+        if (leaves && slot == slot0[q] && front0[q]) room->fronts[atomicAdd(&n_fronts, 1)] = {p, to, front0[q], 0};
+        return true;
+    };
+    // items of the sequences c .. c + PLAN - 1, and where they start
+    auto list = [&](int c) {
+        int n = 0, items;
+        if (c + tid < B.n_seqs) {
+            const KvSeq q = kv_seq(B, c + tid);
+            const int lo = q.lo(), hi = q.hi(B);
+            slot0[tid] = lo >> lg_page;
+            front0[tid] = ((lo & ((1 << lg_page) - 1)) + KV_BLOCK - 1) / KV_BLOCK;
+            n = hi > lo ? ((hi - 1) >> lg_page) - slot0[tid] + 1 : 0;
+        }
+        start[tid] = block_scan(n, part, items);
+        if (tid == 0) start[PLAN] = items;
+        __syncthreads();
+        return items;
+    };
+    auto sequence = [&](int i) {  // the last one that starts at or before item i
+        int s = 0;
+#pragma unroll
+        for (int o = PLAN / 2; o; o /= 2)
+            if (start[s + o] <= i) s += o;
+        return s;
+    };
+
     if (tid == 0) n_fronts = 0;
+    lost[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < SLOTS / PLAN; i++) {
+        key[tid + PLAN * i] = -1;
+        asked[tid + PLAN * i] = 0;
+        first_ask[tid + PLAN * i] = PLAN;
+    }
+    int items = list(0);
+    if (B.n_seqs <= PLAN && items <= PLAN) {
+        const bool is = tid < items;
+        const int s = sequence(min(tid, max(items - 1, 0))), slot = slot0[s] + tid - start[s];
+        const int p = is ? *entry(s, slot) : 0;
+        const bool named = (unsigned)p < (unsigned)R.n_pages;
+        const int refs = is && named ? R.refs[p] : 0;
+        bool need = is && !named, leaves = is && named && refs > 1;
+        if (__syncthreads_or(leaves)) {
+            int h = (int)(((uint32_t)p * 2654435769u) >> 21);  // of 2048
+            static_assert(SLOTS == 2048, "11 bits");
+            if (leaves) {
+                for (;;) {  // at most PLAN of the SLOTS are taken: an empty one comes
+                    const int k = atomicCAS(key + h, -1, p);
+                    if (k == -1 || k == p) break;
+                    h = (h + 1) & (SLOTS - 1);
+                }
+                atomicAdd(asked + h, 1);
+                atomicMin(first_ask + h, tid);
+            }
+            __syncthreads();
+            if (leaves && asked[h] == refs && first_ask[h] == tid) leaves = false;
+            need |= leaves;
+        }
+        int total;
+        const int rank = block_scan(need, part, total);
+        while (have < total && looked < R.n_pages) look();  // the same in every thread
+        if (need) {
+            if (leaves) atomicSub(R.refs + p, 1);
+            if (!give(s, slot, rank, p, leaves)) atomicAdd(lost + s, 1);
+        }
+        __syncthreads();
+        if (missing && tid < B.n_seqs) missing[tid] = lost[tid];
+        if (tid == 0) room->n_fronts = n_fronts;
+        return;
+    }
+
     if (missing)
         for (int s = tid; s < B.n_seqs; s += PLAN) missing[s] = 0;
-    if (!B.n_rows || !B.cap) return;  // no items; the batch's arrays may be null
-    int chunk = -1, items = 0;
-    // f(item number, sequence, its page's place in the table, place of its first item) for every item, PLAN at a time; every thread
-    // calls it (item -1: none)
+    // f(number of the first, items' sequences and places, how many) for EACH consecutive items of every thread; every thread calls it
+    int chunk = 0;
     auto each = [&](auto f) {
         int before = 0;
         for (int c = 0; c < B.n_seqs; c += PLAN) {
             if (c != chunk) {
-                const int s = c + tid;
-                int n = 0;
                 __syncthreads();
-                if (s < B.n_seqs) {
-                    const KvSeq q = kv_seq(B, s);
-                    slot0[tid] = q.lo() >> lg_page;
-                    n = q.hi(B) > q.lo() ? ((q.hi(B) - 1) >> lg_page) - slot0[tid] + 1 : 0;
-                }
-                start[tid] = block_scan(n, part, items);
-                if (tid == 0) start[PLAN] = items;
+                items = list(c);
                 chunk = c;
-                __syncthreads();
             }
-            for (int i0 = 0; i0 < items; i0 += PLAN) {
-                const int i = i0 + tid;
-                int s = 0;
+            for (int i0 = 0; i0 < items; i0 += EACH * PLAN) {
+                int s[EACH], slot[EACH];
+                const int i = i0 + EACH * tid, n = min(EACH, max(0, items - i));
+                int q = sequence(min(i, items - 1));
 #pragma unroll
-                for (int o = PLAN / 2; o; o /= 2)  // the last sequence that starts at or before i
-                    if (start[s + o] <= i) s += o;
-                f(i < items ? before + i : -1, c + s, slot0[s] + i - start[s], slot0[s]);
+                for (int e = 0; e < EACH; e++) {
+                    const int at = min(i + e, items - 1);
+                    while (start[q + 1] <= at) q++;  // start[PLAN] is above all
+                    s[e] = c + q;
+                    slot[e] = slot0[q] + at - start[q];
+                }
+                f(before + i, s, slot, n);
             }
             before += items;
         }
     };
-    auto entry = [&](int s, int slot) { return pages + (size_t)s * B.max_pages + slot; };
 
     bool shared = false;
-    each([&](int item, int s, int slot, int) {
-        if (item < 0) return;
-        const int p = *entry(s, slot);
-        const int want = (unsigned)p >= (unsigned)R.n_pages ? 1 : R.refs[p] > 1 ? 2 : 0;
-        room->wants[item] = (uint8_t)want;
-        shared |= want == 2;
+    each([&](int item, const int (&s)[EACH], const int (&slot)[EACH], int n) {
+        int p[EACH], refs[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) p[e] = *entry(s[e], slot[e]);
+#pragma unroll
+        for (int e = 0; e < EACH; e++) refs[e] = (unsigned)p[e] < (unsigned)R.n_pages ? R.refs[p[e]] : 0;
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+            if (e < n) {
+                const int want = (unsigned)p[e] >= (unsigned)R.n_pages ? 1 : refs[e] > 1 ? 2 : 0;
+                room->wants[item + e] = (uint8_t)want;
+                shared |= want == 2;
+            }
     });
     if (__syncthreads_or(shared)) {
-        each([&](int item, int s, int slot, int) {
-            if (item >= 0 && room->wants[item] == 2) atomicSub(R.refs + *entry(s, slot), 1);
+        each([&](int item, const int (&s)[EACH], const int (&slot)[EACH], int n) {
+            for (int e = 0; e < n; e++)
+                if (room->wants[item + e] == 2) atomicSub(R.refs + *entry(s[e], slot[e]), 1);
         });
-        __threadfence();
-        __syncthreads();
-        each([&](int item, int s, int slot, int) {
-            if (item < 0 || room->wants[item] != 2) return;
-            int32_t *r = R.refs + *entry(s, slot);
-            if (seen(r) <= 0) atomicMin(r, item - CODE);
+        arrived();
+        each([&](int item, const int (&s)[EACH], const int (&slot)[EACH], int n) {
+            for (int e = 0; e < n; e++) {
+                if (room->wants[item + e] != 2) continue;
+                int32_t *r = R.refs + *entry(s[e], slot[e]);
+                if (seen(r) <= 0) atomicMin(r, item + e - CODE);
+            }
         });
     }
-    __threadfence();
-    __syncthreads();
-    int head = 0, have = 0, looked = 0;  // the ring's first free page, its free pages, counts looked at
-    each([&](int item, int s, int slot, int first) {
-        const int want = item < 0 ? 0 : room->wants[item];
-        int p = -1;
-        bool need = want == 1;
-        if (want == 2) {
-            p = *entry(s, slot);
-            need = seen(R.refs + p) != item - CODE;
-            if (!need) __hip_atomic_store(R.refs + p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        int total;
-        const int rank = block_scan(need, part, total);
-        while (have < total && looked < R.n_pages) {  // the same in every thread
-            int free[EACH], n = 0;
+    arrived();
+    each([&](int item, const int (&s)[EACH], const int (&slot)[EACH], int n) {
+        int p[EACH], count = 0;
+        bool need[EACH], leaves[EACH];
 #pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const int at = looked + EACH * tid + e;
-                free[e] = at < R.n_pages && seen(R.refs + at) == 0;
-                n += free[e];
+        for (int e = 0; e < EACH; e++) {
+            const int want = e < n ? room->wants[item + e] : 0;
+            leaves[e] = want == 2;
+            need[e] = want == 1;
+            p[e] = -1;
+            if (leaves[e]) {
+                p[e] = *entry(s[e], slot[e]);
+                leaves[e] = need[e] = seen(R.refs + p[e]) != item + e - CODE;
+                if (!need[e]) __hip_atomic_store(R.refs + p[e], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            int more, at = block_scan(n, part, more);
+            count += need[e];
+        }
+        int total, rank = block_scan(count, part, total);
+        while (have < total && looked < R.n_pages) look();  // the same in every thread
 #pragma unroll
-            for (int e = 0; e < EACH; e++)
-                if (free[e]) ring[(head + have + at++) & (RING - 1)] = looked + EACH * tid + e;
-            have += more;
-            looked += min(EACH * PLAN, R.n_pages - looked);
-            __syncthreads();
-        }
-        if (need) {
-            const int to = rank < have ? ring[(head + rank) & (RING - 1)] : -1;
-            *entry(s, slot) = to;
-            if (to >= 0) {
-                R.refs[to] = 1;
-                // what stands in front of the call's rows in the page it leaves
-                const KvSeq q = kv_seq(B, s);
-                const int in_front = q.lo() & ((1 << lg_page) - 1);
-                if (want == 2 && slot == first && in_front)
-                    room->fronts[atomicAdd(&n_fronts, 1)] = {p, to, (in_front + KV_BLOCK - 1) / KV_BLOCK, 0};
-            } else if (missing) {
-                atomicAdd(missing + s, 1);
-            }
-        }
+        for (int e = 0; e < EACH; e++)
+            if (need[e] && !give(s[e], slot[e], rank++, p[e], leaves[e]) && missing) atomicAdd(missing + s[e], 1);
         const int used = min(have, total);
         head = (head + used) & (RING - 1);
         have -= used;
@@ -213,11 +345,19 @@ __global__ __launch_bounds__(256) void k_kv_copy_fronts(KvPool P, int d, const R
 
 // Pages src[i] of one pool to dst[i] of another (or the same), i < *count (null: n): a block takes PIECE bytes of a page's
 // keys or values, every block of the grid the next ones.
+// The first `renaming` blocks give the entries of t their pages' new ids instead.
 constexpr int PIECE = 16384;
 __global__ __launch_bounds__(256) void k_kv_copy(KvPool A, KvPool B, size_t page_bytes, int pieces, const int32_t *src, const int32_t *dst,
-                                                 const int32_t *count, int n) {
+                                                 const int32_t *count, int n, KvTable t, const int32_t *new_ids, unsigned renaming) {
+    if (blockIdx.x < renaming) {
+        for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < t.entries(); i += renaming * 256) {
+            const int p = t.pages[i];
+            if ((unsigned)p < (unsigned)A.n_pages) t.pages[i] = new_ids[p];
+        }
+        return;
+    }
     const size_t units = (size_t)(count ? *count : n) * 2 * pieces;
-    for (size_t u = blockIdx.x; u < units; u += gridDim.x) {
+    for (size_t u = blockIdx.x - renaming; u < units; u += gridDim.x - renaming) {
         const size_t m = u / (2 * pieces);
         const int rest = (int)(u - m * 2 * pieces), kind = rest & 1, piece = rest >> 1;
         const int a = src[m], b = dst[m];
@@ -245,89 +385,88 @@ struct Moves {
     int count, pad[3];
     int32_t src[KV_COMPACT_PAGES / 2], dst[KV_COMPACT_PAGES / 2];
 };
+// One block: the used pages are counted, then the free ones among the first n_used ranked, then the used ones behind them, LOOK
+// consecutive counts a thread and step.
+constexpr int LOOK = 16;
+__device__ __forceinline__ void look_at(const KvRefs &R, int from, int (&r)[LOOK]) {
+#pragma unroll
+    for (int e = 0; e < LOOK; e++) r[e] = R.refs[min(from + numbered<LOOK>(e), R.n_pages - 1)];
+#pragma unroll
+    for (int e = 0; e < LOOK; e++) r[e] = from + numbered<LOOK>(e) < R.n_pages ? r[e] : 0;
+}
 __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids, int32_t *n_used, Moves *moves) {
-    __shared__ int part[PLAN / 64];
+    __shared__ int part[PLAN / 64], list[LOOK * PLAN / 2];  // where ref holds all counts, what is free below n: half of them at most
     const int tid = threadIdx.x;
-    int used = 0;
-    for (int p0 = 0; p0 < R.n_pages; p0 += EACH * PLAN) {
+    int ref[LOOK], of[LOOK], n = 0;
+    bool is[LOOK];
+    for (int p0 = 0; p0 < R.n_pages; p0 += LOOK * PLAN) {
+        look_at(R, p0, ref);
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const int p = p0 + PLAN * e + tid;
-            used += p < R.n_pages && R.refs[p] != 0;
-        }
+        for (int e = 0; e < LOOK; e++) is[e] = ref[e] != 0;
+        n += ranks<LOOK>(is, part, of);
     }
-    int n;
-    block_scan(used, part, n);
     if (tid == 0 && n_used) *n_used = n;
+    const bool once = R.n_pages <= LOOK * PLAN;  // ref holds all counts
     int holes = 0;
-    for (int p0 = 0; p0 < n; p0 += EACH * PLAN) {
-        bool hole[EACH];
-        int c = 0, total;
+    for (int p0 = 0; p0 < n; p0 += LOOK * PLAN) {
+        if (!once) look_at(R, p0, ref);
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const int p = p0 + EACH * tid + e;
-            hole[e] = p < n && R.refs[p] == 0;
-            c += hole[e];
-            if (p < n) new_ids[p] = hole[e] ? -1 : p;
+        for (int e = 0; e < LOOK; e++) is[e] = p0 + numbered<LOOK>(e) < n && ref[e] == 0;
+        const int total = ranks<LOOK>(is, part, of);
+#pragma unroll
+        for (int e = 0; e < LOOK; e++) {
+            const int p = p0 + numbered<LOOK>(e);
+            if (is[e]) {
+                moves->dst[holes + of[e]] = p;
+                if (once) list[of[e]] = p;
+            }
+            if (p < n) new_ids[p] = is[e] ? -1 : p;
         }
-        int at = holes + block_scan(c, part, total);
-#pragma unroll
-        for (int e = 0; e < EACH; e++)
-            if (hole[e]) moves->dst[at++] = p0 + EACH * tid + e;
         holes += total;
     }
-    __threadfence();
-    __syncthreads();
+    if (once) __syncthreads();
+    else arrived();
     int moved = 0;
-    for (int p0 = n; p0 < R.n_pages; p0 += EACH * PLAN) {
-        int ref[EACH], c = 0, total;
+    for (int p0 = once ? 0 : n; p0 < R.n_pages; p0 += LOOK * PLAN) {
+        if (!once) look_at(R, p0, ref);
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const int p = p0 + EACH * tid + e;
-            ref[e] = p < R.n_pages ? R.refs[p] : 0;
-            c += ref[e] != 0;
-        }
-        int at = moved + block_scan(c, part, total);
+        for (int e = 0; e < LOOK; e++) is[e] = p0 + numbered<LOOK>(e) >= n && ref[e] != 0;
+        const int total = ranks<LOOK>(is, part, of);
+        int to[LOOK];
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const int p = p0 + EACH * tid + e;
-            int to = -1;
-            if (ref[e]) {
-                to = seen(moves->dst + at);
-                moves->src[at++] = p;
-                R.refs[to] = ref[e];
+        for (int e = 0; e < LOOK; e++) to[e] = !is[e] ? -1 : once ? list[of[e]] : seen(moves->dst + moved + of[e]);
+#pragma unroll
+        for (int e = 0; e < LOOK; e++) {
+            const int p = p0 + numbered<LOOK>(e);
+            if (is[e]) {
+                moves->src[moved + of[e]] = p;
+                R.refs[to[e]] = ref[e];
                 R.refs[p] = 0;
             }
-            if (p < R.n_pages) new_ids[p] = to;
+            if (p >= n && p < R.n_pages) new_ids[p] = to[e];
         }
         moved += total;
     }
     if (tid == 0) moves->count = moved;
 }
 
-__global__ __launch_bounds__(256) void k_kv_rename(KvTable t, const int32_t *new_ids, int n_pages) {
-    const unsigned at = blockIdx.x * 256 + threadIdx.x;
-    if (at >= t.entries()) return;
-    const int p = t.pages[at];
-    if ((unsigned)p < (unsigned)n_pages) t.pages[at] = new_ids[p];
-}
-
 dim3 over_entries(const KvTable &t) { return dim3((unsigned)((t.entries() + 255) / 256)); }
-constexpr size_t COPY_BLOCKS = 4096;
+constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256, FRONT_BLOCKS = 512;
+
+void copy_pages(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, const int32_t *count, int n,
+                const KvTable &t, const int32_t *new_ids, hipStream_t s) {
+    const size_t bytes = ((size_t)from.heads << from.lg_b) * KV_BLOCK * d_head, pieces = (bytes + PIECE - 1) / PIECE;
+    const size_t renaming = std::min(RENAME_BLOCKS, (t.entries() + 255) / 256);
+    const dim3 g((unsigned)(std::min(COPY_BLOCKS, std::max((size_t)1, (size_t)n * 2 * pieces)) + renaming));
+    hipLaunchKernelGGL(k_kv_copy, g, dim3(256), 0, s, from, to, bytes, (int)pieces, src, dst, count, n, t, new_ids, (unsigned)renaming);
+}
 
 }  // namespace
 
 size_t kv_pages_bytes() { return std::max(sizeof(Room), sizeof(Moves)); }
 
-static void copy_pages(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, const int32_t *count, int n,
-                       hipStream_t s) {
-    const size_t bytes = ((size_t)from.heads << from.lg_b) * KV_BLOCK * d_head, pieces = (bytes + PIECE - 1) / PIECE;
-    const dim3 g((unsigned)std::max((size_t)1, std::min(COPY_BLOCKS, (size_t)n * 2 * pieces)));
-    hipLaunchKernelGGL(k_kv_copy, g, dim3(256), 0, s, from, to, bytes, (int)pieces, src, dst, count, n);
-}
-
 hipError_t launch_kv_copy(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, int n, hipStream_t s) {
-    copy_pages(from, to, d_head, src, dst, nullptr, n, s);
+    copy_pages(from, to, d_head, src, dst, nullptr, n, {nullptr, 0, 0}, nullptr, s);
     return hipGetLastError();
 }
 
@@ -346,7 +485,7 @@ hipError_t launch_kv_reserve(const KvPool &pool, const KvRows &rows, int d_head,
     Room *r = static_cast<Room *>(room);
     hipLaunchKernelGGL(k_kv_reserve, dim3(1), dim3(PLAN), 0, s, rows, pool.lg_b + 4, pages, KvRefs{refs, pool.n_pages}, missing, r);
     if (!rows.n_rows || !rows.cap) return hipGetLastError();
-    const dim3 g((unsigned)std::min((size_t)2048, (size_t)rows.n_seqs * pool.heads * 2));
+    const dim3 g((unsigned)std::min(FRONT_BLOCKS, (size_t)rows.n_seqs * pool.heads * 2));
     hipLaunchKernelGGL(k_kv_copy_fronts, g, dim3(256), 0, s, pool, d_head, r);
     return hipGetLastError();
 }
@@ -355,8 +494,7 @@ hipError_t launch_kv_compact(const KvPool &pool, int d_head, const KvTable &t, i
                              void *room, hipStream_t s) {
     Moves *m = static_cast<Moves *>(room);
     hipLaunchKernelGGL(k_kv_compact, dim3(1), dim3(PLAN), 0, s, KvRefs{refs, pool.n_pages}, new_ids, n_used, m);
-    copy_pages(pool, pool, d_head, m->src, m->dst, &m->count, pool.n_pages / 2, s);
-    if (t.entries()) hipLaunchKernelGGL(k_kv_rename, over_entries(t), dim3(256), 0, s, t, new_ids, pool.n_pages);
+    copy_pages(pool, pool, d_head, m->src, m->dst, &m->count, pool.n_pages / 2, t, new_ids, s);
     return hipGetLastError();
 }
 
