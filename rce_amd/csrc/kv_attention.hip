@@ -93,14 +93,14 @@ struct Args {
     int vec;        // query rows (1) and rotation table (2) can be read, output rows (4) written 16 bytes at a time
 };
 
-// The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one,
-// numbers t0 .. t0 + tiles - 1.
+// The units of a sequence (per kv head; 0 where it is not of the part) and the tiles of its longest one: t0 .. t0 + tiles - 1.
 //
-// Sinks: the tiles of the first positions stand in front of the window's.  Tile number t from `own` on is the tile of
-// positions 64 t .., a number below it is a tile from the sequence's beginning (0 for t0), as many as the
-// sinks reach into and the window does not.
+// With sinks a range is cut from what a unit visits, not from the positions: a list of the blocks of 16 positions that the
+// sinks reach into (as far as its window does not) and its window's, four of them a tile, number 0 ..; `tiles` is what the
+// sequence's longest unit can come to.  Blocks and not tiles of 64 positions stand in a row: 4 sinks and a window of 1024 of 32 tokens
+// are 17 tiles, not 18.5 (2 prompts of up to 6000, 338 -> 328 us).
 struct Span {
-    int units, t0, tiles, own;
+    int units, t0, tiles;
 };
 template <bool SINKS>
 __device__ __forceinline__ Span span_of(const Args &A, const KvSeq &q) {
@@ -108,38 +108,39 @@ __device__ __forceinline__ Span span_of(const Args &A, const KvSeq &q) {
     const int x = (q.r1 - q.r0) * A.G;
     s.units = x >= A.lo_x && x <= A.hi_x ? (x + A.rows - 1) / A.rows : 0;
     const int lo = max(0, q.lo() - (A.a.window - 1));
-    s.own = lo / TILE;
-    s.t0 = SINKS ? s.own - min(s.own, (A.a.sinks + TILE - 1) / TILE) : s.own;
+    s.t0 = lo / TILE;
     s.tiles = q.hi(A.B) > q.lo() ? (q.hi(A.B) + TILE - 1) / TILE - s.t0 : 0;
+    if constexpr (SINKS) {
+        if (s.tiles) {
+            // a unit's tokens stand in a row, their windows span that many positions together
+            const int tokens = min(q.r1 - q.r0, (A.rows - 1) / A.G + 2);
+            const int own = (int)(((int64_t)A.a.window + tokens - 2) / KV_BLOCK) + 2, reach = (A.a.sinks + KV_BLOCK - 1) / KV_BLOCK;
+            s.tiles = min(s.t0 + s.tiles, (own + reach + 3) / 4);
+        }
+        s.t0 = 0;
+    }
     return s;
 }
 
-// The tiles that a unit visits of its range [w_lo, w_hi) of tile numbers: those that sinks reach into, then the window's, numbers
-// `lo` .. `hi` - 1.  Without sinks the numbers are the tiles.
+// The tiles that a unit visits of its range [w_lo, w_hi); its window reaches into the positions p_lo .. p_hi - 1.
 template <bool SINKS>
 struct Visits {
-    int lo, hi;
-    int n_front, front, back, own, t0;  // SINKS: visit i < n_front is number front + i, the others back + i
-    __device__ Visits(const Args &A, const Span &p, int w_lo, int w_hi, int u_lo, int u_hi) {
+    int lo, hi, front, back;  // block i of the list is block i below `front`, else i + back
+    __device__ Visits(const Args &A, int w_lo, int w_hi, int p_lo, int p_hi) {
         if constexpr (SINKS) {
-            own = p.own;
-            t0 = p.t0;
-            const int end = min(w_hi, u_hi), reach = min(end, max(own, (A.a.sinks + TILE - 1) / TILE));
-            front = w_lo;
-            n_front = max(0, reach - w_lo);
-            const int from = max(max(w_lo, reach), u_lo);
-            back = from - n_front;
-            lo = 0;
-            hi = n_front + max(0, end - from);
+            const int first = p_lo / KV_BLOCK, end = (p_hi + KV_BLOCK - 1) / KV_BLOCK;
+            front = min(min((A.a.sinks + KV_BLOCK - 1) / KV_BLOCK, first), end);
+            back = first - front;
+            lo = w_lo;
+            hi = min(w_hi, (front + max(0, end - first) + 3) / 4);
         } else {
-            lo = max(u_lo, w_lo);
-            hi = min(u_hi, w_hi);
+            lo = max(p_lo / TILE, w_lo);
+            hi = min((p_hi + TILE - 1) / TILE, w_hi);
         }
     }
-    __device__ __forceinline__ int tile(int i) const {
-        if constexpr (!SINKS) return i;
-        const int t = i + (i < n_front ? front : back);
-        return t < own ? t - t0 : t;
+    __device__ __forceinline__ int block(int t, int b) const {  // block b of tile t
+        if constexpr (!SINKS) return 4 * t + b;
+        return 4 * t + b + (4 * t + b < front ? 0 : back);
     }
 };
 // The cells of a unit in the line (below): its prologue's, then one per tile, one if it has none.
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
         const int u_tok0 = x0 / G, u_tok1 = (x0 + n_x - 1) / G;
         const int u_hi = min(A.B.cap - 1, first + u_tok1), u_first = first + u_tok0;
         const int all_lo = max(0, max(0, u_hi) - (A.a.window - 1)), all_hi = u_first;  // seen by every row (if all have positions)
-        const Visits<SINKS> visit(A, w.sp, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, u_hi < 0 ? 0 : u_hi / TILE + 1);
+        const Visits<SINKS> visit(A, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)), max(u_hi + 1, 0));
         const bool placed = u_first >= 0 && first + u_tok1 < A.B.cap;  // every row has a position
         const int32_t *pages = A.B.pages + (size_t)w.seq * A.B.max_pages;
         const int bmask = (1 << A.P.lg_b) - 1;
@@ -496,11 +497,10 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
 #pragma unroll
         for (int i = 0; i < NT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
-        for (int i_t = visit.lo + wave; i_t < visit.hi; i_t += WAVES) {
-            const int t = visit.tile(i_t);
+        for (int t = visit.lo + wave; t < visit.hi; t += WAVES) {
             // the K block of this lane's operand rows, the block of its scores
             const int max_block = A.B.cap / KV_BLOCK - 1;
-            const int kb = min(4 * t + (n >> 2), max_block), vb = min(4 * t + g, max_block);
+            const int kb = min(visit.block(t, n >> 2), max_block), vb = min(visit.block(t, g), max_block);
             const int kp = pages[kb >> A.P.lg_b], vp = pages[vb >> A.P.lg_b];
             const bool k_ok = (unsigned)kp < (unsigned)A.P.n_pages, v_ok = (unsigned)vp < (unsigned)A.P.n_pages;
             const size_t kblk = (((size_t)(k_ok ? kp : 0) * A.P.heads + h) << A.P.lg_b) + (kb & bmask);
@@ -538,13 +538,15 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
                 }
             }
             const float f = sk * qs;
-            const bool full = placed && (TILE * t >= all_lo || (SINKS && TILE * t + TILE <= A.a.sinks)) && TILE * t + TILE - 1 <= all_hi;  // the same in all lanes
+            // the tile's first and last position; the same in all lanes
+            const int p0 = KV_BLOCK * visit.block(t, 0), p1 = KV_BLOCK * visit.block(t, 3) + KV_BLOCK - 1;
+            const bool full = placed && (p0 >= all_lo || (SINKS && p1 < A.a.sinks)) && p1 <= all_hi;
             const bool masked = !full || __ballot(!v_ok) != 0;
             if (masked) {
                 bool any = false;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const int p = TILE * t + 16 * g + j;
+                    const int p = KV_BLOCK * visit.block(t, g) + j;
                     const bool see = v_ok && (p >= p_lo || (SINKS && p < A.a.sinks)) && p <= p_hi;
                     any |= see;
                     x[j] = see ? x[j] * f : -INFINITY;
@@ -669,6 +671,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
 // the LDS reads per product).
 constexpr int P_ROWS = 128, P_WAVES = 8;
 constexpr float LAG = 6.0f, UP = 512.0f;  // UP = 2^9
+constexpr int UNSEEN = -(1 << 30);  // scores of two limbs are above -2^30 (256 dimensions: 256 * 127 * 2^14)
 
 // A lane's accumulators times f: four consecutive values every 16 from value index i; vec:
 // at multiples of their size.
@@ -745,7 +748,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int all_lo = max(0, max(0, f1) - (A.a.window - 1)), all_hi = f0;
     // the block's tiles
     const int u_first = first + x0 / G, u_hi = min(A.B.cap - 1, first + (x0 + n_x - 1) / G);
-    const Visits<SINKS> visit(A, w.sp, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)) / TILE, u_hi < 0 ? 0 : u_hi / TILE + 1);
+    const Visits<SINKS> visit(A, w.t_lo, w.t_hi, max(0, max(u_first, 0) - (A.a.window - 1)), max(u_hi + 1, 0));
     const int t_lo = visit.lo, t_hi = visit.hi;
     const int32_t *__restrict__ pages = page_table + (size_t)w.seq * A.B.max_pages;
     const int bmask = (1 << A.P.lg_b) - 1, max_block = A.B.cap / KV_BLOCK - 1;
@@ -759,7 +762,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     float ksr = 0.0f, vsr = 0.0f;
     int pg[NK], pgs = 0, oks = 0;  // the next tile's page ids, loaded a tile ahead
     auto mine = [&](int i) { return 4 * BP % (64 * P_WAVES) == 0 || wave * 64 + 64 * P_WAVES * i < 4 * BP; };  // the same in a wave
-    auto block_of = [&](int t, int b) { return min(4 * t + b, max_block); };
+    auto block_of = [&](int t, int b) { return min(visit.block(t, b), max_block); };
     auto look = [&](int t) {
 #pragma unroll
         for (int i = 0; i < NK; i++)
@@ -823,19 +826,19 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int k_pos = 16 * (n >> 2) + (n & 3);
     const int k_row0 = k_pos * D + key_piece<D>(k_pos, g) * 16, v_row0 = n * TILE + (2 * g ^ (n & 7)) * 8;
     if (t_lo < t_hi) {
-        look(visit.tile(t_lo));
-        fetch(visit.tile(t_lo));
-        look(visit.tile(t_lo + 1));
+        look(t_lo);
+        fetch(t_lo);
+        look(t_lo + 1);
         place(buf[0]);
-        if (t_lo + 1 < t_hi) fetch(visit.tile(t_lo + 1));
-        look(visit.tile(t_lo + 2));
+        if (t_lo + 1 < t_hi) fetch(t_lo + 1);
+        look(t_lo + 2);
     }
     __syncthreads();
-    for (int i_t = t_lo; i_t < t_hi; i_t++) {
-        const PShared<D> &sh = buf[(i_t - t_lo) & (BUFS - 1)];
-        const int t = visit.tile(i_t);
-        if (TILE * t <= w_hi && (TILE * t + TILE - 1 >= w_lo || (SINKS && TILE * t < A.a.sinks))) {  // some row of the wave sees it (the same in all lanes)
-            const bool full = placed && (TILE * t >= all_lo || (SINKS && TILE * t + TILE <= A.a.sinks)) && TILE * t + TILE - 1 <= all_hi;
+    for (int t = t_lo; t < t_hi; t++) {
+        const PShared<D> &sh = buf[(t - t_lo) & (BUFS - 1)];
+        const int p0 = KV_BLOCK * visit.block(t, 0), p1 = KV_BLOCK * visit.block(t, 3) + KV_BLOCK - 1;  // its first and last position
+        if (p0 <= w_hi && (p1 >= w_lo || (SINKS && p0 < A.a.sinks))) {  // some row of the wave sees it (the same in all lanes)
+            const bool full = placed && (p0 >= all_lo || (SINKS && p1 < A.a.sinks)) && p1 <= all_hi;
             const bool masked = !full || !(sh.ok[0] & sh.ok[1] & sh.ok[2] & sh.ok[3]);
             // opaque: what is formed from them would be kept over the loop, in registers that spill
             int k_row = k_row0, v_row = v_row0;
@@ -868,7 +871,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
             uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
             if (HILO || masked) {
                 if (masked) {
-                    const int p = TILE * t + 16 * g, lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
+                    const int p = KV_BLOCK * visit.block(t, g), lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
                     seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
                     if constexpr (SINKS) {
                         const int last = min(hi, A.a.sinks - 1 - p);
@@ -877,8 +880,20 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                     if (!seen) sv = 0.0f;  // as in k_kv_attention
                 }
                 asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
+                if constexpr (SINKS && !HILO) {
+                    // what a row does not see is below all that it sees; a row that sees nothing has no score
+                    int x = UNSEEN;
 #pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+                    for (int e = 0; e < 16; e++) {
+                        const int is = (int)(seen << (31 - e)) >> 31;
+                        xi[e] = (xi[e] & is) | (UNSEEN & ~is);
+                        x = max(x, xi[e]);
+                    }
+                    top = seen ? (float)x * f : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+                }
             } else {
                 int x = xi[0];
 #pragma unroll
@@ -922,6 +937,16 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                     ph[e >> 3][e & 7] = (_Float16)p;
                 }
                 l = __builtin_fmaf(sum, exp2_(-lw), l);
+            } else if constexpr (SINKS && !HILO) {  // xi is UNSEEN where the row does not see it: the weight is taken out
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int is = (int)(seen << (31 - e)) >> 31;
+                    const float y = __int_as_float(__float_as_int(exp2_(__builtin_fmaf((float)xi[e], f, -base))) & is);
+                    sum += y;
+                    ph[e >> 3][e & 7] = (_Float16)__int_as_float(__float_as_int(y * pw) & is);
+                }
+                l += sum;
             } else {
                 float sum = 0.0f;
 #pragma unroll
@@ -945,10 +970,10 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
                 }
         }
         if constexpr (BUFS == 1) __syncthreads();
-        if (i_t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
-            place(buf[(i_t + 1 - t_lo) & (BUFS - 1)]);
-            if (i_t + 2 < t_hi) fetch(visit.tile(i_t + 2));
-            look(visit.tile(i_t + 3));
+        if (t + 1 < t_hi) {  // the next tile to the other buffer, the one after it on its way
+            place(buf[(t + 1 - t_lo) & (BUFS - 1)]);
+            if (t + 2 < t_hi) fetch(t + 2);
+            look(t + 3);
         }
         __syncthreads();
     }
@@ -1073,9 +1098,9 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
     if (!rows.n_rows) return hipSuccess;
     const int G = a.n_q / pool.heads;
     const size_t x = (size_t)rows.n_rows * G;
-    // positions that the tiles of a sequence span at most: with sinks the window's and theirs (a sequence's rows are n_rows at most)
-    const int64_t span = a.sinks ? std::min((int64_t)rows.cap, TILE * (((int64_t)a.sinks + TILE - 1) / TILE + ((int64_t)a.window + rows.n_rows) / TILE + 2))
-                                 : (int64_t)rows.cap;
+    // positions that the tiles of a sequence span at most; with sinks its longest unit's (a sequence's rows are n_rows at most)
+    const int64_t reach = (a.sinks + KV_BLOCK - 1) / KV_BLOCK, own = ((int64_t)a.window + rows.n_rows) / KV_BLOCK + 2;
+    const int64_t span = a.sinks ? std::min((int64_t)rows.cap, TILE * ((reach + own + 3) / 4)) : (int64_t)rows.cap;
     auto go = [&](auto d, auto with_sinks) {
         constexpr int D = decltype(d)::value;
         constexpr bool SINKS = decltype(with_sinks)::value;

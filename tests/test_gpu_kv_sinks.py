@@ -184,6 +184,17 @@ def test_long_prompt_among_tokens(ctx):
     r.free()
 
 
+@pytest.mark.parametrize("lens,news,page", [([237, 250], [10, 12], 128), ([256], [200], 64), ([1020, 1000], [1, 1], 1024), ([1024, 500], [3, 3], 512)])
+def test_tables_as_long_as_the_keys(ctx, lens, news, page):
+    """Windows and sinks that together pass what the table spans: units of no more tiles than positions, none split where
+    the call has no join."""
+    rng = np.random.default_rng(len(lens) + page)
+    r = Run(ctx, rng, lens, news, page, 1, 8, 64, G.F16, G.F16, rope=64)
+    for window, sinks in ((983, 4), (200, 200), (5000, 64), (150, 17), (lens[0], lens[0])):
+        r.check(window, sinks, rows={0, news[0] - 1, news[0], sum(news) - 1})
+    r.free()
+
+
 def test_strides_of_queries(ctx):
     rng = np.random.default_rng(7)
     for gap in (1, 64):
