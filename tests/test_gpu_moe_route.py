@@ -127,6 +127,36 @@ def test_odd_rows(ctx, experts, how, bias):
             check(ctx, lg, dtype, how, bias=b)
 
 
+MANY = 10003  # tokens of a call from which several share a wave, and an odd rest
+
+
+@pytest.mark.parametrize("experts,how", [(9, dict(top_k=2)), (60, dict(top_k=4, sigmoid=True)), (64, dict(top_k=16)), (64, dict(top_k=6, groups=8, kept=3)),
+                                         (100, dict(top_k=5, normalize=False)), (128, dict(top_k=8, groups=4, kept=2, group_top=2, sigmoid=True)),
+                                         (160, dict(top_k=6, groups=10, kept=4)), (160, dict(top_k=6, groups=8, kept=3, group_top=2)), (256, dict(top_k=8, sigmoid=True)),
+                                         (256, dict(top_k=8, groups=8, kept=4, group_top=2, sigmoid=True)), (256, dict(top_k=1, groups=2, kept=1, group_top=2)),
+                                         (256, dict(top_k=12, groups=16, kept=5, normalize=False)), (250, dict(top_k=3)), (200, dict(top_k=2, groups=5, kept=2))])
+@pytest.mark.parametrize("bias", [None, "some", "odd", "wide"])
+def test_many_tokens(ctx, experts, how, bias):
+    """Rows of all sorts among ordinary ones; strides that are whole words, and not; biases far beyond the scores."""
+    print(f"route many experts={experts} {how} bias={bias}", flush=True)
+    rng = np.random.default_rng(experts)
+    lg = (rng.standard_normal((MANY, experts)) * 2).astype(F32)
+    lg[100:114], lg[-14:] = odd_rows(rng, experts), odd_rows(rng, experts)
+    lg[500:700] = np.round(lg[500:700] * 4) / 4  # equals in every row
+    b = None
+    if bias:
+        b = (rng.standard_normal(experts) * (3 if bias == "wide" else 0.3)).astype(F32)
+        if bias == "odd":
+            b[:5] = np.nan, -np.inf, np.inf, 1e30, -1e30
+    at = np.concatenate([np.arange(90, 120), rng.integers(0, MANY, 100), np.arange(500, 540), np.arange(MANY - 20, MANY)])
+    for i, dtype in enumerate((G.F32, G.BF16, G.F16)):
+        bits = kc.to_bits(lg, dtype)
+        ids, w = run(ctx, bits, dtype, how, stride=experts + (3, 0, 4)[i], bias=b)
+        want_ids, want = sc.route(kc.widen(bits[at], dtype), bias=b, **how)
+        assert np.array_equal(ids[at], want_ids), np.argwhere(ids[at] != want_ids)[:5]
+        assert np.all(np.abs(w[at] - want) <= WEIGHT * np.abs(want) + 2.0 ** -150)
+
+
 def test_scores_next_to_each_other(ctx):
     """Scores that 32 bits hold as equals, a bias apart: 1 - 2^-26 against 1 - 2^-27 by the sigmoid, and by the
     softmax two logits that differ by 2^-23 under a bias of 1000."""
@@ -134,6 +164,18 @@ def test_scores_next_to_each_other(ctx):
     check(ctx, lg, G.F32, dict(top_k=1, sigmoid=True), bias=np.zeros(8, F32))
     lg = np.array([[0.5, 0.5 + 2.0 ** -23, 0, 0], [0.5 + 2.0 ** -23, 0.5, 0, 0]], F32)
     check(ctx, lg, G.F32, dict(top_k=1), bias=np.array([1000, 1000, 0, 0], F32))
+    # among many tokens, and of many experts: the first two a step of the last bit apart, either way round
+    for e, n in ((16, 10002), (100, 9), (256, 10002), (256, 9)):
+        rng = np.random.default_rng(e)
+        lg = (rng.standard_normal((n, e)) * 0.3).astype(F32)
+        up, down = F32(3), np.nextafter(F32(3), F32(0))
+        lg[::2, e // 2], lg[::2, e // 3] = up, down
+        lg[1::2, e // 2], lg[1::2, e // 3] = down, up
+        for bias in (None, np.full(e, 0.5, F32)):
+            at = np.arange(0, n, max(1, n // 40))
+            for how in (dict(top_k=2, sigmoid=True), dict(top_k=1)):
+                ids, _ = run(ctx, lg, G.F32, how, bias=bias)
+                assert np.array_equal(ids[at], sc.route(lg[at], bias=bias, **how)[0])
 
 
 def test_a_wide_call(ctx):
