@@ -78,6 +78,10 @@ constexpr int FEW = 32;       // query rows per kv head up to which a sequence i
 // LONG: 16 sequences of 5 drafts in long tables are spared the launch (4 us of 27).
 constexpr int LONG = 1536, LONG_TILES = 48;
 
+// With sinks no unit visits more tiles than a window's.  Up to SHORT of them a few sequences have one part (a long one is there: units of few rows
+// take no longer than its), and units that are TARGET and more are not split: 3 x 500 rows after 9000, a window of 2048: 125 -> XX us.
+constexpr int SHORT = 64;
+
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -1139,6 +1143,8 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         };
         auto many = [&](int lo) {
             Args A{pool, rows, a, G, P_ROWS, lo, INT_MAX, target(MANY_PARTS, P_ROWS), P_MIN_CHUNK, 0, vec};
+            // units of much the same length, enough of them: none is split
+            if (SINKS && span <= SHORT * TILE && x / P_ROWS * pool.heads >= (size_t)A.target) A.min_chunk = WHOLE;
             A.a.parts += FEW_PARTS / sizeof(float);
             const dim3 g = grid(A, units(A, INT_MAX)), b(64 * P_WAVES);
             if (f32) hipLaunchKernelGGL((k_kv_prompt<D, true, SINKS>), g, b, 0, s, A, rows.pages);
@@ -1148,7 +1154,7 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         const bool prompt = more >= (size_t)LONG &&
                             (double)more / ROWS * (span / TILE) * pool.heads >= (double)LONG_TILES * TARGET;
         if (x > (size_t)FEW * rows.n_seqs || prompt) {
-            const bool one = rows.n_seqs == 1 && span <= ONE_TABLE * TILE;
+            const bool one = (rows.n_seqs == 1 && span <= ONE_TABLE * TILE) || (SINKS && rows.n_seqs <= 16 && span <= SHORT * TILE);
             many(one ? 0 : FEW + 1);
             if (!one) few(FEW);
         } else {

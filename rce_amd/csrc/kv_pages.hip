@@ -123,7 +123,20 @@ __device__ __forceinline__ int ranks(const bool (&is)[N], int *part, int (&of)[N
 template <int N>
 __device__ __forceinline__ int numbered(int e) { return 64 * (N * (threadIdx.x >> 6) + e) + (threadIdx.x & 63); }
 
-__global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int32_t *pages, KvRefs R, int32_t *missing, Room *room) {
+// A front's head h and kind (0 keys, 1 values): thread i of n.
+__device__ __forceinline__ void copy_front(const KvPool &P, int d, const Front &f, int h, int kind, int i, int n) {
+    const size_t a = ((size_t)f.src * P.heads + h) << P.lg_b, b = ((size_t)f.dst * P.heads + h) << P.lg_b;
+    int8_t *codes = kind ? P.v : P.k;
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(codes + a * (KV_BLOCK * d));
+    u32x4 *to = reinterpret_cast<u32x4 *>(codes + b * (KV_BLOCK * d));
+#pragma unroll 4
+    for (int j = i; j < f.blocks * d; j += n) to[j] = from[j];
+    float *scale = kind ? P.v_scale : P.k_scale;
+    for (int j = i; j < f.blocks; j += n) scale[b + j] = scale[a + j];
+}
+
+// d: 0, or the head size where the block copies the fronts itself.
+__global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int32_t *pages, KvRefs R, int32_t *missing, Room *room, KvPool P, int d) {
     __shared__ int part[PLAN / 64], start[PLAN + 1], slot0[PLAN], front0[PLAN], lost[PLAN], ring[RING];
     __shared__ int n_fronts;
     int *const key = ring, *const asked = ring + SLOTS, *const first_ask = ring + 2 * SLOTS;  // before the ring is used
@@ -191,6 +204,19 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
         return s;
     };
 
+    auto copy = [&] {  // the fronts, or their number for the next kernel
+        if (!d) {
+            __syncthreads();
+            if (tid == 0) room->n_fronts = n_fronts;
+            return;
+        }
+        arrived();
+        for (int u = tid >> 6; u < n_fronts * P.heads * 2; u += PLAN / 64) {
+            const int *p = &room->fronts[(u >> 1) / P.heads].src;
+            copy_front(P, d, {seen(p), seen(p + 1), seen(p + 2), 0}, (u >> 1) % P.heads, u & 1, tid & 63, 64);
+        }
+    };
+
     if (tid == 0) n_fronts = 0;
     lost[tid] = 0;
 #pragma unroll
@@ -230,9 +256,8 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
             if (leaves) atomicSub(R.refs + p, 1);
             if (!give(s, slot, rank, p, leaves)) atomicAdd(lost + s, 1);
         }
-        __syncthreads();
+        copy();
         if (missing && tid < B.n_seqs) missing[tid] = lost[tid];
-        if (tid == 0) room->n_fronts = n_fronts;
         return;
     }
 
@@ -321,24 +346,14 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
         have -= used;
         __syncthreads();  // the ring's places are read
     });
-    __syncthreads();
-    if (tid == 0) room->n_fronts = n_fronts;
+    copy();
 }
 
 // A block takes a front's head and kind (keys, values), every block of the grid the next ones.
 __global__ __launch_bounds__(256) void k_kv_copy_fronts(KvPool P, int d, const Room *room) {
     const int n = room->n_fronts * P.heads * 2;
-    for (int u = blockIdx.x; u < n; u += gridDim.x) {
-        const int kind = u & 1, h = (u >> 1) % P.heads;
-        const Front f = room->fronts[(u >> 1) / P.heads];
-        const size_t a = ((size_t)f.src * P.heads + h) << P.lg_b, b = ((size_t)f.dst * P.heads + h) << P.lg_b;
-        int8_t *codes = kind ? P.v : P.k;
-        const u32x4 *from = reinterpret_cast<const u32x4 *>(codes + a * (KV_BLOCK * d));
-        u32x4 *to = reinterpret_cast<u32x4 *>(codes + b * (KV_BLOCK * d));
-        for (int i = threadIdx.x; i < f.blocks * d; i += 256) to[i] = from[i];
-        float *scale = kind ? P.v_scale : P.k_scale;
-        for (int i = threadIdx.x; i < f.blocks; i += 256) scale[b + i] = scale[a + i];
-    }
+    for (int u = blockIdx.x; u < n; u += gridDim.x)
+        copy_front(P, d, room->fronts[(u >> 1) / P.heads], (u >> 1) % P.heads, u & 1, threadIdx.x, 256);
 }
 
 // ---- whole pages ------------------------------------------------------------
@@ -452,6 +467,7 @@ __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids,
 }
 
 dim3 over_entries(const KvTable &t) { return dim3((unsigned)((t.entries() + 255) / 256)); }
+constexpr size_t OWN_COPY = (size_t)128 << 10;  // bytes that the planning block copies itself: 4 beams of 4 heads of 64, whole pass with fork and release 17.1 -> 13.8 us
 constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256, FRONT_BLOCKS = 512;
 
 void copy_pages(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, const int32_t *count, int n,
@@ -484,8 +500,11 @@ hipError_t launch_kv_release(const KvTable &t, int page_tokens, const int32_t *f
 hipError_t launch_kv_reserve(const KvPool &pool, const KvRows &rows, int d_head, int32_t *pages, int32_t *refs, int32_t *missing,
                              void *room, hipStream_t s) {
     Room *r = static_cast<Room *>(room);
-    hipLaunchKernelGGL(k_kv_reserve, dim3(1), dim3(PLAN), 0, s, rows, pool.lg_b + 4, pages, KvRefs{refs, pool.n_pages}, missing, r);
-    if (!rows.n_rows || !rows.cap) return hipGetLastError();
+    // what the fronts come to at most: a page per sequence
+    const bool small = ((size_t)rows.n_seqs * pool.heads * 2 << pool.lg_b) * KV_BLOCK * d_head <= OWN_COPY;
+    hipLaunchKernelGGL(k_kv_reserve, dim3(1), dim3(PLAN), 0, s, rows, pool.lg_b + 4, pages, KvRefs{refs, pool.n_pages}, missing, r, pool,
+                       small ? d_head : 0);
+    if (!rows.n_rows || !rows.cap || small) return hipGetLastError();
     const dim3 g((unsigned)std::min(FRONT_BLOCKS, (size_t)rows.n_seqs * pool.heads * 2));
     hipLaunchKernelGGL(k_kv_copy_fronts, g, dim3(256), 0, s, pool, d_head, r);
     return hipGetLastError();

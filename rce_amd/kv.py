@@ -31,11 +31,15 @@ _HEADS = struct.Struct("@PNPNPN")
 _SCALING = struct.Struct("@ffPNff")
 
 
+def _range(e: struct.error) -> QmmError:
+    return QmmError(2, f"an address or a size is out of range: {e}")
+
+
 def _pack(fmt: struct.Struct, *values: int) -> bytes:
     try:
         return fmt.pack(*values)
     except struct.error as e:
-        raise QmmError(2, f"an address or a size is out of range: {e}") from None
+        raise _range(e) from None
 
 
 class KvCache:
@@ -46,7 +50,10 @@ class KvCache:
 
     def __init__(self, n_pages: int, page_tokens: int, n_kv_heads: int, d_head: int, k: int = 0, v: int = 0,
                  k_scale: int = 0, v_scale: int = 0):
-        self.raw = _pack(_CACHE, k, v, k_scale, v_scale, n_pages, page_tokens, n_kv_heads, d_head)
+        try:
+            self.raw = _CACHE.pack(k, v, k_scale, v_scale, n_pages, page_tokens, n_kv_heads, d_head)
+        except struct.error as e:
+            raise _range(e) from None
         self.d_head = d_head
         self.buffers: tuple = ()
 
@@ -85,7 +92,10 @@ class KvBatch:
     __slots__ = ("raw",)
 
     def __init__(self, row_offsets: int, seq_lens: int, pages: int, n_seqs: int, n_rows: int, max_pages: int):
-        self.raw = _pack(_BATCH, row_offsets, seq_lens, pages, n_seqs, n_rows, max_pages)
+        try:
+            self.raw = _BATCH.pack(row_offsets, seq_lens, pages, n_seqs, n_rows, max_pages)
+        except struct.error as e:
+            raise _range(e) from None
 
 
 class Rope:
@@ -94,7 +104,10 @@ class Rope:
     __slots__ = ("raw", "buffer")
 
     def __init__(self, cs: int, dim: int, n_pos: int):
-        self.raw = _pack(_ROPE, cs, dim, n_pos)
+        try:
+            self.raw = _ROPE.pack(cs, dim, n_pos)
+        except struct.error as e:
+            raise _range(e) from None
         self.buffer: DeviceBuffer | None = None
 
     @staticmethod
@@ -142,7 +155,10 @@ class KvTable:
     __slots__ = ("raw",)
 
     def __init__(self, pages: int, n_seqs: int, max_pages: int):
-        self.raw = _pack(_TABLE, pages, n_seqs, max_pages)
+        try:
+            self.raw = _TABLE.pack(pages, n_seqs, max_pages)
+        except struct.error as e:
+            raise _range(e) from None
 
 
 class Heads:
@@ -152,7 +168,10 @@ class Heads:
     __slots__ = ("raw",)
 
     def __init__(self, in_dev: int, in_stride: int, n_heads: int, out_dev: int, out_stride: int, weight: int = 0):
-        self.raw = _pack(_HEADS, in_dev, in_stride, out_dev, out_stride, weight, n_heads)
+        try:
+            self.raw = _HEADS.pack(in_dev, in_stride, out_dev, out_stride, weight, n_heads)
+        except struct.error as e:
+            raise _range(e) from None
 
 
 def _raw(x) -> bytes | None:
@@ -197,8 +216,8 @@ def kv_attention_sinks_dev(ctx: Context, cache: KvCache, batch: KvBatch, q_dev: 
     every row sees (rce_qmm_kv_attention_sinks_dev)."""
     if out_stride is None and cache is not None:
         out_stride = n_q_heads * cache.d_head
-    st = lib().rce_qmm_kv_attention_sinks_dev(ctx.handle, _raw(cache), _raw(batch), q_dev, q_dtype, q_stride, n_q_heads,
-                                              _raw(rope), scale, window, sinks, out_dev, out_dtype, out_stride or 0, stream)
+    st = lib().rce_qmm_kv_attention_sinks_dev(ctx.handle, cache and cache.raw, batch and batch.raw, q_dev, q_dtype, q_stride,
+                                              n_q_heads, rope and rope.raw, scale, window, sinks, out_dev, out_dtype, out_stride or 0, stream)
     if st:
         check(st)
 
@@ -208,8 +227,8 @@ def qk_norm_rope_dev(ctx: Context, batch: KvBatch, q: Heads | None, k: Heads | N
                      stream: int | None = None) -> None:
     """Norms (eps None: none) and rotation of query and key heads in one
     pass (rce_qmm_qk_norm_rope_dev)."""
-    st = lib().rce_qmm_qk_norm_rope_dev(ctx.handle, _raw(batch), _raw(q), _raw(k), d_head, in_dtype, out_dtype,
-                                        -1.0 if eps is None else eps, _raw(rope), interleaved, stream)
+    st = lib().rce_qmm_qk_norm_rope_dev(ctx.handle, batch and batch.raw, q and q.raw, k and k.raw, d_head, in_dtype, out_dtype,
+                                        -1.0 if eps is None else eps, rope and rope.raw, interleaved, stream)
     if st:
         check(st)
 
@@ -217,7 +236,7 @@ def qk_norm_rope_dev(ctx: Context, batch: KvBatch, q: Heads | None, k: Heads | N
 def kv_copy_dev(ctx: Context, src: KvCache, dst: KvCache, src_ids_dev: int, dst_ids_dev: int, n: int,
                 stream: int | None = None) -> None:
     """Pages of one pool to pages of another, or of itself (rce_qmm_kv_copy_dev)."""
-    st = lib().rce_qmm_kv_copy_dev(ctx.handle, _raw(src), _raw(dst), src_ids_dev, dst_ids_dev, n, stream)
+    st = lib().rce_qmm_kv_copy_dev(ctx.handle, src and src.raw, dst and dst.raw, src_ids_dev, dst_ids_dev, n, stream)
     if st:
         check(st)
 
@@ -226,7 +245,7 @@ def kv_fork_dev(ctx: Context, cache: KvCache, src: KvTable, dst: KvTable, parent
                 stream: int | None = None) -> None:
     """Every sequence of `dst` gets its parent's pages in `src`
     (rce_qmm_kv_fork_dev)."""
-    st = lib().rce_qmm_kv_fork_dev(ctx.handle, _raw(cache), _raw(src), _raw(dst), parents_dev, refs_dev, stream)
+    st = lib().rce_qmm_kv_fork_dev(ctx.handle, cache and cache.raw, src and src.raw, dst and dst.raw, parents_dev, refs_dev, stream)
     if st:
         check(st)
 
@@ -235,7 +254,7 @@ def kv_release_dev(ctx: Context, cache: KvCache, table: KvTable, refs_dev: int, 
                    to_dev: int | None = None, stream: int | None = None) -> None:
     """Give up the pages wholly in positions from .. to - 1 of each sequence
     (rce_qmm_kv_release_dev; None: all)."""
-    st = lib().rce_qmm_kv_release_dev(ctx.handle, _raw(cache), _raw(table), from_dev, to_dev, refs_dev, stream)
+    st = lib().rce_qmm_kv_release_dev(ctx.handle, cache and cache.raw, table and table.raw, from_dev, to_dev, refs_dev, stream)
     if st:
         check(st)
 
@@ -244,7 +263,7 @@ def kv_reserve_dev(ctx: Context, cache: KvCache, batch: KvBatch, refs_dev: int, 
                    stream: int | None = None) -> None:
     """Pages of their own for the batch's rows, written into its tables
     (rce_qmm_kv_reserve_dev)."""
-    st = lib().rce_qmm_kv_reserve_dev(ctx.handle, _raw(cache), _raw(batch), refs_dev, missing_dev, stream)
+    st = lib().rce_qmm_kv_reserve_dev(ctx.handle, cache and cache.raw, batch and batch.raw, refs_dev, missing_dev, stream)
     if st:
         check(st)
 
@@ -252,7 +271,7 @@ def kv_reserve_dev(ctx: Context, cache: KvCache, batch: KvBatch, refs_dev: int, 
 def kv_compact_dev(ctx: Context, cache: KvCache, table: KvTable, refs_dev: int, new_ids_dev: int,
                    n_used_dev: int | None = None, stream: int | None = None) -> None:
     """The used pages to the front of the pool (rce_qmm_kv_compact_dev)."""
-    st = lib().rce_qmm_kv_compact_dev(ctx.handle, _raw(cache), _raw(table), refs_dev, new_ids_dev, n_used_dev, stream)
+    st = lib().rce_qmm_kv_compact_dev(ctx.handle, cache and cache.raw, table and table.raw, refs_dev, new_ids_dev, n_used_dev, stream)
     if st:
         check(st)
 

@@ -146,6 +146,19 @@ def test_what_is_copied(ctx, lo):
     p.free()
 
 
+@pytest.mark.parametrize("heads,d", [(1, 64), (8, 256)])
+def test_what_is_copied_in_front_of_many_pages(ctx, heads, d):
+    """A shared page at a long chunk's beginning: more items than a round, copied by the plan or behind it."""
+    p = Pages(ctx, np.random.default_rng(heads), 1300, 16, heads, d, 2, 1200)
+    rows = np.full((2, 1200), -1)
+    rows[0, :3], rows[1, :3] = (5, 700, 9), (5, 700, 11)
+    p.put(rows)
+    p.reserve([1100 * 16, 0], [40 + 1100 * 16, 40])
+    p.put(rows)
+    p.reserve([1100 * 16, 20], [23 + 1100 * 16, 43])
+    p.free()
+
+
 def test_a_pool_that_runs_out(ctx):
     """Pages go to the first that ask; what misses is counted, its entries name none, a shared page is lost there."""
     p = Pages(ctx, np.random.default_rng(2), 5, 16, 1, 64, 4, 3)
