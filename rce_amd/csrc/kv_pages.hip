@@ -468,7 +468,7 @@ __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids,
 
 dim3 over_entries(const KvTable &t) { return dim3((unsigned)((t.entries() + 255) / 256)); }
 constexpr size_t OWN_COPY = (size_t)128 << 10;  // bytes that the planning block copies itself: 4 beams of 4 heads of 64, whole pass with fork and release 17.1 -> 13.8 us
-constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256, FRONT_BLOCKS = 512;
+constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256, FRONT_BLOCKS = 2048;
 
 void copy_pages(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, const int32_t *count, int n,
                 const KvTable &t, const int32_t *new_ids, hipStream_t s) {
