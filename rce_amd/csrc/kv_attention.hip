@@ -1102,8 +1102,9 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
     if (!rows.n_rows) return hipSuccess;
     const int G = a.n_q / pool.heads;
     const size_t x = (size_t)rows.n_rows * G;
-    // positions that the tiles of a sequence span at most; with sinks its longest unit's (a sequence's rows are n_rows at most)
-    const int64_t reach = (a.sinks + KV_BLOCK - 1) / KV_BLOCK, own = ((int64_t)a.window + rows.n_rows) / KV_BLOCK + 2;
+    // positions that the tiles of a sequence span at most; with sinks its longest unit's (span_of; units of P_ROWS hold the most tokens)
+    const int64_t tokens = std::min(rows.n_rows, (P_ROWS - 1) / G + 2);
+    const int64_t reach = (a.sinks + KV_BLOCK - 1) / KV_BLOCK, own = ((int64_t)a.window + tokens) / KV_BLOCK + 2;
     const int64_t span = a.sinks ? std::min((int64_t)rows.cap, TILE * ((reach + own + 3) / 4)) : (int64_t)rows.cap;
     auto go = [&](auto d, auto with_sinks) {
         constexpr int D = decltype(d)::value;
