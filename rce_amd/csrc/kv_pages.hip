@@ -58,14 +58,17 @@ __global__ __launch_bounds__(256) void k_kv_release(KvTable t, int page_tokens, 
 // order, looked for EACH * PLAN counts at a time.
 //
 // A call of up to PLAN items (a token of every sequence) keeps them in registers and finds who asks for the same page in a
-// table in LDS.  Others go over the items once per step, and count on the pages' own counts: an item that asks takes one off;
-// where that leaves none, the least item number - CODE that is written there keeps the page.
+// table in LDS.  One of up to HOLD * PLAN items without a shared page (prompts) is held as well.  Others go over the items once per
+// step, and count on the pages' own counts: an item that asks takes one off; where that leaves none, the least item number - CODE that is
+// written there keeps the page.
 //
 // What bounds it: the chain of loads (lengths, entries, counts), barriers of 16 waves.
 constexpr int PLAN = 1024;       // threads
 constexpr int CODE = 1 << 30;    // items are fewer than 2^24
 constexpr int EACH = 4;          // counts that a thread looks at for free pages, and items of a thread's step
 constexpr int RING = 2 * EACH * PLAN;
+constexpr int HOLD = 8;          // items that a thread holds
+constexpr int AHEAD = 4;         // looks' counts that are loaded first of all: behind other kernels each load comes from HBM
 constexpr int SLOTS = 2 * PLAN;  // of the table in LDS
 
 struct Front {  // the first `blocks` blocks of page src to page dst, every head
@@ -150,25 +153,35 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
     auto entry = [&](int s, int slot) { return pages + (size_t)s * B.max_pages + slot; };
 
     // the first counts, on their way while the items are found
-    int ahead[EACH];
+    int ahead[AHEAD][EACH];
 #pragma unroll
-    for (int e = 0; e < EACH; e++) ahead[e] = R.refs[min(numbered<EACH>(e), R.n_pages - 1)];
+    for (int a = 0; a < AHEAD; a++)
+#pragma unroll
+        for (int e = 0; e < EACH; e++) ahead[a][e] = R.refs[min(EACH * PLAN * a + numbered<EACH>(e), R.n_pages - 1)];
     int head = 0, have = 0, looked = 0;  // the ring's first free page, its free pages, counts looked at
-    auto look = [&] {
+    auto look = [&](const int (&counts)[EACH]) {
         bool free[EACH];
         int of[EACH];
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const int at = looked + numbered<EACH>(e);
-            free[e] = at < R.n_pages && (looked ? seen(R.refs + at) : ahead[e]) == 0;
-        }
+        for (int e = 0; e < EACH; e++) free[e] = looked + numbered<EACH>(e) < R.n_pages && counts[e] == 0;
         const int more = ranks<EACH>(free, part, of);
 #pragma unroll
         for (int e = 0; e < EACH; e++)
-            if (free[e]) ring[(head + have + of[e]) & (RING - 1)] = looked + numbered<EACH>(e);
+            if (free[e] && have + of[e] < RING) ring[(head + have + of[e]) & (RING - 1)] = looked + numbered<EACH>(e);
         have += more;
         looked += min(EACH * PLAN, R.n_pages - looked);
         __syncthreads();
+    };
+    auto look_for = [&](int wanted) {  // the same in every thread
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+            if (looked == EACH * PLAN * a && have < wanted && looked < R.n_pages) look(ahead[a]);
+        while (have < wanted && looked < R.n_pages) {
+            int counts[EACH];
+#pragma unroll
+            for (int e = 0; e < EACH; e++) counts[e] = seen(R.refs + min(looked + numbered<EACH>(e), R.n_pages - 1));
+            look(counts);
+        }
     };
     // a free page for an item (rank: items of this step that need one before it), or none; its page p is left behind if it has one
     auto give = [&](int s, int slot, int rank, int p, bool leaves) {
@@ -251,7 +264,7 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
         }
         int total;
         const int rank = block_scan(need, part, total);
-        while (have < total && looked < R.n_pages) look();  // the same in every thread
+        look_for(total);
         if (need) {
             if (leaves) atomicSub(R.refs + p, 1);
             if (!give(s, slot, rank, p, leaves)) atomicAdd(lost + s, 1);
@@ -259,6 +272,37 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
         copy();
         if (missing && tid < B.n_seqs) missing[tid] = lost[tid];
         return;
+    }
+
+    if (B.n_seqs <= PLAN && items <= HOLD * PLAN) {  // consecutive items, HOLD a thread; no shared page among them
+        const int i = HOLD * tid, n = min(HOLD, max(0, items - i));
+        int q = sequence(min(i, items - 1)), s[HOLD], slot[HOLD], p[HOLD], count = 0;
+#pragma unroll
+        for (int e = 0; e < HOLD; e++) {
+            const int at = min(i + e, items - 1);
+            while (start[q + 1] <= at) q++;  // start[PLAN] is above all
+            s[e] = q;
+            slot[e] = slot0[q] + at - start[q];
+        }
+#pragma unroll
+        for (int e = 0; e < HOLD; e++) p[e] = *entry(s[e], slot[e]);
+        bool shared = false;
+#pragma unroll
+        for (int e = 0; e < HOLD; e++) {
+            const bool named = (unsigned)p[e] < (unsigned)R.n_pages;
+            if (e < n && named) shared |= R.refs[p[e]] > 1;
+            count += e < n && !named;
+        }
+        if (!__syncthreads_or(shared)) {
+            int total, rank = block_scan(count, part, total);
+            look_for(total);
+#pragma unroll
+            for (int e = 0; e < HOLD; e++)
+                if (e < n && (unsigned)p[e] >= (unsigned)R.n_pages && !give(s[e], slot[e], rank++, -1, false)) atomicAdd(lost + s[e], 1);
+            copy();
+            if (missing && tid < B.n_seqs) missing[tid] = lost[tid];
+            return;
+        }
     }
 
     if (missing)
@@ -337,7 +381,7 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
             count += need[e];
         }
         int total, rank = block_scan(count, part, total);
-        while (have < total && looked < R.n_pages) look();  // the same in every thread
+        look_for(total);
 #pragma unroll
         for (int e = 0; e < EACH; e++)
             if (need[e] && !give(s[e], slot[e], rank++, p[e], leaves[e]) && missing) atomicAdd(missing + s[e], 1);
@@ -401,8 +445,8 @@ struct Moves {
     int count, pad[3];
     int32_t src[KV_COMPACT_PAGES / 2], dst[KV_COMPACT_PAGES / 2];
 };
-// One block: the used pages are counted, then the free ones among the first n_used ranked, then the used ones behind them, LOOK
-// consecutive counts a thread and step.
+// One block: the used pages are counted; then each page's place among the used ones says what it is to do, LOOK counts a thread and
+// step: the free ones among the first n are listed, and the used ones behind them take them in order.
 constexpr int LOOK = 16;
 __device__ __forceinline__ void look_at(const KvRefs &R, int from, int (&r)[LOOK]) {
 #pragma unroll
@@ -413,6 +457,7 @@ __device__ __forceinline__ void look_at(const KvRefs &R, int from, int (&r)[LOOK
 __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids, int32_t *n_used, Moves *moves) {
     __shared__ int part[PLAN / 64], list[LOOK * PLAN / 2];  // where ref holds all counts, what is free below n: half of them at most
     const int tid = threadIdx.x;
+    __shared__ int before_n;  // used pages among the first n
     int ref[LOOK], of[LOOK], n = 0;
     bool is[LOOK];
     for (int p0 = 0; p0 < R.n_pages; p0 += LOOK * PLAN) {
@@ -421,49 +466,53 @@ __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids,
         for (int e = 0; e < LOOK; e++) is[e] = ref[e] != 0;
         n += ranks<LOOK>(is, part, of);
     }
-    if (tid == 0 && n_used) *n_used = n;
-    const bool once = R.n_pages <= LOOK * PLAN;  // ref holds all counts
-    int holes = 0;
-    for (int p0 = 0; p0 < n; p0 += LOOK * PLAN) {
-        if (!once) look_at(R, p0, ref);
+    const bool once = R.n_pages <= LOOK * PLAN;  // ref, is and of hold all
+    int used = 0;                                // before this step
+    for (int p0 = 0; p0 < R.n_pages; p0 += LOOK * PLAN) {
+        int total = n;
+        if (!once) {
+            look_at(R, p0, ref);
 #pragma unroll
-        for (int e = 0; e < LOOK; e++) is[e] = p0 + numbered<LOOK>(e) < n && ref[e] == 0;
-        const int total = ranks<LOOK>(is, part, of);
+            for (int e = 0; e < LOOK; e++) is[e] = ref[e] != 0;
+            total = ranks<LOOK>(is, part, of);
+        }
+        // what is not used before n, in order: the pages before it less the used ones
 #pragma unroll
         for (int e = 0; e < LOOK; e++) {
-            const int p = p0 + numbered<LOOK>(e);
-            if (is[e]) {
-                moves->dst[holes + of[e]] = p;
-                if (once) list[of[e]] = p;
+            const int p = p0 + numbered<LOOK>(e), u = used + of[e];
+            if (p == n) before_n = u;
+            if (p >= n) continue;
+            if (!is[e]) {
+                moves->dst[p - u] = p;
+                if (once) list[p - u] = p;
             }
-            if (p < n) new_ids[p] = is[e] ? -1 : p;
+            new_ids[p] = is[e] ? p : -1;
         }
-        holes += total;
-    }
-    if (once) __syncthreads();
-    else arrived();
-    int moved = 0;
-    for (int p0 = once ? 0 : n; p0 < R.n_pages; p0 += LOOK * PLAN) {
-        if (!once) look_at(R, p0, ref);
-#pragma unroll
-        for (int e = 0; e < LOOK; e++) is[e] = p0 + numbered<LOOK>(e) >= n && ref[e] != 0;
-        const int total = ranks<LOOK>(is, part, of);
+        if (once) __syncthreads();
+        else arrived();
         int to[LOOK];
 #pragma unroll
-        for (int e = 0; e < LOOK; e++) to[e] = !is[e] ? -1 : once ? list[of[e]] : seen(moves->dst + moved + of[e]);
+        for (int e = 0; e < LOOK; e++) {
+            const int r = used + of[e] - before_n;
+            to[e] = p0 + numbered<LOOK>(e) < n || !is[e] ? -1 : once ? list[r] : seen(moves->dst + r);
+        }
 #pragma unroll
         for (int e = 0; e < LOOK; e++) {
             const int p = p0 + numbered<LOOK>(e);
+            if (p < n || p >= R.n_pages) continue;
             if (is[e]) {
-                moves->src[moved + of[e]] = p;
+                moves->src[used + of[e] - before_n] = p;
                 R.refs[to[e]] = ref[e];
                 R.refs[p] = 0;
             }
-            if (p >= n && p < R.n_pages) new_ids[p] = to[e];
+            new_ids[p] = to[e];
         }
-        moved += total;
+        used += total;
     }
-    if (tid == 0) moves->count = moved;
+    if (tid == 0) {
+        moves->count = n < R.n_pages ? n - before_n : 0;
+        if (n_used) *n_used = n;
+    }
 }
 
 dim3 over_entries(const KvTable &t) { return dim3((unsigned)((t.entries() + 255) / 256)); }
