@@ -81,6 +81,9 @@ constexpr int LONG = 1536, LONG_TILES = 48;
 // With sinks no unit visits more tiles than a window's.  Up to SHORT of them a few sequences have one part (a long one is there: units of few rows
 // take no longer than its), and units that are TARGET and more are not split: 3 x 500 rows after 9000, a window of 2048: 117 -> 104 us.
 constexpr int SHORT = 64;
+// Tiles of the shortest range of few rows there, and beyond.  In ranges of 8 : of 4 (us, whole calls): one row, window 1024, 4 kv heads of 64,
+// f32 14.5 : 13.2; window 1500, 8 of 128 17.9 : 15.7; 8 rows, window 1024 20.4 : 19.8; one row, window 8192 21.1 : 22.4.
+constexpr int SHORT_CHUNK = 4;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -1130,7 +1133,8 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         };
         auto target = [](size_t room, int unit) { return std::min(TARGET, (int)(room / ((size_t)unit * (D + 2) * sizeof(float)) * 16 / 34)); };
         auto few = [&](int hi) {
-            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS), span > SPLIT_FROM * TILE ? MIN_CHUNK : WHOLE, 0, vec};
+            Args A{pool, rows, a, G, ROWS, 0, hi, target(FEW_PARTS, ROWS),
+                   span <= SPLIT_FROM * TILE ? WHOLE : SINKS && span <= SHORT * TILE ? SHORT_CHUNK : MIN_CHUNK, 0, vec};
             const size_t u = units(A, hi);
             // can its tiles come to a line at all?
             A.line = span > SPLIT_FROM * TILE && pool.heads * 20 <= A.target &&

@@ -274,31 +274,28 @@ __global__ __launch_bounds__(PLAN) void k_kv_reserve(KvRows B, int lg_page, int3
         return;
     }
 
-    if (B.n_seqs <= PLAN && items <= HOLD * PLAN) {  // consecutive items, HOLD a thread; no shared page among them
-        const int i = HOLD * tid, n = min(HOLD, max(0, items - i));
-        int q = sequence(min(i, items - 1)), s[HOLD], slot[HOLD], p[HOLD], count = 0;
+    if (B.n_seqs <= PLAN && items <= HOLD * PLAN) {  // HOLD items a thread, no shared page among them
+        int s[HOLD], slot[HOLD], p[HOLD], of[HOLD];
+        bool need[HOLD], shared = false;
 #pragma unroll
         for (int e = 0; e < HOLD; e++) {
-            const int at = min(i + e, items - 1);
-            while (start[q + 1] <= at) q++;  // start[PLAN] is above all
-            s[e] = q;
-            slot[e] = slot0[q] + at - start[q];
+            const int at = min(numbered<HOLD>(e), items - 1);
+            s[e] = sequence(at);
+            slot[e] = slot0[s[e]] + at - start[s[e]];
         }
 #pragma unroll
         for (int e = 0; e < HOLD; e++) p[e] = *entry(s[e], slot[e]);
-        bool shared = false;
 #pragma unroll
         for (int e = 0; e < HOLD; e++) {
             const bool named = (unsigned)p[e] < (unsigned)R.n_pages;
-            if (e < n && named) shared |= R.refs[p[e]] > 1;
-            count += e < n && !named;
+            need[e] = numbered<HOLD>(e) < items && !named;
+            if (named) shared |= R.refs[p[e]] > 1;  // (behind the last item: its own again)
         }
         if (!__syncthreads_or(shared)) {
-            int total, rank = block_scan(count, part, total);
-            look_for(total);
+            look_for(ranks<HOLD>(need, part, of));
 #pragma unroll
             for (int e = 0; e < HOLD; e++)
-                if (e < n && (unsigned)p[e] >= (unsigned)R.n_pages && !give(s[e], slot[e], rank++, -1, false)) atomicAdd(lost + s[e], 1);
+                if (need[e] && !give(s[e], slot[e], of[e], -1, false)) atomicAdd(lost + s[e], 1);
             copy();
             if (missing && tid < B.n_seqs) missing[tid] = lost[tid];
             return;
