@@ -198,8 +198,10 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
     for (int base = 0; base < A.B.n_seqs; base += 64) {
         const int s = base + lane;
         int c = 0, sc = 0;
+        KvSeq q{0, 0, 0};
         if (s < A.B.n_seqs) {
-            const Span p = span_of<SINKS>(A, kv_seq(A.B, s));
+            q = kv_seq(A.B, s);
+            const Span p = span_of<SINKS>(A, q);
             const int n = ranges(p.tiles, chunk);
             c = p.units * n;
             sc = n > 1 ? c : 0;
@@ -210,7 +212,7 @@ __device__ __forceinline__ bool find_work(const Args &A, int item, int chunk, Wo
             const int l = __builtin_ctzll(__ballot(item < run + incl));
             const int at = item - run - __builtin_amdgcn_readlane(incl - c, l);
             w.seq = base + l;
-            w.q = kv_seq(A.B, w.seq);
+            w.q = {__builtin_amdgcn_readlane(q.r0, l), __builtin_amdgcn_readlane(q.r1, l), __builtin_amdgcn_readlane(q.len, l)};
             w.sp = span_of<SINKS>(A, w.q);
             const int n = ranges(w.sp.tiles, chunk), step = range_tiles(w.sp.tiles, n);
             const int u = at / n, range = at - u * n;
@@ -400,7 +402,14 @@ __device__ __forceinline__ void query_codes(const Args &A, const KvSeq &q, int h
         load_pieces<NQ>(A.a.q, A.a.q_dtype, own, x);
         if (half) {
             float y[NQ][16];
-            load_pieces<NQ>(A.a.q, A.a.q_dtype, other, y);
+            if (NQ % 2 == 0 && 2 * half == D) {  // the lane's own pieces
+#pragma unroll
+                for (int s = 0; s < NQ; s++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) y[s][j] = x[(s + NQ / 2) % NQ][j];
+            } else {
+                load_pieces<NQ>(A.a.q, A.a.q_dtype, other, y);
+            }
 #pragma unroll
             for (int s = 0; s < NQ; s++) {
                 const int d = 64 * s + 16 * g;
@@ -727,6 +736,8 @@ template <int D, bool HILO, bool SINKS>
 __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k_kv_prompt(Args A, const int32_t *__restrict__ page_table) {
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
+    constexpr bool QUICK = SINKS && !HILO;
+    constexpr float lag = QUICK ? 0.0f : LAG;  // QUICK comes to the maximum only where m was too low
     constexpr int NK = (TILE * D + 16 * 64 * P_WAVES - 1) / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
     constexpr int BUFS = D <= 128 ? 2 : 1;  // two where they fit 64 KB
     __shared__ PShared<D> buf[BUFS];
@@ -734,7 +745,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.P.heads;
     Work w;
-    if (!find_work<SINKS>(A, blockIdx.x / A.P.heads, cut_of<false, SINKS>(A).chunk, w)) return;
+    if (!find_work<SINKS>(A, blockIdx.x / A.P.heads, SINKS && A.min_chunk == WHOLE ? WHOLE : cut_of<false, SINKS>(A).chunk, w)) return;
     const KvSeq &q = w.q;
     const int G = A.G, first = q.first();
     const int x0 = w.unit * P_ROWS, n_x = min(P_ROWS, (q.r1 - q.r0) * G - x0);
@@ -744,7 +755,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
 
     i32x4 qf[NQ][LIMBS];
     float qs;
-    query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
+    if constexpr (!SINKS) query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
 
     const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;
     // the wave's rows: positions that all of them see, or that any of them sees
@@ -836,6 +847,11 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
         look(t_lo);
         fetch(t_lo);
         look(t_lo + 1);
+    }
+    // With sinks units are short, and the first tile comes while the query rows do (with the rows' halves read once
+    // 2 prompts of up to 6000, window 1024 289 -> 280 us); without, 3 x 201 rows f32 take 31.6 us so, 31.1 the other way.
+    if constexpr (SINKS) query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
+    if (t_lo < t_hi) {
         place(buf[0]);
         if (t_lo + 1 < t_hi) fetch(t_lo + 1);
         look(t_lo + 2);
@@ -874,98 +890,120 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
             }
             auto score = [&](int e) { return HILO ? xh[HILO ? e : 0] + (float)xi[e] : (float)xi[e]; };
             const float f = sh.ks[g] * qs;
-            float sv = sh.vs[g], top = -INFINITY;
-            uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
-            if (HILO || masked) {
-                if (masked) {
-                    const int p = KV_BLOCK * visit.block(t, g), lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
-                    seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
-                    if constexpr (SINKS) {
-                        const int last = min(hi, A.a.sinks - 1 - p);
-                        if (sh.ok[g] && last >= 0) seen |= 0xFFFFu >> (15 - last);
+            float sv = sh.vs[g];
+            half8 ph[2], pl[2];
+            // QUICK: a tile that all its rows see is weighted with the m and ref there are, with no maximum over
+            // it.  It stands where no weight is past binary16 (the sum of a lane's 16 bounds each; an m of
+            // -infinity and a NaN fail) and the scale is as in the ordinary tile below; else the tile is weighted again,
+            // after a new m.  2 prompts of up to 6000, window 1024, 4 sinks, f16 280 -> 262 us; 3 x 500 rows, window 2048 100 -> 93.
+            bool done = false;
+            if constexpr (QUICK) {
+                if (!masked) {
+                    const float pw = sv * inv_ref, lw = __builtin_amdgcn_logf(pw), off = lw - m;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float p = exp2_(__builtin_fmaf((float)xi[e], f, off));
+                        sum += p;
+                        ph[e >> 3][e & 7] = (_Float16)p;
                     }
-                    if (!seen) sv = 0.0f;  // as in k_kv_attention
+                    done = !__ballot(!(pw >= 0.125f && pw < 2.0f * UP && sum <= 65504.0f));
+                    if (done) l = __builtin_fmaf(sum, exp2_(-lw), l);
                 }
-                asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
-                if constexpr (SINKS && !HILO) {
-                    // what a row does not see is below all that it sees; a row that sees nothing has no score
-                    int x = UNSEEN;
+            }
+            if (!done) {
+                float top = -INFINITY;
+                uint32_t seen = 0xFFFFu;  // bit e: the row sees the position of score e
+                if (HILO || masked) {
+                    if (masked) {
+                        const int p = KV_BLOCK * visit.block(t, g), lo = max(p_lo - p, 0), hi = min(p_hi - p, 15);
+                        seen = sh.ok[g] && lo <= hi ? (0xFFFFu << lo) & (0xFFFFu >> (15 - hi)) : 0u;
+                        if constexpr (SINKS) {
+                            const int last = min(hi, A.a.sinks - 1 - p);
+                            if (sh.ok[g] && last >= 0) seen |= 0xFFFFu >> (15 - last);
+                        }
+                        if (!seen) sv = 0.0f;  // as in k_kv_attention
+                    }
+                    asm volatile("" : "+v"(seen));  // else its bits are tested in front of the branch
+                    if constexpr (SINKS && !HILO) {
+                        // what a row does not see is below all that it sees; a row that sees nothing has no score
+                        int x = UNSEEN;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int is = (int)(seen << (31 - e)) >> 31;
+                            xi[e] = (xi[e] & is) | (UNSEEN & ~is);
+                            x = max(x, xi[e]);
+                        }
+                        top = seen ? (float)x * f : -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+                    }
+                } else {
+                    int x = xi[0];
+#pragma unroll
+                    for (int e = 1; e < 16; e++) x = max(x, xi[e]);
+                    top = (float)x * f;
+                }
+                top = swap_max(top);
+                // `top` above m + LAG, or a larger value scale that the row sees: rescale (lanes alone for the
+                // scale: a ballot over both costs registers that spill)
+                const bool fin = sv < __builtin_inff();
+                const float scale = swap_max(fin ? sv : 0.0f);
+                if (__ballot(top > m + lag) || scale > ref) {
+                    const float m_new = top > m + lag ? top : m, ref_new = fmaxf(ref, scale);
+                    const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
+                    const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
+                    l *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][e] *= back;
+                    m = m_new;
+                    ref = ref_new;
+                    inv_ref = UP / ref;
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                // what the values' scale makes of the weights; an infinite or NaN one makes NaN of the
+                // rows that see its block, no others
+                const float pw = fin ? sv * inv_ref : sv;
+                // The ordinary tile: no mask, value scales above 2^-12 of `ref`.  The scale goes into the
+                // exponent, l gets the sum of the weights in f32 over it (the rounded ones would leave out
+                // those below 2^-25 / pw: 1 % of the sum of 65536 at 2^-22.6).
+                // Two terms (HILO) and all else take the longer way.
+                if (!HILO && !QUICK && !masked && !__ballot(!(pw >= 0.125f && pw < 2.0f * UP))) {
+                    const float lw = __builtin_amdgcn_logf(pw), off = lw - base;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float p = exp2_(__builtin_fmaf((float)xi[e], f, off));
+                        sum += p;
+                        ph[e >> 3][e & 7] = (_Float16)p;
+                    }
+                    l = __builtin_fmaf(sum, exp2_(-lw), l);
+                } else if constexpr (SINKS && !HILO) {  // xi is UNSEEN where the row does not see it: the weight is taken out
+                    float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const int is = (int)(seen << (31 - e)) >> 31;
-                        xi[e] = (xi[e] & is) | (UNSEEN & ~is);
-                        x = max(x, xi[e]);
+                        const float y = __int_as_float(__float_as_int(exp2_(__builtin_fmaf((float)xi[e], f, -base))) & is);
+                        sum += y;
+                        ph[e >> 3][e & 7] = (_Float16)__int_as_float(__float_as_int(y * pw) & is);
                     }
-                    top = seen ? (float)x * f : -INFINITY;
+                    l += sum;
                 } else {
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) top = fmaxf(top, seen >> e & 1 ? score(e) * f : -INFINITY);
+                    for (int e = 0; e < 16; e++) {
+                        const bool see = seen >> e & 1;
+                        const float y = see ? exp2_(score(e) * f - base) : 0.0f, p = see ? y * pw : 0.0f;
+                        sum += y;
+                        const _Float16 hi = (_Float16)p;
+                        ph[e >> 3][e & 7] = hi;
+                        if constexpr (HILO) pl[e >> 3][e & 7] = (_Float16)(p - (float)hi);
+                    }
+                    l += sum;
                 }
-            } else {
-                int x = xi[0];
-#pragma unroll
-                for (int e = 1; e < 16; e++) x = max(x, xi[e]);
-                top = (float)x * f;
-            }
-            top = swap_max(top);
-            // `top` above m + LAG, or a larger value scale that the row sees: rescale (lanes alone for the
-            // scale: a ballot over both costs registers that spill)
-            const bool fin = sv < __builtin_inff();
-            const float scale = swap_max(fin ? sv : 0.0f);
-            if (__ballot(top > m + LAG) || scale > ref) {
-                const float m_new = top > m + LAG ? top : m, ref_new = fmaxf(ref, scale);
-                const float alpha = m == -INFINITY ? 0.0f : exp2_(m - m_new);
-                const float back = ref_new > ref ? ref / ref_new * alpha : alpha;
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][e] *= back;
-                m = m_new;
-                ref = ref_new;
-                inv_ref = UP / ref;
-            }
-            const float base = m == -INFINITY ? 0.0f : m;
-            // what the values' scale makes of the weights; an infinite or NaN one makes NaN of the
-            // rows that see its block, no others
-            const float pw = fin ? sv * inv_ref : sv;
-            half8 ph[2], pl[2];
-            // The ordinary tile: no mask, value scales above 2^-12 of `ref`.  The scale goes into the
-            // exponent, l gets the sum of the weights in f32 over it (the rounded ones would leave out
-            // those below 2^-25 / pw: 1 % of the sum of 65536 at 2^-22.6).
-            // Two terms (HILO) and all else take the longer way.
-            if (!HILO && !masked && !__ballot(!(pw >= 0.125f && pw < 2.0f * UP))) {
-                const float lw = __builtin_amdgcn_logf(pw), off = lw - base;
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float p = exp2_(__builtin_fmaf((float)xi[e], f, off));
-                    sum += p;
-                    ph[e >> 3][e & 7] = (_Float16)p;
-                }
-                l = __builtin_fmaf(sum, exp2_(-lw), l);
-            } else if constexpr (SINKS && !HILO) {  // xi is UNSEEN where the row does not see it: the weight is taken out
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int is = (int)(seen << (31 - e)) >> 31;
-                    const float y = __int_as_float(__float_as_int(exp2_(__builtin_fmaf((float)xi[e], f, -base))) & is);
-                    sum += y;
-                    ph[e >> 3][e & 7] = (_Float16)__int_as_float(__float_as_int(y * pw) & is);
-                }
-                l += sum;
-            } else {
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const bool see = seen >> e & 1;
-                    const float y = see ? exp2_(score(e) * f - base) : 0.0f, p = see ? y * pw : 0.0f;
-                    sum += y;
-                    const _Float16 hi = (_Float16)p;
-                    ph[e >> 3][e & 7] = hi;
-                    if constexpr (HILO) pl[e >> 3][e & 7] = (_Float16)(p - (float)hi);
-                }
-                l += sum;
             }
 #pragma unroll
             for (int u = 0; u < 2; u++)  // positions 16 g + 8 u ...
