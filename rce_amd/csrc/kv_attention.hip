@@ -7,7 +7,8 @@
 // tiles of 64 positions; a block takes one range, its four waves every fourth
 // tile, and joins the waves' (m, l, o) in LDS.  A unit of one range is
 // finished there; the ranges of a longer one leave (m, l, o) in `parts`, which
-// k_kv_join adds up in range order.
+// k_kv_join adds up in range order.  With first positions that stay visible beside a window (SINKS,
+// rce_qmm_kv_attention_sinks_dev) a unit's tiles are four blocks each of what it visits (Span, Visits).
 //
 // Every block plans for itself: it reads the sequences' lengths (device
 // memory, no host round trip), forms the total of tiles and from it the chunk
