@@ -381,7 +381,7 @@ __device__ __forceinline__ void load_pieces(const void *p, uint32_t t, const siz
 
 // Row x_row of the sequence and kv head h, rotated to position pos, as codes: the 16 dimensions
 // 64 s + 16 g .. of this lane in qf[s], the factor of its base-2 scores in qs.  is: the row has a position.
-template <int D, int LIMBS>
+template <int D, int LIMBS, bool SINKS>
 __device__ __forceinline__ void query_codes(const Args &A, const KvSeq &q, int h, int x_row, int pos, bool is, int g,
                                             i32x4 (&qf)[D / 64][LIMBS], float &qs) {
     constexpr int NQ = D / 64;
@@ -401,9 +401,29 @@ __device__ __forceinline__ void query_codes(const Args &A, const KvSeq &q, int h
             other[s] = at + (d < half ? d + half : d < 2 * half ? d - half : d);
         }
         load_pieces<NQ>(A.a.q, A.a.q_dtype, own, x);
-        if (half) {
+        // All of a head turned, two operands or more: the lane holds its pieces' partners.  With sinks their pairs turn
+        // together, by table values read once (2 x 6000 tokens, window 64 132 -> 119 us); without, that spills registers
+        // (3 x 4096 488 -> 497 us).
+        const bool partners = NQ % 2 == 0 && 2 * half == D;
+        if (SINKS && partners) {
+            constexpr int H = NQ / 2;
+#pragma unroll
+            for (int s = 0; s < H; s++) {
+                const float4 *c = reinterpret_cast<const float4 *>(cs + 2 * (64 * s + 16 * g));
+                float (&a)[16] = x[s], (&b)[16] = x[(s + H) % NQ];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 v = c[j];
+                    const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
+                    a[2 * j] = a0 * v.x - b0 * v.y;
+                    a[2 * j + 1] = a1 * v.z - b1 * v.w;
+                    b[2 * j] = a0 * v.y + b0 * v.x;
+                    b[2 * j + 1] = a1 * v.w + b1 * v.z;
+                }
+            }
+        } else if (half) {
             float y[NQ][16];
-            if (NQ % 2 == 0 && 2 * half == D) {  // the lane's own pieces
+            if (!SINKS && partners) {
 #pragma unroll
                 for (int s = 0; s < NQ; s++)
 #pragma unroll
@@ -499,7 +519,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
         const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;  // keys p_lo .. p_hi
         i32x4 qf[NQ][LIMBS];
         float qs;
-        query_codes<D, LIMBS>(A, q, h, x0 + n, pos, is, g, qf, qs);
+        query_codes<D, LIMBS, SINKS>(A, q, h, x0 + n, pos, is, g, qf, qs);
 
         // tiles of this unit and range; keys that every row sees need no mask
         const int u_tok0 = x0 / G, u_tok1 = (x0 + n_x - 1) / G;
@@ -756,7 +776,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
 
     i32x4 qf[NQ][LIMBS];
     float qs;
-    if constexpr (!SINKS) query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
+    if constexpr (!SINKS) query_codes<D, LIMBS, SINKS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
 
     const int p_hi = is ? pos : -1, p_lo = is ? max(0, pos - (A.a.window - 1)) : 0;
     // the wave's rows: positions that all of them see, or that any of them sees
@@ -851,7 +871,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     }
     // With sinks units are short, and the first tile comes while the query rows do (with the rows' halves read once
     // 2 prompts of up to 6000, window 1024 289 -> 280 us); without, 3 x 201 rows f32 take 31.6 us so, 31.1 the other way.
-    if constexpr (SINKS) query_codes<D, LIMBS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
+    if constexpr (SINKS) query_codes<D, LIMBS, SINKS>(A, q, h, x0 + xr, pos, is, g, qf, qs);
     if (t_lo < t_hi) {
         place(buf[0]);
         if (t_lo + 1 < t_hi) fetch(t_lo + 1);
