@@ -267,7 +267,8 @@ struct Groups {
 };
 
 // The groups that experts are chosen from, group g's bit at g << lg: a group's lanes find its two largest values (in LDS, v), the
-// groups' worth is compared.  slack above 0: `sure` becomes false where two worths are that near each other.
+// groups' worth is compared.  slack above 0: `sure` becomes false where two worths are nearer each other than that and what their
+// addends' roundings come to, or their addends pass binary32.
 template <class V>
 __device__ __forceinline__ uint64_t kept_groups(const Routing &A, const V *v, const Groups &G, float slack, bool &sure) {
     const V none = -(V)__builtin_inff();
@@ -287,13 +288,21 @@ __device__ __forceinline__ uint64_t kept_groups(const Routing &A, const V *v, co
         b = d > b ? d : b;
         b = low > b ? low : b;
     }
-    if (A.group_top == 2 && b > none) a += b;
+    // of the addends, not of a sum that they cancel in; no expert: below all
+    float addends = a > none ? fabsf((float)a) : -1.0f;
+    if (A.group_top == 2 && b > none) {
+        a += b;
+        addends += fabsf((float)b);
+    }
     int rank = 0;
     bool near = false;
     for (int i = 0; i < A.n_group; i++) {
         const V o = lane_value(a, i << lg);
         rank += o > a || (o == a && i < g);
-        if (slack > 0.0f) near |= i != g && fabsf((float)(o - a)) <= slack + 0x1p-21f * fabsf((float)a);
+        if (slack > 0.0f) {
+            const float larger = fmaxf(addends, lane_value(addends, i << lg));
+            near |= i != g && larger >= 0.0f && !(fabsf((float)(o - a)) > slack + 0x1p-21f * larger);
+        }
     }
     if (slack > 0.0f && __ballot(near && g < A.n_group)) sure = false;
     return __ballot(g < A.n_group && rank < A.topk_group);
@@ -308,7 +317,8 @@ __device__ __forceinline__ uint64_t kept_groups(const Routing &A, const V *v, co
 //   (<= 1/4); 2^-24 + 2^-23 for the sum and the reciprocal: below 2^-22;
 //   softmax, t = top - x: 2.5 * 2^-24 t + 2^-23 of e^-t, in the sum too (its weighted mean of t is at most ln 1024), whose 1024 terms add up in
 //   21 roundings (16 a lane, six steps between lanes), reciprocal and product: 45 * 2^-24 of a score, below 2^-18 of the highest.
-// Sums with the bias, and of two, are rounded to 2^-24 each.
+// A sum with the bias is rounded to 2^-24 of itself.  So is a group's sum of two, whose addends may be far larger than it: two groups' sums
+// are off by 2^-23 of what each one's addends come to, less than 2^-21 of the larger.
 constexpr float SIGMOID_ERROR = 0x1p-22f, SOFTMAX_ERROR = 0x1p-18f;
 
 __device__ __forceinline__ float rough_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }

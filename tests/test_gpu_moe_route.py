@@ -178,6 +178,62 @@ def test_scores_next_to_each_other(ctx):
                 assert np.array_equal(ids[at], sc.route(lg[at], bias=bias, **how)[0])
 
 
+def near_groups(rng, n, e, groups, size, sigmoid):
+    """(logits [n, e], bias [e], the two groups): two groups of which each counts by a bias of +b and one of -b, their sums
+    1e-7 to 1e-5 apart one way or the other (a logit's rounding moves a sum by 2^-24 at most); all other experts far below."""
+    g0, g1 = sorted(rng.choice(groups, 2, replace=False))
+    at = [g0 * size, g0 * size + size - 1, g1 * size, g1 * size + size - 1]
+    lg = np.full((n, e), -30.0, F32)
+    apart = 10.0 ** rng.uniform(-7, -5, n) * rng.choice([-1, 1], n)
+    if sigmoid:
+        s = rng.uniform(0.3, 0.7, (n, 3))
+        s = np.column_stack([s, s[:, 0] + s[:, 1] - s[:, 2] + apart])
+        s = np.where((s[:, 3:] > 0.05) & (s[:, 3:] < 0.95), s, np.array([0.4, 0.6, 0.55, 0.45]) + apart[:, None] * [0, 0, 0, 1])
+        lg[:, at] = np.log(s / (1 - s))
+    else:
+        a = rng.uniform(0.1, 0.9, (n, 2)) * np.column_stack([0.5 + apart / 2, 0.5 - apart / 2])
+        lg[:, at] = np.log(np.column_stack([a[:, 0], 0.5 + apart / 2 - a[:, 0], a[:, 1], 0.5 - apart / 2 - a[:, 1]]))
+    return lg, at
+
+
+@pytest.mark.parametrize("experts,groups", [(4, 2), (16, 4), (64, 8), (128, 4), (256, 8), (256, 2), (512, 16), (1024, 32)])
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("size", [2.0, 16.0, 100.0, 1000.0, 3e4])
+def test_groups_whose_biases_cancel(ctx, experts, groups, sigmoid, size):
+    """A group counts by two experts of opposite large biases: the sum is small, what 32 bits lose of each addend is not.  Few
+    tokens, and the same rows in a call of many."""
+    print(f"route cancelling experts={experts} groups={groups} sigmoid={sigmoid} size={size}", flush=True)
+    rng = np.random.default_rng(experts + int(size))
+    per = experts // groups
+    lg, at = near_groups(rng, 200, experts, groups, per, sigmoid)
+    bias = np.full(experts, -4 * size, F32)
+    bias[at] = size, -size, size, -size
+    how = dict(top_k=2, sigmoid=sigmoid, groups=groups, kept=1, group_top=2)
+    check(ctx, lg, G.F32, how, bias=bias)
+    many = np.tile(lg, (33, 1))  # 6600 tokens
+    ids, _ = run(ctx, many, G.F32, how, bias=bias)
+    assert np.array_equal(ids, np.tile(sc.route(lg, bias=bias, **how)[0], (33, 1)))
+
+
+def test_a_group_lost_to_its_neighbour(ctx):
+    """64 bits: 0.67821895 against 0.67821878; sums of what 32 bits hold of the addends: 0.67821789 against 0.67821980."""
+    lg = np.array([[-0.96945596, -0.39202467, 0.28211886, -2.1097460]], F32)
+    check(ctx, lg, G.F32, dict(top_k=2, sigmoid=True, groups=2, kept=1, group_top=2), bias=np.array([16, -16, 16, -16], F32))
+
+
+def test_group_sums_beyond_32_bits(ctx):
+    """Two biases whose sum passes binary32, up or down, beside groups that are as far out, nearer, or hold no expert."""
+    big = 3e38
+    for b in ([big, big, big, 3.1e38, 1, 1, 0, 0], [-big, -big, -3.1e38, -big, np.nan, np.nan, -np.inf, -np.inf],
+              [-big, -big, np.nan, -np.inf, -big, -3.1e38, np.nan, np.nan], [np.inf, 0, big, big, np.inf, 1, np.nan, np.inf]):
+        rng = np.random.default_rng(11)
+        lg = rng.standard_normal((20, 8)).astype(F32)
+        for perm in ([0, 1, 2, 3, 4, 5, 6, 7], [6, 7, 0, 1, 4, 5, 2, 3], [2, 3, 6, 7, 0, 1, 4, 5]):
+            for kept, k in ((1, 1), (1, 2), (2, 3), (3, 6)):
+                with np.errstate(over="ignore"):
+                    check(ctx, lg, G.F32, dict(top_k=k, sigmoid=True, groups=4, kept=kept, group_top=2), bias=np.array(b, F32)[perm])
+
+
 def test_a_wide_call(ctx):
     """Rows further apart than 2^31 values, and more tokens than a launch's first blocks."""
     n, e, stride = 3, 8, (1 << 30) + 8
