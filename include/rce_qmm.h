@@ -540,7 +540,7 @@ typedef struct rce_qmm_heads {
  * head x becomes x / sqrt(mean x^2 + eps) * weight (eps below 0: no norm, no weight), its first
  * rope->dim values then turn by the row's position (rope NULL: not), pairs (i, i + dim / 2) or,
  * `interleaved` not 0, (2 i, 2 i + 1); f32, one rounding to out_dtype.  The sum of
- * squares has to fit binary32.
+ * squares must not pass binary32; values of any smallness are held.
  * q, k: either may be NULL or have no heads; d_head even, 2 to 1024, any other
  * alignment than that of the values; in_dtype and out_dtype F32, F16 or BF16.  out may be in
  * (one type size, one stride); other overlaps are not allowed.  Of the batch only

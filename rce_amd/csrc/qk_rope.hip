@@ -70,6 +70,11 @@ __device__ __forceinline__ int position_of(const QkNormRope &A, int r) {
     return r >= q.r0 && r < q.r1 && (!A.rope.cs || pos < A.n_pos) ? pos : -1;
 }
 
+// A head whose mean square and eps together are below TINY: its squares leave binary32's normal numbers, and the root's reciprocal
+// takes a subnormal number for 0.  Its values are times TINY_UP first, eps times that twice, which cancels: values below 2^-45 come
+// to less than 2^59, a head's squares to less than 2^118, and the least subnormal value's square to 2^-90.
+constexpr float TINY = 0x1p-100f, TINY_UP = 0x1p104f;
+
 template <class T>
 struct alignas(16) Piece {
     T t[8];
@@ -122,7 +127,20 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope(QkNormRope A, int lanes, i
 #pragma unroll
             for (int i = 0; i < 8; i++) s = __builtin_fmaf(x[e][i], x[e][i], s);
         s = sum_over(is ? s : 0.0f, lanes);
-        const float f = __builtin_amdgcn_rsqf(s * (1.0f / (float)A.d) + A.eps);
+        float m = s * (1.0f / (float)A.d) + A.eps;
+        if (__ballot(m < TINY)) {
+            const float up = m < TINY ? TINY_UP : 1.0f;
+            s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[e][i] *= up;
+                    s = __builtin_fmaf(x[e][i], x[e][i], s);
+                }
+            m = sum_over(is ? s : 0.0f, lanes) * (1.0f / (float)A.d) + A.eps * up * up;
+        }
+        const float f = __builtin_amdgcn_rsqf(m);
         float y[2][8];
 #pragma unroll
         for (int i = 0; i < 8; i++) y[0][i] = y[1][i] = 1.0f;
@@ -209,7 +227,21 @@ __global__ __launch_bounds__(256) void k_qk_norm_rope_any(QkNormRope A) {
         b[j] = is ? widen(in[second(p)]) : 0.0f;
         s = __builtin_fmaf(b[j], b[j], __builtin_fmaf(a[j], a[j], s));
     }
-    const float f = A.eps >= 0.0f ? __builtin_amdgcn_rsqf(sum_over(s, 64) * (1.0f / (float)A.d) + A.eps) : 1.0f;
+    float f = 1.0f;
+    if (A.eps >= 0.0f) {
+        float m = sum_over(s, 64) * (1.0f / (float)A.d) + A.eps;
+        if (m < TINY) {  // the same in all lanes
+            s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                a[j] *= TINY_UP;
+                b[j] *= TINY_UP;
+                s = __builtin_fmaf(b[j], b[j], __builtin_fmaf(a[j], a[j], s));
+            }
+            m = sum_over(s, 64) * (1.0f / (float)A.d) + A.eps * TINY_UP * TINY_UP;
+        }
+        f = __builtin_amdgcn_rsqf(m);
+    }
 #pragma unroll
     for (int j = 0; j < J; j++) {
         const int p = lane + 64 * j;

@@ -176,6 +176,49 @@ def test_small_and_large(ctx, size):
     case(ctx, 7, [30], [30], 2, 2, 64, G.F32, G.F32, rope=64, size=size, eps=1e-30 if size < 1 else 1e-6)
 
 
+@pytest.mark.parametrize("d,rope", [(16, 16), (64, 64), (192, 64), (1024, 0), (66, 66), (130, 0)])
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-42])
+@pytest.mark.parametrize("it", [G.F32, G.BF16])
+def test_mean_squares_below_binary32(ctx, d, rope, eps, it):
+    """Heads whose mean square, or every square, is a subnormal number or none of binary32, between heads of ordinary
+    size, and heads of subnormal values.  (The smallest are 0 in BF16: 0 / 0 without an eps.)"""
+    c = Call(ctx, np.random.default_rng(d), [40], [40], 5, 3, d, it, G.F32, rope=rope, eps=eps)
+    sizes = np.array([1, 1e-18, 1e-19, 1e-20, 3e-16, 1e-23, 1e-30, 1e-37, 1e-39, 1e-41])
+    x = kc.widen(c.bits, it).astype(np.float64)
+    heads = x[:, :8 * d].reshape(c.rows, 8, d)
+    heads *= sizes[np.arange(c.rows * 8).reshape(c.rows, 8) % len(sizes)][..., None]
+    c.bits = kc.to_bits(x.astype(F32), it)
+    c.x.upload(c.bits.ravel())
+    c.run()
+    ctx.synchronize()
+    half, tiny = sc.half_step(G.F32)
+    for i in range(2):
+        o, _ = c.got(i)
+        for r, (y, b) in c.want(i).items():
+            nothing = np.isnan(y).all(1)
+            assert eps == 0 or not nothing.any()
+            assert np.isnan(o[r][nothing]).all()
+            with np.errstate(invalid="ignore"):
+                err = np.abs(o[r].astype(np.float64) - y)
+            assert np.all((err <= b + half * (np.abs(y) + b) + tiny)[~nothing]), (r, i)
+    c.free()
+
+
+@pytest.mark.parametrize("d", [64, 66])
+@pytest.mark.parametrize("eps", [1e-38, 1e-42])
+def test_zeros_with_a_small_eps(ctx, d, eps):
+    c = Call(ctx, np.random.default_rng(d), [6], [6], 3, 1, d, G.F32, G.F32, rope=64, eps=eps)
+    bits = c.bits.copy()
+    bits[::2, :3 * d] = 0
+    c.bits = bits
+    c.x.upload(bits.ravel())
+    c.run()
+    ctx.synchronize()
+    c.compare()
+    assert np.all(c.got(0)[0][::2] == 0)
+    c.free()
+
+
 def test_zeros_and_what_is_not_finite(ctx):
     """A head of zeros stays zeros; a NaN or infinity spoils its own head alone."""
     c = Call(ctx, np.random.default_rng(8), [6], [6], 3, 1, 64, G.F32, G.F32, rope=64)
