@@ -708,7 +708,7 @@ __global__ __launch_bounds__(64 * WAVES, D * LIMBS <= 256 ? 3 : D <= 192 ? 2 : 1
 // the LDS reads per product).
 constexpr int P_ROWS = 128, P_WAVES = 8;
 constexpr float LAG = 6.0f, UP = 512.0f;  // UP = 2^9
-constexpr int UNSEEN = -(1 << 30);  // scores of two limbs are above -2^30 (256 dimensions: 256 * 127 * 2^14)
+constexpr int UNSEEN = -(1 << 30);  // below all scores of two limbs: at 256 dimensions they reach 256 * 128 * 127 * 256, 0.8 % less
 
 // A lane's accumulators times f: four consecutive values every 16 from value index i; vec:
 // at multiples of their size.
@@ -758,6 +758,7 @@ __global__ __launch_bounds__(64 * P_WAVES, D <= 128 ? (HILO ? 3 : 4) : 2) void k
     constexpr int NQ = D / 64, NT = D / 16;
     constexpr int LIMBS = HILO ? 3 : 2;
     constexpr bool QUICK = SINKS && !HILO;
+    static_assert(!QUICK || (int64_t)D * 128 * 127 * 256 < -(int64_t)UNSEEN, "codes of 128, queries of 127 * 256");
     constexpr float lag = QUICK ? 0.0f : LAG;  // QUICK comes to the maximum only where m was too low
     constexpr int NK = (TILE * D + 16 * 64 * P_WAVES - 1) / (16 * 64 * P_WAVES);  // 16-byte pieces of codes a thread moves
     constexpr int BUFS = D <= 128 ? 2 : 1;  // two where they fit 64 KB

@@ -185,6 +185,94 @@ def test_no_sinks_is_the_window_alone(ctx):
         r.free()
 
 
+def per_key(pool, batch, q, scale, window, sinks, f32_out, row):
+    """(out, bound) [n_q, d] of a row, the bound from each key's own error.
+
+    A key's weight is w_j (1 + a_j), |a_j| <= h_j = e^(s_j) - 1: s_j holds the score's error -- the query's whole numbers', 0.51 steps of two
+    limbs and one step of three (the f32 product in front of the rounding has steps of a half there), times scale sum|k_j|, and
+    2^-21 |score| for some eight roundings of its factors -- and 2^-21 for the exponential and the products after it.  A rescale by e^(m - m'),
+    at most one a tile, adds 2^-22 and 2^-24 of the difference; the differences add up to twice the largest score at most.  With
+    a_ the mean of a, out' - out = sum w_j a_j (v_j - out) / (1 + a_).  The products' weights alone are rounded to binary16
+    (2^-11; two terms, 2^-20 with the factors' roundings), or in its steps of 2^-24 below 2^-14: 2^-25 of 512 for the
+    largest scale, 2^-34 max |v| a key; sums of n terms add n 2^-23."""
+    n_q, d = q.shape
+    qmax = 127.0 * (65536 if f32_out else 256)
+    s = int(np.searchsorted(batch.offsets, row, side="right")) - 1
+    pos = batch.lens[s] - (int(batch.offsets[s + 1]) - row)
+    j = np.arange(pos + 1)
+    j = j[(j > pos - window) | (j < sinks)]
+    g = batch.pages[s, j // pool.page]
+    b, i = j % pool.page // kc.BLOCK, j % kc.BLOCK
+    K = pool.k[g, :, b, i].astype(np.float64) * pool.k_scale[g, :, b].astype(np.float64)[..., None]
+    V = pool.v[g, :, b, :, i].astype(np.float64) * pool.v_scale[g, :, b].astype(np.float64)[..., None]
+    out, bound = np.zeros((n_q, d)), np.zeros((n_q, d))
+    for h in range(n_q):
+        k, v, x = K[:, h // (n_q // pool.heads)], V[:, h // (n_q // pool.heads)], q[h].astype(np.float64)
+        sc = k @ x * scale
+        w = np.exp(sc - sc.max())
+        w /= w.sum()
+        out[h] = w @ v
+        step = np.abs(x).max() / qmax
+        e = scale * np.abs(k).sum(1) * step * (1.0 if f32_out else 0.51) + 2.0 ** -21 * np.abs(sc) + 2.0 ** -21
+        e += (len(j) / 64 + 2) * 2.0 ** -22 + 2.0 ** -23 * np.abs(sc).max()
+        eta = np.expm1(e)
+        mean = w @ eta
+        assert mean < 0.5
+        bound[h] = (w * eta) @ np.abs(v - out[h]) / (1 - mean)
+        bound[h] += ((2.0 ** -20 if f32_out else 2.0 ** -11) + len(j) * 2.0 ** -23) * (w @ np.abs(v)) * (1 + 2 * mean)
+        bound[h] += 2.0 ** -34 * len(j) * np.abs(v).max()
+    return out, bound
+
+
+@pytest.mark.parametrize("d,it,ot", [(64, G.F16, G.F16), (128, G.BF16, G.BF16), (128, G.F32, G.F16), (256, G.F32, G.F16), (256, G.F16, G.F32),
+                                     (64, G.F32, G.F32)])
+@pytest.mark.parametrize("how", ["grow", "fall", "apart", "few"])
+@pytest.mark.parametrize("news", [1, 7, 290])
+def test_scores_that_move_by_each_keys_error(ctx, d, it, ot, how, news):
+    """Blocks of keys whose scores grow or fall along the row, or lie apart at random, within bounds that results of a wrong weight or a
+    rescale left out do not keep: most are a few roundings of the result."""
+    print(f"sinks moving by key {how} new={news} d={d} {it}->{ot}", flush=True)
+
+    def edit(pool, batch):
+        rng = np.random.default_rng(d)
+        for s, length in enumerate(batch.lens):
+            blocks = -(-length // 16)
+            for blk in range(blocks):
+                at = batch.pages[s, blk * 16 // pool.page], slice(None), blk % pool.b
+                part = blk / blocks
+                f = {"grow": 10.0 ** (2 * part - 1), "fall": 10.0 ** (1 - 2 * part), "apart": rng.choice([0.1, 1, 10]),
+                     "few": rng.choice([0, 0.3, 1, 3])}[how]
+                pool.k_scale[at] *= F32(f)
+    r = Run(ctx, np.random.default_rng(d + news), [700, 290], [news, news], 32, 1, 2, d, it, ot, edit=edit)
+    window, sinks = 330, 20
+    r.ob.upload(r.blank)
+    r.call(window, sinks)
+    ctx.synchronize()
+    o = kc.widen(r.out(), ot).astype(np.float64)
+    x = kc.widen(r.q, it)[:, :r.n_q * d].reshape(-1, r.n_q, d)
+    eps, step = kc.out_eps(ot), 2.0 ** -25 if ot == G.F16 else 0.0
+    for row in sorted({0, news // 3, news // 2, news - 1, news, news + news // 2, 2 * news - 1}):
+        y, b = per_key(r.pool, r.batch, x[row], r.scale, window, sinks, ot == G.F32, row)
+        err = np.abs(o[row] - y)
+        assert np.all(err <= b + np.maximum(eps * (np.abs(y) + b), step)), (row, float(np.max(err / b)))
+    r.free()
+
+
+def test_a_window_alone_against_64_bits(ctx):
+    """Both entry points without sinks, or without a window, each on cleared results and within the bound."""
+    rng = np.random.default_rng(3)
+    for news in (1, 9, 200):
+        r = Run(ctx, rng, [1500, 300], [news, news], 32, 2, 4, 64, G.F16, G.F16, rope=64)
+        for window, sinks in ((100, 0), (0, 0), (0, 50)):
+            r.check(window, sinks, rows={0, news - 1, news, 2 * news - 1})
+            a = r.out()
+            r.ob.upload(r.blank)
+            rce_amd.kv_attention_dev(ctx, r.dev.cache, r.dev.b, r.qb.ptr, r.it, r.q_stride, r.n_q, r.ob.ptr, r.ot, r.scale, rope=r.dev.rope, window=window)
+            ctx.synchronize()
+            assert np.array_equal(a.view(np.uint8), r.out().view(np.uint8))
+        r.free()
+
+
 @pytest.mark.parametrize("ot", [G.F32, G.F16])
 @pytest.mark.parametrize("news", [1, 4, 60])
 def test_split_ranges(ctx, news, ot):
