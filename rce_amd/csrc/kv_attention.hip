@@ -81,7 +81,10 @@ constexpr int LONG = 1536, LONG_TILES = 48;
 
 // With sinks no unit visits more tiles than a window's.  Up to SHORT of them a few sequences have one part (a long one is there: units of few rows
 // take no longer than its), and units that are TARGET and more are not split: 3 x 500 rows after 9000, a window of 2048: 117 -> 104 us.
-constexpr int SHORT = 64;
+// Two parts : one (us, f16, 32 / 8 heads of 128, a window of 1024 where none is named): 3 x 500 rows, 2048 96.4 : 88.4; 16 x 20 rows 39.9 : 33.8;
+// 15 single tokens and 1000 rows 58.6 : 51.0, and 4000 121 : 117, and 500 with 3000 89.6 : 86.8; 15 x 4 and 2000 rows, 2048 118.9 : 120.5.
+// Of more than SHORT_SEQS sequences one part measured no worse either (31 single tokens and 1000 rows 61.4 : 48, 24 x 300 199 : 190).
+constexpr int SHORT = 64, SHORT_SEQS = 16;
 // Tiles of the shortest range of few rows there, and beyond.  In ranges of 8 : of 4 (us, whole calls): one row, window 1024, 4 kv heads of 64,
 // f32 14.5 : 13.2; window 1500, 8 of 128 17.9 : 15.7; 8 rows, window 1024 20.4 : 19.8; one row, window 8192 21.1 : 22.4.
 constexpr int SHORT_CHUNK = 4;
@@ -1219,7 +1222,7 @@ hipError_t launch_kv_attention(const KvPool &pool, const KvRows &rows, int d_hea
         const bool prompt = more >= (size_t)LONG &&
                             (double)more / ROWS * (span / TILE) * pool.heads >= (double)LONG_TILES * TARGET;
         if (x > (size_t)FEW * rows.n_seqs || prompt) {
-            const bool one = (rows.n_seqs == 1 && span <= ONE_TABLE * TILE) || (SINKS && rows.n_seqs <= 16 && span <= SHORT * TILE);
+            const bool one = (rows.n_seqs == 1 && span <= ONE_TABLE * TILE) || (SINKS && rows.n_seqs <= SHORT_SEQS && span <= SHORT * TILE);
             many(one ? 0 : FEW + 1);
             if (!one) few(FEW);
         } else {

@@ -62,7 +62,9 @@ __global__ __launch_bounds__(256) void k_kv_release(KvTable t, int page_tokens, 
 // step, and count on the pages' own counts: an item that asks takes one off; where that leaves none, the least item number - CODE that is
 // written there keeps the page.
 //
-// What bounds it: the chain of loads (lengths, entries, counts), barriers of 16 waves.
+// What bounds it: the chain of loads (lengths, entries, counts), barriers of 16 waves.  Behind the first AHEAD looks each look for free pages is a
+// load and two barriers more, 1 us for 4096 counts: 64 tokens that each need a page, with the free ones at the pool's end: 4.0 us in a pool of 16384 pages,
+// 16 of 65536, 64 of 262144, 256 of 2^20.
 constexpr int PLAN = 1024;       // threads
 constexpr int CODE = 1 << 30;    // items are fewer than 2^24
 constexpr int EACH = 4;          // counts that a thread looks at for free pages, and items of a thread's step
@@ -514,7 +516,10 @@ __global__ __launch_bounds__(PLAN) void k_kv_compact(KvRefs R, int32_t *new_ids,
 
 dim3 over_entries(const KvTable &t) { return dim3((unsigned)((t.entries() + 255) / 256)); }
 constexpr size_t OWN_COPY = (size_t)128 << 10;  // bytes that the planning block copies itself: 4 beams of 4 heads of 64, whole pass with fork and release 17.1 -> 13.8 us
-constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256, FRONT_BLOCKS = 2048;
+constexpr size_t COPY_BLOCKS = 4096, RENAME_BLOCKS = 256;
+// Whole reservations with blocks of up to 256 : 512 : 1024 : 2048 : 4096 for the fronts (us, 8 heads of 128, half a page of 128 positions each): 128 fronts
+// 13.9 : 10.3 : 8.7 : 8.9 : 9.2, 512 fronts 51 : 33 : 24 : 21 : 20; with nothing to copy the launch costs 2 us of 7, whatever their number.
+constexpr size_t FRONT_BLOCKS = 2048;
 
 void copy_pages(const KvPool &from, const KvPool &to, int d_head, const int32_t *src, const int32_t *dst, const int32_t *count, int n,
                 const KvTable &t, const int32_t *new_ids, hipStream_t s) {

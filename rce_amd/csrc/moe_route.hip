@@ -664,8 +664,11 @@ __global__ __launch_bounds__(256) void k_moe_route_fours(Routing A, int group_la
     finish<16>(A, is, at, row, sub, id, top, total);
 }
 
-// From so many tokens on four share a wave.  A wave per token : four (us, whole calls), 256 experts in groups with a bias: 4096 tokens 10.2 : 11.6,
-// 8192 15.6 : 12.7, 16384 23.8 : 16.0; 128 experts, logits alone: 8192 tokens 7.1 : 8.0, 32768 20.0 : 13.8.
+// From so many tokens on four share a wave.  A wave per token : four (us, whole calls, f32 logits):
+//   256 experts, 8 groups that count by two, a bias: 2048 tokens 6.8 : 14.9, 4096 12.1 : 11.0, 6000 11.4 : 11.1, 8192 15.4 : 12.2, 16384 23.3 : 15.9;
+//   64 experts, 8 groups that count by two, a bias: 2048 5.5 : 6.6, 4096 8.2 : 6.8, 6000 8.3 : 6.9, 16384 16.5 : 7.8;
+//   logits alone, 64 experts in 8 groups: 6000 7.0 : 7.4, 8192 8.4 : 9.4, 10000 9.7 : 7.7, 16384 13.5 : 8.6; 32 in 4: 6000 6.1 : 6.5, 10000 8.3 : 7.1;
+//   128 experts without groups: 8192 6.8 : 8.9, 10000 7.9 : 7.5, 16384 11.0 : 9.1.
 constexpr int FOURS_FROM = 6000, FOURS_FROM_PLAIN = 10000;
 
 }  // namespace

@@ -9,7 +9,8 @@
 // A lane holds two pieces of 8 values (16 or 32 bytes each), d / 16 lanes a
 // head.  Where pairs are (i, i + half) the pieces are `half` values apart, so
 // that no value of a pair is another lane's.  What does not fit that (heads not
-// of 16 values, rotated parts not of 16, addresses not of 16 bytes) goes value by value.
+// of 16 values, rotated parts not of 16, addresses not of 16 bytes) goes value by value,
+// a wave to a head: 40 heads of 80, f16, 5 x up to 2500 rows with 20 values of each rotated as halves take 112 us, with all 80 (by pieces) 22.
 #include "qk_rope.h"
 
 #include <algorithm>
